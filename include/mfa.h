@@ -14,7 +14,7 @@
  *   s  = softcap * tanh(s / softcap)              if softcap > 0
  *   s -= alibi[b*Hq + h] * |center - j|           if alibi != NULL
  *   masked (-inf) unless kmin <= j < kmax, with center = i + (Lk - Lq) (bottom-right),
- *     causal: j <= center; win_left >= 0: j >= center - win_left;
+ *     causal: j <= center; win_left >= 0: j >= center - win_left or j < sink;
  *     win_right >= 0: j <= center + win_right
  *   o  = softmax(s) @ v ; a row with no unmasked key is 0 (nan_to_num, _kernel.py:1206)
  * GQA/MQA: query head h reads kv head h / (Hq / Hkv).
@@ -33,7 +33,7 @@
 extern "C" {
 #endif
 
-#define MFA_ABI_VERSION 8
+#define MFA_ABI_VERSION 9
 
 /* Status codes. The Python layer maps them to the reference's exception types. */
 enum mfa_status {
@@ -101,6 +101,10 @@ typedef struct mfa_fwd_params {
    * exactly the CTAs the sequences need, longest sequence first, instead of max_lq's row
    * blocks for every sequence with the surplus CTAs exiting at once. */
   const int32_t* cu_q_host;
+  /* First keys that stay visible: with win_left >= 0 a row also sees the keys j < sink left of
+   * its window (global positions; the causal and right limits hold for them too). 0 = none; no
+   * counterpart in the reference. */
+  int32_t sink;
 } mfa_fwd_params;
 
 /* Attention forward. Replaces the tier dispatch under flash_attn_forward

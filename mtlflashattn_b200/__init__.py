@@ -12,7 +12,8 @@ import math
 
 import torch
 
-from ._kernel import MAX_HEAD_DIM, _BiasParams, _broadcast_alibi_slopes, flash_attn_forward
+from ._kernel import (MAX_HEAD_DIM, _BiasParams, _broadcast_alibi_slopes, _check_sink,
+                      flash_attn_forward)
 from . import _kernel
 from ._version import __version__
 from .host import flash_attn_host, flash_attn_varlen_host
@@ -102,15 +103,21 @@ def flash_attn_func(
     alibi_slopes=None,
     deterministic=False,
     return_attn_probs=False,
+    sink_tokens=0,
 ):
     """Drop-in for flash_attn.flash_attn_func (forward only).
 
     q: [B, Lq, Hq, D]; k, v: [B, Lk, Hkv, D]. Hkv must divide Hq (GQA/MQA).
     Returns [B, Lq, Hq, D] in q.dtype (reference: metal_flash_attn/__init__.py:62-99; the
     output is written in place in this layout, so no transpose copy follows the kernel).
+
+    sink_tokens (no counterpart there): the first ``sink_tokens`` keys stay visible to every row
+    whatever the left side of ``window_size`` hides; the causal and right limits hold for them
+    too. Without a left window it changes nothing.
     """
     _check_supported(q, k, v, dropout_p, window_size, softcap, alibi_slopes,
                      deterministic, return_attn_probs)
+    sink = _check_sink(sink_tokens)
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
         raise ValueError(f"mtlflashattn_b200: expected 4-D [B,S,H,D] tensors, got q.dim()={q.dim()}")
     Hq, Hkv = q.shape[2], k.shape[2]
@@ -123,7 +130,7 @@ def flash_attn_func(
     B, Lq = q.shape[0], q.shape[1]
     alibi = (_broadcast_alibi_slopes(alibi_slopes, B, Hq, q.device)
              if alibi_slopes is not None else None)
-    bias = _BiasParams(softcap, window_size[0], window_size[1], alibi)
+    bias = _BiasParams(softcap, window_size[0], window_size[1], alibi, sink)
     out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
     # the kernel reads raw pointers: no autograd graph is recorded, so no detach is needed
     _kernel.forward_bshd(q, k, v, out, scale, causal, bias)
@@ -147,6 +154,7 @@ def flash_attn_varlen_func(
     deterministic=False,
     return_attn_probs=False,
     block_table=None,
+    sink_tokens=0,
 ):
     """Drop-in for flash_attn.flash_attn_varlen_func (forward only).
 
@@ -155,10 +163,11 @@ def flash_attn_varlen_func(
     Checks and errors follow the reference (metal_flash_attn/__init__.py:102-183), including
     its host read of cu_seqlens; all sequences then run in one launch. ``max_seqlen_*`` are
     accepted and, as in the reference, not trusted: the launch uses the lengths read from
-    cu_seqlens.
+    cu_seqlens. ``sink_tokens`` as in ``flash_attn_func``, for each sequence's own first keys.
     """
     _check_supported(q, k, v, dropout_p, window_size, softcap, alibi_slopes,
                      deterministic, return_attn_probs)
+    sink = _check_sink(sink_tokens)
     if block_table is not None:
         raise NotImplementedError("mtlflashattn_b200: block_table (paged KV cache) not supported")
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
@@ -200,7 +209,7 @@ def flash_attn_varlen_func(
     if alibi_slopes is not None:
         # the reference applies [Hq] slopes per sequence (each a B=1 call), [batch, Hq] by row
         alibi = _broadcast_alibi_slopes(alibi_slopes, batch, Hq, q.device)
-    bias = _BiasParams(softcap, window_size[0], window_size[1], alibi)
+    bias = _BiasParams(softcap, window_size[0], window_size[1], alibi, sink)
     cu_q_dev = _as_cu(cu_seqlens_q, q.device)
     cu_k_dev = _as_cu(cu_seqlens_k, q.device)
     _kernel.forward_varlen(q, k, v, out, cu_q_dev, cu_k_dev, max(lens_q), max(lens_k), scale,

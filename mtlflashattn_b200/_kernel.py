@@ -34,8 +34,10 @@ from . import _lib
 MAX_HEAD_DIM = 128
 
 # Bias/masking knobs, as in the reference (_kernel.py:20-24): softcap (0 = off),
-# window_left/window_right (-1 = open), alibi: [B*Hq] fp32 slopes already broadcast, or None.
-_BiasParams = namedtuple("_BiasParams", "softcap window_left window_right alibi")
+# window_left/window_right (-1 = open), alibi: [B*Hq] fp32 slopes already broadcast, or None;
+# and sink: how many first keys stay visible left of the window (no counterpart there).
+_BiasParams = namedtuple("_BiasParams", "softcap window_left window_right alibi sink",
+                         defaults=(0,))
 
 _DTYPES = {torch.float16: _lib.FP16, torch.bfloat16: _lib.BF16, torch.float32: _lib.FP32}
 
@@ -175,6 +177,13 @@ def _broadcast_alibi_slopes(alibi_slopes, B, Hq, device):
     return s.reshape(-1).contiguous()
 
 
+def _check_sink(sink_tokens):
+    """The validated number of first keys that stay visible, as the int32 libmfa takes."""
+    if not isinstance(sink_tokens, int) or isinstance(sink_tokens, bool) or sink_tokens < 0:
+        raise ValueError("mtlflashattn_b200: sink_tokens must be an int >= 0 (0 = none)")
+    return min(sink_tokens, 2**31 - 1)
+
+
 def _last_dim_contig(t):
     return t if t.stride(-1) == 1 else t.contiguous()
 
@@ -206,7 +215,7 @@ def _values(q, k, v, o, B, Hq, Hkv, Lq, Lk, D, q_st, k_st, v_st, o_st, scale, ca
             int(bias.window_left), int(bias.window_right),
             bias.alibi.data_ptr() if bias.alibi is not None else 0,
             _DTYPES[q.dtype], _DTYPES[o.dtype], int(k_pos_offset), int(lk_total), kernel,
-            _err_word(q.device).data_ptr(), 0, 0, cu_q_host)
+            _err_word(q.device).data_ptr(), 0, 0, cu_q_host, bias.sink)
 
 
 def _params(q, k, v, o, *, B, Hq, Hkv, Lq, Lk, D, q_st, k_st, v_st, o_st, scale, causal,
@@ -250,7 +259,10 @@ def _workspace(dev, stream, need):
     demand and reused by every later call. Work on one stream runs in order, so a call never
     overwrites partials an earlier call still reads; a replaced buffer goes back to torch's
     caching allocator, which keeps it until the work queued on its stream is done. Saves a
-    torch.empty per decode-sized call."""
+    torch.empty per decode-sized call. A call that is being captured takes a buffer of its own
+    from the graph's pool: two graphs captured on one stream may be replayed on two."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(need, dtype=torch.uint8, device=dev)
     key = (dev, stream)
     ws = _workspaces.get(key)
     if ws is None or ws.numel() < need:
@@ -353,18 +365,20 @@ def forward_varlen(q, k, v, out, cu_q, cu_k, max_lq, max_lk, scale, causal, bias
 
 
 def flash_attn_forward(q, k, v, scale, causal, softcap=0.0, window_left=-1, window_right=-1,
-                       alibi_slopes=None):
-    """q: [B,Hq,Lq,D], k/v: [B,Hkv,Lk,D] (heads-second, any strides).
+                       alibi_slopes=None, sink_tokens=0):
+    """q: [B,Hq,Lq,D], k/v: [B,Hkv,Lk,D] (heads-second, any strides). ``sink_tokens`` as in
+    ``flash_attn_func``.
 
     Returns [B,Hq,Lq,D] contiguous, in q.dtype (reference: _kernel.py:1052-1153).
     """
     if softcap < 0:
         raise ValueError("mtlflashattn_b200: softcap must be >= 0 (0 disables capping)")
+    sink = _check_sink(sink_tokens)
     _check_tensors(q, k, v)
     B, Hq, Lq, D = q.shape
     alibi = (_broadcast_alibi_slopes(alibi_slopes, B, Hq, q.device)
              if alibi_slopes is not None else None)
-    bias = _BiasParams(softcap, window_left, window_right, alibi)
+    bias = _BiasParams(softcap, window_left, window_right, alibi, sink)
     out = torch.empty(B, Hq, Lq, D, device=q.device, dtype=q.dtype)
     forward_bshd(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), out.transpose(1, 2),
                  scale, causal, bias)

@@ -11,6 +11,7 @@ import shutil
 import subprocess
 import sys
 import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 OUT = os.path.join(HERE, "libmfa.so")
@@ -46,6 +47,7 @@ def up_to_date() -> bool:
 # path and is compiled with IEEE division / square root, accurate expf / tanhf / logf and no
 # flush to zero.
 UNITS = (("mfa_api.cu", ["--use_fast_math"]),
+         ("sink_fwd.cu", ["--use_fast_math"]),
          ("simt_fwd.cu", ["-ftz=false", "-prec-div=true", "-prec-sqrt=true"]))
 
 
@@ -62,14 +64,19 @@ def build(verbose: bool = False, force: bool = False, defines=(), out: str | Non
     objs = []
     logs = []
     with tempfile.TemporaryDirectory() as tmp:
-        for src, flags in UNITS:
+        def compile_unit(unit):
+            src, flags = unit
             obj = os.path.join(tmp, src + ".o")
-            r = subprocess.run([*base, *flags, "-c", "-o", obj, os.path.join(HERE, "csrc", src)],
-                               capture_output=True, text=True)
-            if r.returncode != 0:
-                raise RuntimeError(f"nvcc failed on {src}:\n" + r.stdout + r.stderr)
-            logs.append(r.stdout + r.stderr)
-            objs.append(obj)
+            return src, obj, subprocess.run(
+                [*base, *flags, "-c", "-o", obj, os.path.join(HERE, "csrc", src)],
+                capture_output=True, text=True)
+
+        with ThreadPoolExecutor(len(UNITS)) as pool:  # one nvcc process per unit
+            for src, obj, r in pool.map(compile_unit, UNITS):
+                if r.returncode != 0:
+                    raise RuntimeError(f"nvcc failed on {src}:\n" + r.stdout + r.stderr)
+                logs.append(r.stdout + r.stderr)
+                objs.append(obj)
         r = subprocess.run([nvcc_path(), *ARCH, "-shared", "-o", target + ".tmp", *objs],
                            capture_output=True, text=True)
         if r.returncode != 0:

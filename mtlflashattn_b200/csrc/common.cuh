@@ -36,6 +36,7 @@ struct FwdArgs {
   int max_lq;
   float scale, softcap;
   int causal, wl, wr;
+  int sink;  // the first `sink` keys (global positions) stay visible left of the window
   const float* alibi;
   int o_dtype;  // 0 fp16, 1 bf16, 2 fp32
   int o_vec16;  // 1 if every output row segment is 16-byte aligned (vector stores allowed)
@@ -105,8 +106,9 @@ __device__ __forceinline__ SeqView seq_view(const FwdArgs& a, int b) {
 // Local key interval [lo, hi) that row i of a sequence may attend (bottom-right aligned causal
 // and sliding window, restricted to the local keys [0, lk)). Rule of _flash_torch
 // (metal_flash_attn/_kernel.py:1196-1203) and of the v0 kernel's kmin/kmax (_kernel.py:59-64).
+// sk: the row also sees the keys [0, min(sk, lo)) left of its window (a.sink; 0 when unused).
 struct KeyRange {
-  int lo, hi;
+  int lo, hi, sk;
 };
 __device__ __forceinline__ KeyRange key_range(const FwdArgs& a, const SeqView& s, int64_t i) {
   const int64_t centre = i + s.off;
@@ -121,6 +123,8 @@ __device__ __forceinline__ KeyRange key_range(const FwdArgs& a, const SeqView& s
   KeyRange r;
   r.lo = static_cast<int>(lo > s.lk ? s.lk : lo);
   r.hi = static_cast<int>(hi < 0 ? 0 : hi);
+  const int64_t sk = (int64_t)a.sink - a.k_pos_offset;
+  r.sk = static_cast<int>(sk < 0 ? 0 : sk > r.hi ? r.hi : sk);
   return r;
 }
 

@@ -83,7 +83,15 @@ __global__ void __launch_bounds__(simt::kThreads) fa_fwd_simt(const __grid_const
 #pragma unroll
   for (int c = 0; c < NC; ++c) acc[c] = 0.f;
 
-  for (int kb0 = (khi > klo ? (klo / BN) * BN : khi); kb0 < khi; kb0 += BN) {
+  // the window's key blocks, and before them those of the first keys that stay visible
+  const int kw0 = khi > klo ? (klo / BN) * BN : (klo + BN - 1) / BN * BN;
+  const int sk_last = min(key_range(a, sv, r_last).sk, kw0);
+  const int kend = khi > klo ? khi : sk_last;
+  for (int kb0 = sk_last > 0 ? 0 : kw0; kb0 < kend; kb0 += BN) {
+    if (kb0 >= sk_last && kb0 < kw0) {
+      kb0 = kw0;
+      if (kb0 >= kend) break;
+    }
     __syncthreads();
     for (int e = tid; e < BN * DP; e += kThreads) {
       const int kk = e / DP, d = e % DP;
@@ -110,7 +118,7 @@ __global__ void __launch_bounds__(simt::kThreads) fa_fwd_simt(const __grid_const
       if (a.softcap > 0.f) val = a.softcap * tanhf(val / a.softcap);
       const int key = kb0 + kk;
       if (a.alibi != nullptr) val -= slope * fabsf(centre - (float)(key + a.k_pos_offset));
-      s[i] = (key >= kr.lo && key < kr.hi) ? val : -INFINITY;
+      s[i] = ((key >= kr.lo || key < kr.sk) && key < kr.hi) ? val : -INFINITY;
       mx = fmaxf(mx, s[i]);
     }
 #pragma unroll

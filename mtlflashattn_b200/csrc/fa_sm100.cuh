@@ -261,8 +261,11 @@ __device__ __forceinline__ void named_barrier(int id, int threads) {
 
 // kPack: the row mapping of decode-like launches (query heads packed per KV head, one-tile CTAs);
 // the other instantiations fold pack_shift to 0 at compile time.
+// kSink: the first a.sink keys stay visible left of the sliding window. The CTA then walks two runs
+// of key blocks, those that hold such keys below the window's first block and the window's own;
+// the instantiations without it keep one run and one comparison per masked score.
 template <int DP, bool kBF16, int kBias, int CG = DefaultCG<kBias, DP>::value,
-          int TILES = DefaultTiles<DP, CG, kBias>::value, bool kPack = false,
+          int TILES = DefaultTiles<DP, CG, kBias>::value, bool kPack = false, bool kSink = false,
           int kEmu = (kBias == 2 ? MFA_EMU_SOFTCAP
                                  : DP == 64 ? (TILES == 1 ? MFA_EMU64 : 0) : MFA_EMU128),
           int kHalfExp = (kBias == 0 ? (DP == 64 ? MFA_HALF_EXP64 : MFA_HALF_EXP128) : 0)>
@@ -360,8 +363,25 @@ __global__ void __launch_bounds__(sm100::Roles<CG, TILES>::kThreads,
     klo = max(klo, split * a.split_keys);
     if (split + 1 < a.num_splits) khi = min(khi, (split + 1) * a.split_keys);
   }
-  const int jb = klo / KBN;
-  const int n = khi > klo ? (khi + KBN - 1) / KBN - jb : 0;
+  int jb = klo / KBN;
+  int n = khi > klo ? (khi + KBN - 1) / KBN - jb : 0;
+  // blocks [sb0, sb0 + nsb) hold first keys that stay visible, all below block jb
+  int sb0 = 0, nsb = 0;
+  if constexpr (kSink) {
+    if (n == 0) jb = (klo + KBN - 1) / KBN;
+    int sk = key_range(a, sv, r_last >> ps).sk;  // nondecreasing in the position, as hi is
+    if (a.num_splits > 1) {
+      sb0 = split * (a.split_keys / KBN);  // a split is a whole number of blocks
+      if (split + 1 < a.num_splits) sk = min(sk, (split + 1) * a.split_keys);
+    }
+    nsb = max(0, min((sk + KBN - 1) / KBN, jb) - sb0);
+    n += nsb;
+  }
+  // the j-th key block of this CTA
+  auto block_at = [&](int j) {
+    if constexpr (kSink) return j < nsb ? sb0 + j : jb + j - nsb;
+    else return jb + j;
+  };
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -433,7 +453,7 @@ __global__ void __launch_bounds__(sm100::Roles<CG, TILES>::kThreads,
         bool ok = mbar_wait(&kv_empty[slot], ph ^ 1u, abort_flag);
         if (!__all_sync(kFull, ok)) break;
         if (lane == 0) {
-          const int j = jb + (it >> 1);
+          const int j = block_at(it >> 1);
           const CUtensorMap* m = (it & 1) ? &args.tv : &args.tk;
           if constexpr (MFA_CHECKS) {
             const int krow = sv.k0 + j * KBN;
@@ -600,6 +620,11 @@ __global__ void __launch_bounds__(sm100::Roles<CG, TILES>::kThreads,
     // tile-uniform interval extremes for the "block needs no mask" test
     const int tile_lo_max = key_range(a, sv, (r0 + t * BM + BM - 1) >> ps).lo;
     const int tile_hi_min = key_range(a, sv, (r0 + t * BM) >> ps).hi;
+    const int tile_sk_min = kSink ? key_range(a, sv, (r0 + t * BM) >> ps).sk : 0;
+    auto masked = [&](int kl) {
+      if constexpr (kSink) return (kl < kr.lo && kl >= kr.sk) || kl >= kr.hi;
+      else return kl < kr.lo || kl >= kr.hi;
+    };
     constexpr float kLog2e = 1.4426950408889634f;
     // x (the values kept in registers) times c is the logit in log2 units
     const float c = kGeneral ? 1.f : a.scale * kLog2e;
@@ -634,8 +659,10 @@ __global__ void __launch_bounds__(sm100::Roles<CG, TILES>::kThreads,
         if (lane == 0) mbar_arrive(&s_free[t]);
       }
       float x[NC];
-      const int c0 = (jb + j) * KBN + col0;  // local key index of x[0]
-      const bool need_mask = ((jb + j) * KBN < tile_lo_max) || ((jb + j) * KBN + KBN > tile_hi_min);
+      const int kb0 = block_at(j) * KBN;
+      const int c0 = kb0 + col0;  // local key index of x[0]
+      const bool need_mask = (kb0 < tile_lo_max && !(kSink && kb0 + KBN <= tile_sk_min)) ||
+                             (kb0 + KBN > tile_hi_min);
       // ALiBi on a block whose keys all lie on one side of the centre of every row of this
       // warp (every causal block but the diagonal): |centre - key| is linear in the key index,
       // so the bias is one packed FMA, slope' * i + base, and x = s * scale + bias another.
@@ -665,7 +692,7 @@ __global__ void __launch_bounds__(sm100::Roles<CG, TILES>::kThreads,
 #pragma unroll
           for (int i = 0; i < NC; ++i) {
             const int kl = c0 + i;
-            if (kl < kr.lo || kl >= kr.hi) x[i] = -INFINITY;
+            if (masked(kl)) x[i] = -INFINITY;
           }
         }
       } else if constexpr (kGeneral) {
@@ -717,7 +744,7 @@ __global__ void __launch_bounds__(sm100::Roles<CG, TILES>::kThreads,
 #pragma unroll
           for (int i = 0; i < NC; ++i) {
             const int kl = c0 + i;
-            if (kl < kr.lo || kl >= kr.hi) x[i] = -INFINITY;
+            if (masked(kl)) x[i] = -INFINITY;
           }
         }
       } else {
@@ -725,7 +752,7 @@ __global__ void __launch_bounds__(sm100::Roles<CG, TILES>::kThreads,
 #pragma unroll
           for (int i = 0; i < NC; ++i) {
             const int kl = c0 + i;
-            x[i] = (kl < kr.lo || kl >= kr.hi) ? -INFINITY : __uint_as_float(r[i]);
+            x[i] = masked(kl) ? -INFINITY : __uint_as_float(r[i]);
           }
         } else {
 #pragma unroll

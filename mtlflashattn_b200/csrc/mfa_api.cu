@@ -4,7 +4,6 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <cudaTypedefs.h>
-#include <nvtx3/nvToolsExt.h>
 
 #include <algorithm>
 #include <atomic>
@@ -17,6 +16,8 @@
 #include "../../include/mfa.h"
 #include "fa_simt.cuh"
 #include "fa_sm100.cuh"
+#include "host.cuh"
+#include "sm100_launch.cuh"
 
 namespace mfa {
 // The fp32 CUDA-core forward, compiled in simt_fwd.cu without fast math.
@@ -28,32 +29,6 @@ static_assert(mfa::kErrCheck == MFA_ERR_CHECK, "device check status differs from
 
 namespace mfa {
 namespace {
-
-// ------------------------------------------------------------------ host fault injection
-// MFA_FAULT=<site>[,<site>...] makes the named entry point fail before it launches anything,
-// so callers' error handling can be tested without touching a GPU. Sites: fwd, combine.
-bool fault_injected(const char* site) {
-  const char* env = std::getenv("MFA_FAULT");
-  if (env == nullptr || *env == 0) return false;
-  const size_t n = std::strlen(site);
-  for (const char* p = env; *p;) {
-    const char* e = std::strchr(p, ',');
-    const size_t len = e ? (size_t)(e - p) : std::strlen(p);
-    if (len == n && std::strncmp(p, site, n) == 0) return true;
-    if (!e) break;
-    p = e + 1;
-  }
-  return false;
-}
-
-// ------------------------------------------------------------------ NVTX
-// Host-side range around each launching entry point, named after it, so an nsys / ncu timeline
-// shows which library call queued which kernels. NVTX v3 is header-only: with no tool attached
-// a push/pop is a test of a null function pointer.
-struct NvtxRange {
-  explicit NvtxRange(const char* name) { nvtxRangePushA(name); }
-  ~NvtxRange() { nvtxRangePop(); }
-};
 
 // ------------------------------------------------------------------ driver entry point
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
@@ -69,48 +44,7 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
-struct DevInfo {
-  int major = -1, minor = -1, sms = 0;
-};
-DevInfo dev_info(int dev) {
-  static std::mutex mu;
-  static DevInfo cache[64];
-  std::lock_guard<std::mutex> lk(mu);
-  if (dev < 0 || dev >= 64) return DevInfo{};
-  if (cache[dev].major < 0) {
-    cudaDeviceGetAttribute(&cache[dev].major, cudaDevAttrComputeCapabilityMajor, dev);
-    cudaDeviceGetAttribute(&cache[dev].minor, cudaDevAttrComputeCapabilityMinor, dev);
-    cudaDeviceGetAttribute(&cache[dev].sms, cudaDevAttrMultiProcessorCount, dev);
-  }
-  return cache[dev];
-}
-
-// cudaFuncSetAttribute once per (kernel, device).
-template <typename K>
-cudaError_t ensure_smem(K kernel, int dev, int bytes) {
-  static std::mutex mu;
-  static const void* seen[256];
-  static int seen_dev[256];
-  static int nseen = 0;
-  std::lock_guard<std::mutex> lk(mu);
-  for (int i = 0; i < nseen; ++i)
-    if (seen[i] == (const void*)kernel && seen_dev[i] == dev) return cudaSuccess;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  // all of the SM's unified L1/shared storage as shared memory (two one-tile CTAs per SM)
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
-                             cudaSharedmemCarveoutMaxShared);
-  if (e == cudaSuccess && nseen < 256) {
-    seen[nseen] = (const void*)kernel;
-    seen_dev[nseen] = dev;
-    ++nseen;
-  }
-  return e;
-}
-
 int esize(int dtype) { return dtype == MFA_FP32 ? 4 : 2; }
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Argument checks. Mirrors the checks the reference makes before any tier runs
 // (metal_flash_attn/__init__.py:28-59, 84-90; _kernel.py:1070-1074, 1145-1147).
@@ -122,7 +56,7 @@ int validate(const mfa_fwd_params* p) {
   if (p->D < 1 || p->D > 128) return MFA_ERR_UNSUPPORTED;
   if (p->B < 0 || p->Hq < 1 || p->Hkv < 1 || p->Hq % p->Hkv != 0) return MFA_ERR_INVALID;
   if (!(p->softcap >= 0.f)) return MFA_ERR_INVALID;
-  if (p->win_left < -1 || p->win_right < -1) return MFA_ERR_INVALID;
+  if (p->win_left < -1 || p->win_right < -1 || p->sink < 0) return MFA_ERR_INVALID;
   const bool varlen = p->cu_q != nullptr || p->cu_k != nullptr;
   if (varlen && (p->cu_q == nullptr || p->cu_k == nullptr)) return MFA_ERR_INVALID;
   if (!varlen && (p->Lq < 0 || p->Lk < 0)) return MFA_ERR_INVALID;
@@ -162,6 +96,7 @@ FwdArgs resolve(const mfa_fwd_params* p) {
   a.causal = p->causal ? 1 : 0;
   a.wl = p->win_left;
   a.wr = p->win_right;
+  a.sink = p->win_left >= 0 ? p->sink : 0;  // an open left side sees every key anyway
   a.alibi = p->alibi;
   a.o_dtype = p->o_dtype < 0 ? p->dtype : p->o_dtype;
   const int oes = esize(a.o_dtype);
@@ -377,11 +312,6 @@ int make_map(CUtensorMap* m, const void* base, int dtype, int D, int H, int64_t 
   return rc;
 }
 
-// Tiles per CTA of the tcgen05 kernel fa_fwd_sm100<DP, *, GEN> (its default template argument).
-template <int DP, int GEN>
-constexpr int sm100_tiles() {
-  return DefaultTiles<DP, DefaultCG<GEN, DP>::value, GEN>::value;
-}
 int sm100_tiles_rt(bool wide, int gen) {
   if (wide) return gen == 2 ? sm100_tiles<128, 2>() : gen == 1 ? sm100_tiles<128, 1>() : sm100_tiles<128, 0>();
   return gen == 2 ? sm100_tiles<64, 2>() : gen == 1 ? sm100_tiles<64, 1>() : sm100_tiles<64, 0>();
@@ -411,31 +341,6 @@ int sm100_kbn_rt(bool wide, int gen, bool short_rows) {
                                                                  : sm100_kbn<DP, 0, false>()))
   return wide ? MFA_KBN(128) : MFA_KBN(64);
 #undef MFA_KBN
-}
-
-// SHORT: the one-tile, one-column-group kPack instantiation (sm100_short).
-template <int DP, bool BF16, int GEN, bool SHORT>
-int launch_sm100(const Sm100Args& args, int dev, int64_t grid, cudaStream_t st) {
-  constexpr int CG = SHORT ? 1 : DefaultCG<GEN, DP>::value;
-  constexpr int TILES = SHORT ? 1 : sm100_tiles<DP, GEN>();
-  auto k = fa_fwd_sm100<DP, BF16, GEN, CG, TILES, SHORT>;
-  using R = sm100::Roles<CG, TILES>;
-  constexpr int KBN = sm100::BlockKeys<DP, GEN, CG, TILES, SHORT>::value;
-  const int smem = (int)sm100::Cfg<DP, TILES, KBN>::SMEM;
-  // The kernel re-splits its registers with setmaxnreg assuming exactly kLaunchRegs per thread
-  // at launch; a build that launched with fewer would make setmaxnreg.inc wait forever.
-  static std::atomic<int> launch_regs{-1};
-  int regs = launch_regs.load(std::memory_order_relaxed);
-  if (regs < 0) {
-    cudaFuncAttributes fa;
-    if (cudaFuncGetAttributes(&fa, k) != cudaSuccess) return MFA_ERR_CUDA;
-    regs = fa.numRegs;
-    launch_regs.store(regs, std::memory_order_relaxed);
-  }
-  if (regs != R::kLaunchRegs) return MFA_ERR_UNSUPPORTED;
-  if (ensure_smem(k, dev, smem) != cudaSuccess) return MFA_ERR_CUDA;
-  k<<<(unsigned)grid, R::kThreads, smem, st>>>(args);
-  return MFA_OK;
 }
 
 int launch_combine(const FwdArgs& fin, const float* ws_o, const float* ws_lse, void* o,
@@ -557,32 +462,10 @@ int run_sm100(const mfa_fwd_params* p, FwdArgs a, int dev, cudaStream_t st,
   if (grid == 0) return MFA_OK;
   if (grid >= (1ll << 31)) return MFA_ERR_UNSUPPORTED;
   const bool bf = p->dtype == MFA_BF16;
-#define MFA_SM100(DP, BF, G)                                                     \
-  do {                                                                           \
-    const int rc_ = short_rows ? launch_sm100<DP, BF, G, true>(args, dev, grid, st)   \
-                               : launch_sm100<DP, BF, G, false>(args, dev, grid, st); \
-    if (rc_ != MFA_OK || split.splits < 2) return rc_;                           \
-    return launch_combine(fin, ws_o, ws_lse, p->o, p->lse, st);                  \
-  } while (0)
-  if (wide) {
-    if (bf) {
-      if (gen == 2) MFA_SM100(128, true, 2);
-      if (gen == 1) MFA_SM100(128, true, 1);
-      MFA_SM100(128, true, 0);
-    }
-    if (gen == 2) MFA_SM100(128, false, 2);
-    if (gen == 1) MFA_SM100(128, false, 1);
-    MFA_SM100(128, false, 0);
-  }
-  if (bf) {
-    if (gen == 2) MFA_SM100(64, true, 2);
-    if (gen == 1) MFA_SM100(64, true, 1);
-    MFA_SM100(64, true, 0);
-  }
-  if (gen == 2) MFA_SM100(64, false, 2);
-  if (gen == 1) MFA_SM100(64, false, 1);
-  MFA_SM100(64, false, 0);
-#undef MFA_SM100
+  rc = (a.sink > 0 ? launch_sm100_sink : launch_sm100_rt<false>)(args, dev, wide, bf, gen,
+                                                                 short_rows, grid, st);
+  if (rc != MFA_OK || split.splits < 2) return rc;
+  return launch_combine(fin, ws_o, ws_lse, p->o, p->lse, st);
 }
 
 int run_simt(const mfa_fwd_params* p, const FwdArgs& a, cudaStream_t st) {

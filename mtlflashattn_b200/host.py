@@ -21,7 +21,7 @@ import math
 import torch
 
 from . import _kernel, _lib
-from ._kernel import MAX_HEAD_DIM, _BiasParams, _broadcast_alibi_slopes
+from ._kernel import MAX_HEAD_DIM, _BiasParams, _broadcast_alibi_slopes, _check_sink
 
 __all__ = ["flash_attn_host", "flash_attn_varlen_host"]
 
@@ -73,13 +73,14 @@ def _launch(p, io, device, synchronize, what):
 
 def flash_attn_host(q, k, v, softmax_scale=None, causal=False, window_size=(-1, -1),
                     softcap=0.0, alibi_slopes=None, device=None, out=None, chunks=0,
-                    synchronize=True):
+                    synchronize=True, sink_tokens=0):
     """``flash_attn_func`` on host tensors q ``[B, Lq, Hq, D]``, k/v ``[B, Lk, Hkv, D]``.
 
     Returns the host output ``[B, Lq, Hq, D]`` (``out`` if given, else a new pinned tensor).
     ``device``: the CUDA device that computes (default: the current one). ``chunks``: pipeline
     pieces (0 = automatic, 1 = no overlap)."""
     _check(q, k, v, window_size, softcap)
+    sink = _check_sink(sink_tokens)
     q, k, v = _kernel._last_dim_contig(q), _kernel._last_dim_contig(k), _kernel._last_dim_contig(v)
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     B, Lq, Hq, D = q.shape
@@ -92,7 +93,7 @@ def flash_attn_host(q, k, v, softmax_scale=None, causal=False, window_size=(-1, 
     od = torch.empty(B, Lq, Hq, D, dtype=q.dtype, device=device)
     alibi = (_broadcast_alibi_slopes(alibi_slopes.to(device), B, Hq, device)
              if alibi_slopes is not None else None)
-    bias = _BiasParams(softcap, window_size[0], window_size[1], alibi)
+    bias = _BiasParams(softcap, window_size[0], window_size[1], alibi, sink)
     p = _kernel._params(qd, kd, vd, od, B=B, Hq=Hq, Hkv=Hkv, Lq=Lq, Lk=Lk, D=D,
                         q_st=q.stride()[:3], k_st=k.stride()[:3], v_st=v.stride()[:3],
                         o_st=od.stride()[:3], scale=scale, causal=causal, bias=bias,
@@ -105,11 +106,13 @@ def flash_attn_host(q, k, v, softmax_scale=None, causal=False, window_size=(-1, 
 
 def flash_attn_varlen_host(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k,
                            softmax_scale=None, causal=False, window_size=(-1, -1), softcap=0.0,
-                           alibi_slopes=None, device=None, out=None, chunks=0, synchronize=True):
+                           alibi_slopes=None, device=None, out=None, chunks=0, synchronize=True,
+                           sink_tokens=0):
     """``flash_attn_varlen_func`` on host tensors q ``[total_q, Hq, D]``, k/v
     ``[total_k, Hkv, D]`` and host int32 ``cu_seqlens_*`` ``[batch + 1]``. Returns the host
     output ``[total_q, Hq, D]``."""
     _check(q, k, v, window_size, softcap)
+    sink = _check_sink(sink_tokens)
     q, k, v = _kernel._last_dim_contig(q), _kernel._last_dim_contig(k), _kernel._last_dim_contig(v)
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     cu_q_h = cu_seqlens_q.to("cpu", torch.int32).contiguous()
@@ -132,7 +135,7 @@ def flash_attn_varlen_host(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, ma
         cu_k = cu_k_h.to(device, non_blocking=True)
     alibi = (_broadcast_alibi_slopes(alibi_slopes.to(device), batch, Hq, device)
              if alibi_slopes is not None else None)
-    bias = _BiasParams(softcap, window_size[0], window_size[1], alibi)
+    bias = _BiasParams(softcap, window_size[0], window_size[1], alibi, sink)
     p = _kernel._params(qd, kd, vd, od, B=batch, Hq=Hq, Hkv=Hkv, Lq=total_q, Lk=total_k, D=D,
                         q_st=(0, q.stride(0), q.stride(1)), k_st=(0, k.stride(0), k.stride(1)),
                         v_st=(0, v.stride(0), v.stride(1)), o_st=(0, od.stride(0), od.stride(1)),
