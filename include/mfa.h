@@ -249,6 +249,106 @@ int mfa_fwd_staged(const mfa_fwd_params* p, const mfa_host_io* io, void* cuda_st
  * it faults, traps or hangs nothing. */
 int mfa_selftest_wait_timeout(int32_t* err, uint32_t timeout_us, void* cuda_stream);
 
+/* ---- per-head norm of queries and keys with the position rotation (no counterpart in the
+ * reference). For every head row x of q and k, in fp32 with one rounding at the end:
+ *   y = x / sqrt(mean(x^2) + eps) * weight
+ *   (y_a, y_b) -> (y_a cos - y_b sin, y_a sin + y_b cos), cos/sin row = the token's position,
+ *   over the pairs (i, i + R/2), or (2i, 2i + 1) when interleaved, i < R/2; dims >= R as they are.
+ * A token whose position is not in [0, max_pos) gets rows of zeros, and MFA_ERR_INVALID goes to
+ * *err. Outputs are contiguous and may not overlap the inputs. */
+typedef struct mfa_norm_rope_params {
+  const void* q;      /* [B, L, Hq, D], any (batch, seq, head) strides, last dim stride 1 */
+  const void* k;      /* [B, L, Hkv, D] */
+  void* q_out;        /* contiguous [B, L, Hq, D] */
+  void* k_out;        /* contiguous [B, L, Hkv, D] */
+  int64_t q_stride[3];
+  int64_t k_stride[3];
+  const void* q_weight; /* [D] of w_dtype, or NULL (ones) */
+  const void* k_weight;
+  const void* cos;    /* [max_pos, R/2] of rot_dtype, last dim stride 1; unused when R = 0 */
+  const void* sin;
+  int64_t cos_stride; /* row strides in elements */
+  int64_t sin_stride;
+  const void* positions; /* device int32 (int64 when pos64) per token, or NULL: 0 .. L - 1 */
+  int64_t pos_stride[2]; /* batch, seq */
+  int32_t B, L, Hq, Hkv, D, R, max_pos;
+  int32_t pos64;
+  int32_t dtype;      /* mfa_dtype of q, k and the outputs */
+  int32_t w_dtype;    /* dtype, or MFA_FP32 */
+  int32_t rot_dtype;  /* dtype, or MFA_FP32 */
+  int32_t interleaved;
+  float eps;
+  int32_t* err;       /* optional device int */
+} mfa_norm_rope_params;
+
+int mfa_qk_norm_rope(const mfa_norm_rope_params* p, void* cuda_stream);
+
+/* ---- a paged key/value cache held in 4 bits (no counterpart in the reference). Each group of 16
+ * consecutive dims of one head of one token shares a scale,
+ *   scale = e4m3(min(max|x / unit| / 6, 448)),   code = e2m1 nearest to x / unit / scale, ties to
+ * the even code; it stands for code * scale * unit. A NaN in a group makes its scale, and with it
+ * the whole group, NaN; infinities saturate. Units are powers of two, so everything but the two
+ * roundings is exact and the held value is exact in fp16 and bf16.
+ * Codes take two per byte, the first in the low half, with the dims of a row permuted so that a
+ * thread of the attention reads its own in one load (d = 16 i + j):
+ *   keys    byte (j / 4) (D / 8) + 2 i + (j % 4) / 2, half (j % 4) % 2
+ *   values  byte (j % 8) (D / 16) + i, half j / 8
+ * Token t of sequence b is slot t % page_size of page block_table[b][t / page_size]. A page index
+ * outside [0, num_pages), or a token outside [0, max_pages * page_size), is never dereferenced: it
+ * is skipped and MFA_ERR_INVALID goes to *err. */
+typedef struct mfa_kv4_cache {
+  void* k;            /* [num_pages, Hkv, page_size, D/2] bytes, contiguous, 16-byte aligned */
+  void* v;
+  void* k_scale;      /* [num_pages, Hkv, page_size, D/16] e4m3, contiguous, 16-byte aligned */
+  void* v_scale;
+  const int32_t* block_table; /* [B, max_pages], row stride table_stride (elements) */
+  int64_t table_stride;
+  int32_t num_pages, page_size; /* page_size a power of two, 16 .. 1024 */
+  int32_t Hkv, D;     /* D 64 or 128 */
+  int32_t B, max_pages;
+  float k_unit, v_unit; /* powers of two, 2^-14 .. 2^4 */
+  int32_t* err;       /* optional device int */
+} mfa_kv4_cache;
+
+/* Rows going in (mfa_kv4_append) or coming out (mfa_kv4_gather). */
+typedef struct mfa_kv4_rows {
+  void* k;            /* [B, L, Hkv, D], any (batch, seq, head) strides, last dim stride 1 */
+  void* v;
+  int64_t k_stride[3];
+  int64_t v_stride[3];
+  const int32_t* start; /* device [B]: the token of row 0 (NULL: 0) */
+  const int32_t* lens;  /* device [B]: append, how many of a sequence's L rows count (NULL: L);
+                           gather, the sequence's length (required) */
+  int32_t L;
+  int32_t dtype;      /* append: fp16, bf16; gather: also fp32 */
+} mfa_kv4_rows;
+
+/* Writes row j < lens[b] of sequence b at token start[b] + j. Two rows must not share a slot. */
+int mfa_kv4_append(const mfa_kv4_cache* c, const mfa_kv4_rows* r, void* cuda_stream);
+
+/* Reads token start[b] + j into row j of sequence b; rows at or past lens[b] become 0. */
+int mfa_kv4_gather(const mfa_kv4_cache* c, const mfa_kv4_rows* r, void* cuda_stream);
+
+typedef struct mfa_kv4_fwd_params {
+  const void* q;      /* [B, Lq, Hq, D], any (batch, seq, head) strides, last dim stride 1 */
+  void* o;            /* [B, Lq, Hq, D] */
+  int64_t q_stride[3];
+  int64_t o_stride[3];
+  const int32_t* seqlens; /* device [B]: keys of each sequence, the Lq newest rows' among them */
+  int32_t Lq, Hq;
+  int32_t dtype;      /* fp16 or bf16, of q and o */
+  float scale, softcap;
+  int32_t causal, win_left, win_right, sink; /* as in mfa_fwd_params */
+  const float* alibi; /* optional device fp32 [B * Hq] */
+  void* workspace;    /* device, mfa_kv4_fwd_workspace_size bytes, 16-byte aligned */
+  size_t workspace_bytes;
+} mfa_kv4_fwd_params;
+
+/* Attention of the newest Lq rows of every sequence over its cached keys; the semantics of
+ * mfa_fwd with Lk = seqlens[b]. A row that sees no key is 0. */
+int mfa_kv4_fwd(const mfa_kv4_cache* c, const mfa_kv4_fwd_params* p, void* cuda_stream);
+size_t mfa_kv4_fwd_workspace_size(const mfa_kv4_cache* c, const mfa_kv4_fwd_params* p);
+
 const char* mfa_status_string(int status);
 int mfa_abi_version(void);
 

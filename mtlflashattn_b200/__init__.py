@@ -15,8 +15,11 @@ import torch
 from ._kernel import (MAX_HEAD_DIM, _BiasParams, _broadcast_alibi_slopes, _check_sink,
                       flash_attn_forward)
 from . import _kernel
+from ._grad import _guard_grad
 from ._version import __version__
 from .host import flash_attn_host, flash_attn_varlen_host
+from .kv4 import KV4Cache, flash_attn_with_kv4cache, kv4_append, kv4_cache, kv4_gather
+from .norm_rope import qk_norm_rope
 
 __all__ = [
     "flash_attn_func",
@@ -28,6 +31,12 @@ __all__ = [
     "flash_attn_forward",
     "flash_attn_host",
     "flash_attn_varlen_host",
+    "qk_norm_rope",
+    "KV4Cache",
+    "kv4_cache",
+    "kv4_append",
+    "kv4_gather",
+    "flash_attn_with_kv4cache",
     "__version__",
 ]
 
@@ -69,26 +78,6 @@ def _check_supported(q, k, v, dropout_p, window_size, softcap, alibi_slopes,
         raise NotImplementedError(f"mtlflashattn_b200: head_dim {D} > {MAX_HEAD_DIM}")
     if k.shape[-1] != D or v.shape[-1] != D:
         raise ValueError("mtlflashattn_b200: q/k/v head_dim mismatch")
-
-
-class _NoBackward(torch.autograd.Function):
-    """Marks the output as produced by an inference-only op: backward raises."""
-
-    @staticmethod
-    def forward(ctx, out, *inputs):
-        return out.view_as(out)
-
-    @staticmethod
-    def backward(ctx, *grads):
-        raise NotImplementedError("mtlflashattn_b200: backward is not supported (inference-only)")
-
-
-def _guard_grad(out, *inputs):
-    if torch.is_grad_enabled():
-        ts = [t for t in inputs if torch.is_tensor(t)]
-        if any(t.requires_grad for t in ts):
-            return _NoBackward.apply(out, *ts)
-    return out
 
 
 def flash_attn_func(

@@ -151,7 +151,8 @@ def check_device_errors(device=None):
     if v != 0:
         t.zero_()
         why = ("a kernel gave up on a bounded wait" if v == _lib.ERR_TIMEOUT else
-               "a split launch met a varlen row at or past Lq (Lq < cu_seqlens[-1])"
+               "a kernel met an index outside of its tensors (a varlen row at or past Lq, a position"
+               " outside of the rotation tables, a token without a page) and skipped it"
                if v == _lib.ERR_INVALID else
                "a device-side bounds check (MFA_CHECKS build) failed" if v == _lib.ERR_CHECK
                else "a kernel reported an error")
@@ -249,6 +250,33 @@ def _packed(*args):
         buf = _tls.buf = ctypes.create_string_buffer(_PACK.size)
     _PACK.pack_into(buf, 0, *_values(*args))
     return buf
+
+
+def _scratch(name, fmt):
+    """This thread's reusable buffer for one of the other params structs (valid until the next
+    call on this thread, as ``_packed``)."""
+    buf = getattr(_tls, name, None)
+    if buf is None:
+        buf = ctypes.create_string_buffer(fmt.size)
+        setattr(_tls, name, buf)
+    return buf
+
+
+def _call(dev, what, fn, *args):
+    """Run ``fn(*args, stream)`` with ``dev`` current, on its current stream, and raise on a
+    status that is not OK."""
+    ctx = torch.cuda.device(dev) if dev.index != torch.cuda.current_device() else None
+    if ctx is not None:
+        ctx.__enter__()
+    try:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+        if rc != _lib.OK:
+            _raise_status(rc, what)
+    finally:
+        if ctx is not None:
+            ctx.__exit__(None, None, None)
+    if _sync_check_enabled():
+        check_device_errors(dev)
 
 
 _workspaces = {}  # (device, stream) -> uint8 tensor

@@ -51,6 +51,11 @@ EXPORTED_SYMBOLS = (
     "mfa_peer_open",
     "mfa_peer_close",
     "mfa_peer_free",
+    "mfa_qk_norm_rope",
+    "mfa_kv4_append",
+    "mfa_kv4_gather",
+    "mfa_kv4_fwd",
+    "mfa_kv4_fwd_workspace_size",
     "mfa_selftest_wait_timeout",
     "mfa_status_string",
     "mfa_abi_version",
@@ -138,6 +143,109 @@ class MfaHostIo(ctypes.Structure):
     ]
 
 
+class MfaNormRopeParams(ctypes.Structure):
+    """Mirror of ``struct mfa_norm_rope_params`` (include/mfa.h)."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("k", ctypes.c_void_p),
+        ("q_out", ctypes.c_void_p),
+        ("k_out", ctypes.c_void_p),
+        ("q_stride", ctypes.c_int64 * 3),
+        ("k_stride", ctypes.c_int64 * 3),
+        ("q_weight", ctypes.c_void_p),
+        ("k_weight", ctypes.c_void_p),
+        ("cos", ctypes.c_void_p),
+        ("sin", ctypes.c_void_p),
+        ("cos_stride", ctypes.c_int64),
+        ("sin_stride", ctypes.c_int64),
+        ("positions", ctypes.c_void_p),
+        ("pos_stride", ctypes.c_int64 * 2),
+        ("B", ctypes.c_int32),
+        ("L", ctypes.c_int32),
+        ("Hq", ctypes.c_int32),
+        ("Hkv", ctypes.c_int32),
+        ("D", ctypes.c_int32),
+        ("R", ctypes.c_int32),
+        ("max_pos", ctypes.c_int32),
+        ("pos64", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("w_dtype", ctypes.c_int32),
+        ("rot_dtype", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("err", ctypes.c_void_p),
+    ]
+
+
+class MfaKv4Cache(ctypes.Structure):
+    """Mirror of ``struct mfa_kv4_cache`` (include/mfa.h)."""
+
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("block_table", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("num_pages", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("Hkv", ctypes.c_int32),
+        ("D", ctypes.c_int32),
+        ("B", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+        ("k_unit", ctypes.c_float),
+        ("v_unit", ctypes.c_float),
+        ("err", ctypes.c_void_p),
+    ]
+
+
+class MfaKv4Rows(ctypes.Structure):
+    """Mirror of ``struct mfa_kv4_rows`` (include/mfa.h)."""
+
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_stride", ctypes.c_int64 * 3),
+        ("v_stride", ctypes.c_int64 * 3),
+        ("start", ctypes.c_void_p),
+        ("lens", ctypes.c_void_p),
+        ("L", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+    ]
+
+
+class MfaKv4FwdParams(ctypes.Structure):
+    """Mirror of ``struct mfa_kv4_fwd_params`` (include/mfa.h)."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("o", ctypes.c_void_p),
+        ("q_stride", ctypes.c_int64 * 3),
+        ("o_stride", ctypes.c_int64 * 3),
+        ("seqlens", ctypes.c_void_p),
+        ("Lq", ctypes.c_int32),
+        ("Hq", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("softcap", ctypes.c_float),
+        ("causal", ctypes.c_int32),
+        ("win_left", ctypes.c_int32),
+        ("win_right", ctypes.c_int32),
+        ("sink", ctypes.c_int32),
+        ("alibi", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+# The same layouts as struct.pack formats (see PARAMS_FORMAT).
+NORM_ROPE_FORMAT = "<4Q6q4Q2qQ2q12if4xQ"
+KV4_CACHE_FORMAT = "<5Qq6i2fQ"
+KV4_ROWS_FORMAT = "<2Q6q2Q2i"
+KV4_FWD_FORMAT = "<2Q6qQ3i2f4i4x3Q"
+KV4_FWD_WORKSPACE_OFFSET = 120  # workspace pointer, then workspace_bytes
+
 _lib = None
 _lock = threading.Lock()
 
@@ -214,6 +322,13 @@ def load(path: str | None = None) -> ctypes.CDLL:
         lib.mfa_peer_close.restype = ctypes.c_int
         lib.mfa_peer_free.argtypes = [ctypes.c_void_p]
         lib.mfa_peer_free.restype = ctypes.c_int
+        lib.mfa_qk_norm_rope.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
+        lib.mfa_qk_norm_rope.restype = ctypes.c_int
+        for fn in (lib.mfa_kv4_append, lib.mfa_kv4_gather, lib.mfa_kv4_fwd):
+            fn.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]
+            fn.restype = ctypes.c_int
+        lib.mfa_kv4_fwd_workspace_size.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
+        lib.mfa_kv4_fwd_workspace_size.restype = ctypes.c_size_t
         lib.mfa_selftest_wait_timeout.argtypes = [ctypes.c_void_p, ctypes.c_uint32, ctypes.c_void_p]
         lib.mfa_selftest_wait_timeout.restype = ctypes.c_int
         lib.mfa_status_string.argtypes = [ctypes.c_int]
@@ -326,3 +441,23 @@ def lse_merge_rows(o_ptrs, lse_ptrs, rows_total, row0, nrows, H, D, o_ptr, o_dty
     la = (ctypes.c_void_p * n)(*lse_ptrs)
     return load().mfa_lse_merge_rows(oa, la, n, rows_total, row0, nrows, H, D, o_ptr, o_dtype,
                                      lse_ptr or None, stream)
+
+
+def qk_norm_rope(params, stream: int) -> int:
+    return load().mfa_qk_norm_rope(_addr(params), stream)
+
+
+def kv4_append(cache, rows, stream: int) -> int:
+    return load().mfa_kv4_append(_addr(cache), _addr(rows), stream)
+
+
+def kv4_gather(cache, rows, stream: int) -> int:
+    return load().mfa_kv4_gather(_addr(cache), _addr(rows), stream)
+
+
+def kv4_fwd(cache, params, stream: int) -> int:
+    return load().mfa_kv4_fwd(_addr(cache), _addr(params), stream)
+
+
+def kv4_fwd_workspace_size(cache, params) -> int:
+    return load().mfa_kv4_fwd_workspace_size(_addr(cache), _addr(params))

@@ -46,9 +46,12 @@ def up_to_date() -> bool:
 # kernel's exponentials are ex2.approx by design); the fp32 CUDA-core forward is the accuracy
 # path and is compiled with IEEE division / square root, accurate expf / tanhf / logf and no
 # flush to zero.
+PRECISE = ["-ftz=false", "-prec-div=true", "-prec-sqrt=true"]
 UNITS = (("mfa_api.cu", ["--use_fast_math"]),
          ("sink_fwd.cu", ["--use_fast_math"]),
-         ("simt_fwd.cu", ["-ftz=false", "-prec-div=true", "-prec-sqrt=true"]))
+         ("kv4.cu", PRECISE),
+         ("norm_rope.cu", PRECISE),
+         ("simt_fwd.cu", PRECISE))
 
 
 def build(verbose: bool = False, force: bool = False, defines=(), out: str | None = None) -> str:

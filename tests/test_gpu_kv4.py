@@ -1,0 +1,482 @@
+"""The paged 4-bit cache against its definition (oracle/kv4.py): what append holds, exactly, and
+attention over it in 64 bits on the same held values."""
+import pytest
+import torch
+
+import mtlflashattn_b200 as mfa
+from mtlflashattn_b200 import _kernel, _lib
+from oracle import kv4 as ref
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def table_of(B, each, extra=0, seed=0):
+    """A block table over shuffled pages: (int32 [B, each], number of pages)."""
+    n = B * each + extra
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return torch.randperm(n, device=DEV, generator=g)[:B * each].view(B, each).int(), n
+
+
+def i32(*x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def dirty(cache):
+    """Every byte set, the scales to NaN: what memory may hold where nothing was appended."""
+    cache.k.fill_(0xE7)
+    cache.v.fill_(0x7E)
+    cache.k_scale.view(torch.uint8).fill_(0x7F)
+    cache.v_scale.view(torch.uint8).fill_(0xFF)
+    return cache
+
+
+def reported():
+    with pytest.raises(_lib.MfaError):
+        _kernel.check_device_errors()
+
+
+# ---------------------------------------------------------------------------- append and gather
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("page", [16, 64, 1024])
+@pytest.mark.parametrize("B,L,Hkv", [(1, 1, 1), (3, 1, 8), (2, 37, 3), (1, 130, 2)])
+def test_append_holds_exactly_what_is_defined(dtype, D, page, B, L, Hkv):
+    g = torch.Generator(device=DEV).manual_seed(B + L)
+    start = [0, 13, 50][:B]
+    each = -(-(50 + L) // page)
+    table, pages = table_of(B, each, 2)
+    cache = dirty(mfa.kv4_cache(pages, page, Hkv, D, DEV, k_unit=2.0**-3, v_unit=2.0))
+    k, v = (torch.randn(B, L, Hkv, D, device=DEV, generator=g) for _ in range(2))
+    k *= torch.exp(2 * torch.randn(B, L, Hkv, 1, device=DEV, generator=g))  # rows of other sizes
+    k, v = k.to(dtype), v.to(dtype)
+    before = [t.view(torch.uint8).clone() for t in (cache.k, cache.v, cache.k_scale, cache.v_scale)]
+    mfa.kv4_append(cache, k, v, table, i32(*start))
+    end = i32(*(s + L for s in start))
+    written = torch.zeros(pages, page, dtype=torch.bool, device=DEV)
+    for b, s in enumerate(start):
+        for x, keys, unit in ((k, True, 2.0**-3), (v, False, 2.0)):
+            got = ref.tokens(cache, table[b], s + L, keys)[s:]
+            assert torch.equal(got, ref.held(x[b], unit))
+        at = torch.arange(s, s + L, device=DEV)
+        written[table[b].long()[at // page], at % page] = True
+    for t, old in zip((cache.k, cache.v, cache.k_scale, cache.v_scale), before):
+        new = t.view(torch.uint8).transpose(1, 2)
+        assert torch.equal(new[~written], old.transpose(1, 2)[~written])  # nothing else
+    for out in (dtype, torch.float32):
+        gk, gv = mfa.kv4_gather(cache, table, end, L + 3, starts=i32(*start), dtype=out)
+        for x, got, unit in ((k, gk, 2.0**-3), (v, gv, 2.0)):
+            want = torch.stack([ref.held(x[b], unit) for b in range(B)])
+            assert got.dtype == out
+            assert torch.equal(got[:, :L].double(), want) and bool((got[:, L:] == 0).all())
+    _kernel.check_device_errors()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_borders_zeros_and_what_is_not_finite(dtype):
+    rows = []
+    for top in (6.0, 0.75, 6 * 448.0, 6 * 2.0**-9, 6 * 13 * 2.0**-4, 3 * 2.0**-10, 1e-5, 3000.0):
+        s = ref.quantise(torch.full((16,), top))[1].float().item()
+        for sign in (1, -1):
+            # every border of the codes and its neighbours, with the value that sets the scale
+            borders = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0]) * s * sign
+            edge = borders.to(dtype)
+            up = torch.nextafter(edge, torch.full_like(edge, 6e4))
+            down = torch.nextafter(edge, torch.full_like(edge, -6e4))
+            for x in (edge, up, down):
+                rows.append(torch.cat((torch.tensor([top, 0.0]).to(dtype), x,
+                                       torch.zeros(7, dtype=dtype))))
+    nan, inf = float("nan"), float("inf")
+    for special in ([0.0] * 16, [-0.0] * 16, [nan] + [1.0] * 15, [1.0] * 15 + [nan],
+                    [inf] + [1.0] * 15, [2.0] * 7 + [-inf] + [3.0] * 8, [inf, nan] + [0.0] * 14,
+                    [torch.finfo(dtype).max] * 16, [torch.finfo(dtype).smallest_normal] * 16,
+                    [torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps] * 16):
+        rows.append(torch.tensor(special).to(dtype))
+    while len(rows) % 4:
+        rows.append(torch.ones(16, dtype=dtype))
+    x = torch.cat(rows).view(1, -1, 1, 64).to(DEV)
+    L = x.shape[1]
+    for unit in (1.0, 2.0**-14, 16.0):
+        cache = dirty(mfa.kv4_cache(-(-L // 16), 16, 1, 64, DEV, k_unit=unit, v_unit=unit))
+        table = torch.arange(cache.num_pages, device=DEV).int()[None]
+        mfa.kv4_append(cache, x, x, table, i32(0))
+        want = ref.held(x[0], unit)
+        got = mfa.kv4_gather(cache, table, i32(L), L, dtype=torch.float32)
+        for t in got:
+            torch.testing.assert_close(t[0].double(), want, atol=0, rtol=0, equal_nan=True)
+        # exact in 16 bits too, but where a saturated value passes the type's range
+        half = mfa.kv4_gather(cache, table, i32(L), L, dtype=dtype)[0][0]
+        torch.testing.assert_close(half.double(), want, atol=0, rtol=0, equal_nan=True)
+
+
+def test_padded_rows_views_and_rows_without_a_page():
+    B, L, Hkv, D, page = 4, 6, 2, 64, 16
+    g = torch.Generator(device=DEV).manual_seed(7)
+    qkv = torch.randn(B, L, 4 + 2 * Hkv, D, device=DEV, generator=g).bfloat16()
+    k, v = qkv[:, :, 4:4 + Hkv], qkv[:, :, 4 + Hkv:]
+    table, pages = table_of(B, 2)
+    cache = dirty(mfa.kv4_cache(pages, page, Hkv, D, DEV))
+    lens = (6, 0, 3, 99)  # the last: all of them
+    mfa.kv4_append(cache, k, v, table, i32(0, 5, 14, 20), new_lens=i32(*lens))
+    _kernel.check_device_errors()
+    for b, (s, n) in enumerate(zip((0, 5, 14, 20), (6, 0, 3, 6))):
+        got = ref.tokens(cache, table[b], 32, True)
+        assert torch.equal(got[s:s + n], ref.held(k[b, :n]))
+        rest = torch.ones(32, dtype=torch.bool)
+        rest[s:s + n] = False
+        assert bool(got[rest.to(DEV)].isnan().all())
+    # outside of the table, a page that does not exist, a negative length: skipped and reported
+    snap = [t.view(torch.uint8).clone() for t in (cache.k, cache.v, cache.k_scale, cache.v_scale)]
+    for start, spoil in ((32, None), (-6, None), (2**31 - 1, None), (0, pages), (0, -1),
+                         (0, 2**31 - 1), (0, -2**31)):
+        bad = table.clone()
+        if spoil is not None:
+            bad[1, 0] = spoil
+        only = i32(0, 6, 0, 0)
+        mfa.kv4_append(cache, k, v, bad, i32(0, start, 0, 0), new_lens=only)
+        reported()
+        for t, old in zip((cache.k, cache.v, cache.k_scale, cache.v_scale), snap):
+            assert torch.equal(t.view(torch.uint8), old)
+        gk, gv = mfa.kv4_gather(cache, bad, i32(0, min(start, 2**31 - 8) + 6, 0, 0), 6,
+                                starts=i32(0, min(start, 2**31 - 8), 0, 0))
+        reported()
+        assert bool((gk[1] == 0).all()) and bool((gv[1] == 0).all())
+    # across the end of the table: the rows that have a page are written
+    mfa.kv4_append(cache, k, v, table, i32(0, 29, 0, 0), new_lens=i32(0, 6, 0, 0))
+    reported()
+    assert torch.equal(ref.tokens(cache, table[1], 32, False)[29:], ref.held(v[1, :3]))
+
+
+def test_pool_beyond_32_bits():
+    page, Hkv, D = 1024, 8, 128
+    pages = 2**31 // (page * Hkv * D // 2) + 9
+    cache = mfa.kv4_cache(pages, page, Hkv, D, DEV)
+    table = i32(pages - 1, 3, pages - 2).view(1, 3)
+    g = torch.Generator(device=DEV).manual_seed(8)
+    k, v = (torch.randn(1, 2 * page + 70, Hkv, D, device=DEV, generator=g).bfloat16()
+            for _ in range(2))
+    n = k.shape[1]
+    mfa.kv4_append(cache, k, v, table, i32(0))
+    gk, gv = mfa.kv4_gather(cache, table, i32(n), n)
+    assert torch.equal(gk[0].double(), ref.held(k[0])) and torch.equal(gv[0].double(), ref.held(v[0]))
+    q = torch.randn(1, 1, 8, D, device=DEV, generator=g).bfloat16()
+    out = mfa.flash_attn_with_kv4cache(q, cache, table, i32(n), causal=True)
+    check(out[0], ref.attention(q[0], gk[0], gv[0]), gv[0])
+    _kernel.check_device_errors()
+
+
+# ------------------------------------------------------------------------------------ attention
+def check(out, want, v, softcap=0.0):
+    # Probabilities are rounded to fp16 and once more with the value's scale (2^-11 each), and are
+    # off by what moves a logit: its fp32 sum of 128 products, 2^-16 of sum|q k| / sqrt(D) (under
+    # 64 here) = 2^-10, twice (numerator and sum). With sum p = 1 that is 2^-8.4 max|v| at most.
+    # Then one rounding to the output's type.
+    top = v.double().nan_to_num(0.0).abs().amax() if v.numel() else 0.0
+    step = torch.finfo(out.dtype).eps / 2
+    torch.testing.assert_close(out.double(), want, atol=float(top) * 2**-8.4, rtol=step,
+                               equal_nan=True)
+    # as independent roundings they cancel: the 2-norm is far below the bound
+    w = want.nan_to_num(0.0)
+    off = (out.double().nan_to_num(0.0) - w).norm()
+    assert off <= 2 * (step + 2**-11) * w.norm() + 1e-30
+
+
+def filled(lens, page, Hkv, D, seed=0, **unit):
+    """A cache of normal keys and values for sequences of these lengths, NaN everywhere else."""
+    B = len(lens)
+    each = max(1, -(-max(lens) // page))
+    table, pages = table_of(B, each, 1, seed)
+    cache = dirty(mfa.kv4_cache(pages, page, Hkv, D, DEV, **unit))
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    L = max(max(lens), 1)
+    k, v = (torch.randn(B, L, Hkv, D, device=DEV, generator=g).bfloat16() for _ in range(2))
+    mfa.kv4_append(cache, k, v, table, i32(*[0] * B), new_lens=i32(*lens))
+    return cache, table, g
+
+
+def compare(cache, table, lens, q, **kw):
+    n = i32(*lens)
+    out = mfa.flash_attn_with_kv4cache(q, cache, table, n, causal=kw.get("causal", False),
+                                       window_size=kw.get("window", (-1, -1)),
+                                       softcap=kw.get("softcap", 0.0),
+                                       alibi_slopes=kw.get("slopes"),
+                                       sink_tokens=kw.get("sink", 0),
+                                       softmax_scale=kw.get("scale"))
+    _kernel.check_device_errors()
+    assert out.shape == q.shape and out.dtype == q.dtype
+    for b, length in enumerate(lens):
+        k = ref.tokens(cache, table[b], length, True)
+        v = ref.tokens(cache, table[b], length, False)
+        check(out[b], ref.attention(q[b], k, v, **kw), v)
+    return out
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D,Hq,Hkv", [(128, 4, 4), (128, 32, 4), (64, 16, 1), (64, 6, 2),
+                                      (128, 5, 1), (64, 24, 2)])
+@pytest.mark.parametrize("Lq,page,kw", [
+    (1, 16, dict(causal=True)),
+    (1, 64, dict(causal=True, window=(100, -1), sink=5)),
+    (3, 32, dict(causal=True)),
+    (5, 128, dict(causal=True, window=(33, -1), sink=40)),
+    (2, 16, dict(window=(20, 3), sink=1)),
+    (7, 64, dict(causal=False, scale=-0.2)),
+    (40, 16, dict(causal=True, window=(300, -1), sink=17)),
+])
+def test_attention_against_formula(dtype, D, Hq, Hkv, Lq, page, kw):
+    lens = (0, 1, 15, 16, 17, 200, 531, 64)
+    cache, table, g = filled(lens, page, Hkv, D, seed=Lq)
+    q = torch.randn(len(lens), Lq, Hq, D, device=DEV, generator=g).to(dtype)
+    compare(cache, table, lens, q, **kw)
+
+
+@pytest.mark.parametrize("kw", [dict(softcap=20.0), dict(slopes=True),
+                                dict(softcap=5.0, slopes=True, window=(200, -1), sink=9)])
+@pytest.mark.parametrize("Lq", [1, 4])
+def test_attention_softcap_alibi_units(kw, Lq):
+    lens = (700, 3, 90)
+    cache, table, g = filled(lens, 32, 2, 128, seed=3, k_unit=0.25, v_unit=2.0**-5)
+    q = torch.randn(3, Lq, 8, 128, device=DEV, generator=g).half()
+    if kw.get("slopes"):
+        kw = dict(kw, slopes=torch.tensor([0.5 ** (i + 1) for i in range(8)], device=DEV))
+    compare(cache, table, lens, q, causal=True, **kw)
+
+
+@pytest.mark.parametrize("B,lk,Lq,Hq,Hkv", [(1, 20000, 1, 16, 2), (2, 5000, 1, 8, 8),
+                                            (1, 9000, 3, 8, 1)])
+def test_split_over_a_long_cache(B, lk, Lq, Hq, Hkv):
+    lens = tuple(lk - 37 * b * b for b in range(B))
+    cache, table, g = filled(lens, 64, Hkv, 128, seed=B)
+    q = torch.randn(B, Lq, Hq, 128, device=DEV, generator=g).bfloat16()
+    for kw in (dict(), dict(window=(3000, -1), sink=4), dict(window=(1, -1), sink=2500)):
+        a = compare(cache, table, lens, q, causal=True, **kw)
+        n = i32(*lens)
+        again = mfa.flash_attn_with_kv4cache(q, cache, table, n, causal=True,
+                                             window_size=kw.get("window", (-1, -1)),
+                                             sink_tokens=kw.get("sink", 0))
+        assert torch.equal(a, again)
+
+
+@pytest.mark.parametrize("Lq,Hq,Hkv,D", [(130, 8, 2, 64), (300, 4, 4, 128), (257, 6, 1, 128)])
+def test_chunk_of_a_prompt(Lq, Hq, Hkv, D):
+    lens = (700, Lq, 0, 40)  # the last two: rows before the first key see nothing
+    cache, table, g = filled(lens, 32, Hkv, D, seed=Lq)
+    q = torch.randn(4, Lq, Hq, D, device=DEV, generator=g).bfloat16()
+    compare(cache, table, lens, q, causal=True)
+    compare(cache, table, lens, q, causal=True, window=(100, -1), sink=6)
+
+
+def test_extreme_queries():
+    """Query rows far outside of fp16's range in bf16, zeros, and infinities in one row only."""
+    lens = (300,)
+    cache, table, g = filled(lens, 32, 1, 64, seed=5)
+    q = torch.randn(1, 1, 8, 64, device=DEV, generator=g).bfloat16()
+    size = torch.tensor([1e-30, 1e-8, 1e-3, 1.0, 3.0, 0.0, 1e-38, 1.0], device=DEV)
+    q = (q.float() * size[:, None]).bfloat16()
+    compare(cache, table, lens, q)
+    scaled = (q.float() * 2.0**100).bfloat16()
+    scaled[0, 0, 2:5] = 0
+    scaled[0, 0, 7] = 0
+    out = mfa.flash_attn_with_kv4cache(scaled, cache, table, i32(300), softmax_scale=2.0**-103)
+    want = mfa.flash_attn_with_kv4cache((scaled.float() * 2.0**-100).bfloat16(), cache, table,
+                                        i32(300), softmax_scale=2.0**-3)
+    assert torch.equal(out[0, 0, :2], want[0, 0, :2]) and torch.equal(out[0, 0, 5:], want[0, 0, 5:])
+    good = mfa.flash_attn_with_kv4cache(q, cache, table, i32(300))
+    q[0, 0, 3, 10] = float("nan")
+    q[0, 0, 6] = float("inf")
+    out = mfa.flash_attn_with_kv4cache(q, cache, table, i32(300))
+    rest = [0, 1, 2, 4, 5, 7]
+    assert torch.equal(out[0, 0, rest], good[0, 0, rest])
+    assert bool(out[0, 0, 3].isnan().all()) and bool(out[0, 0, 6].isnan().all())
+
+
+def test_what_masked_tokens_hold_does_not_matter():
+    """NaN keys and values that a row does not see, next to ones that it does, in one tile."""
+    page, D, n = 16, 64, 100
+    cache, table, g = filled((n,), page, 2, D, seed=6)
+    q = torch.randn(1, 4, 4, D, device=DEV, generator=g).bfloat16()
+    kw = dict(causal=True, window_size=(20, -1), sink_tokens=3)
+    good = mfa.flash_attn_with_kv4cache(q, cache, table, i32(n), **kw)
+    k = torch.full((1, 70, 2, D), float("nan"), device=DEV).bfloat16()
+    mfa.kv4_append(cache, k, k, table, i32(4))  # hidden from every row: tokens 4 .. 73
+    assert torch.equal(mfa.flash_attn_with_kv4cache(q, cache, table, i32(n), **kw), good)
+    one = k[:, :1]
+    mfa.kv4_append(cache, one, one, table, i32(77))  # only the first two rows see it
+    out = mfa.flash_attn_with_kv4cache(q, cache, table, i32(n), **kw)
+    assert bool(out[0, :2].isnan().all()) and torch.equal(out[0, 2:], good[0, 2:])
+    mfa.kv4_append(cache, one, one, table, i32(99))  # only the newest row sees it
+    out = mfa.flash_attn_with_kv4cache(q, cache, table, i32(n), **kw)
+    assert bool(out[0, 3].isnan().all()) and torch.equal(out[0, 2], good[0, 2])
+
+
+def test_bad_tables_and_lengths_are_reported():
+    lens = (90, 90)
+    cache, table, g = filled(lens, 16, 2, 64, seed=9)
+    for Lq in (1, 200):
+        q = torch.randn(2, Lq, 4, 64, device=DEV, generator=g).bfloat16()
+        good = mfa.flash_attn_with_kv4cache(q, cache, table, i32(*lens))
+        for page in (-1, cache.num_pages, 2**31 - 1):
+            bad = table.clone()
+            bad[1, 2] = page
+            out = mfa.flash_attn_with_kv4cache(q, cache, bad, i32(*lens))
+            reported()
+            assert torch.equal(out[0], good[0])
+            k, v = (torch.cat((t[:32], t[48:])) for t in
+                    (ref.tokens(cache, table[1], 90, keys) for keys in (True, False)))
+            check(out[1], ref.attention(q[1], k, v), v)
+        full = mfa.flash_attn_with_kv4cache(q, cache, table, i32(90, 96))
+        for n in (97, 2**31 - 1):  # more than the table covers: what it covers
+            out = mfa.flash_attn_with_kv4cache(q, cache, table, i32(90, n))
+            reported()
+            torch.testing.assert_close(out, full, atol=0, rtol=0, equal_nan=True)
+        out = mfa.flash_attn_with_kv4cache(q, cache, table, i32(90, -5))
+        reported()
+        assert bool((out[1] == 0).all()) and torch.equal(out[0], good[0])
+    empty = table[:, :0]
+    out = mfa.flash_attn_with_kv4cache(q, cache, empty, i32(0, 0))
+    _kernel.check_device_errors()
+    assert bool((out == 0).all())
+
+
+def test_strided_queries_and_empty_batches():
+    lens = (50, 33)
+    cache, table, g = filled(lens, 16, 2, 64, seed=10)
+    big = torch.randn(2, 6, 12, 65, device=DEV, generator=g).half()
+    q = big[:, ::2, 1:9, 1:]
+    want = mfa.flash_attn_with_kv4cache(q.contiguous(), cache, table, i32(*lens), causal=True)
+    assert torch.equal(mfa.flash_attn_with_kv4cache(q, cache, table, i32(*lens), causal=True), want)
+    wide = torch.zeros(2, 9, dtype=torch.int32, device=DEV)
+    wide[:, 2:2 + table.shape[1]] = table
+    assert torch.equal(mfa.flash_attn_with_kv4cache(q, cache, wide[:, 2:2 + table.shape[1]],
+                                                    i32(*lens), causal=True), want)
+    assert mfa.flash_attn_with_kv4cache(q[:, :0], cache, table, i32(*lens)).shape == (2, 0, 8, 64)
+    assert mfa.flash_attn_with_kv4cache(q[:0], cache, table[:0], i32()).shape == (0, 3, 8, 64)
+    mfa.kv4_append(cache, big[:0, :, :2, :64], big[:0, :, :2, :64], table[:0], i32())
+    assert mfa.kv4_gather(cache, table, i32(*lens), 0)[0].shape == (2, 0, 2, 64)
+
+
+def test_refusals_on_the_gpu():
+    cache, table, g = filled((40, 40), 16, 2, 64)
+    q = torch.zeros(2, 1, 4, 64, device=DEV, dtype=torch.float16)
+    kv = torch.zeros(2, 1, 2, 64, device=DEV, dtype=torch.float16)
+    n = i32(40, 40)
+    attend = [(q, cache, table, n.long()), (q, cache, table, i32(40)), (q, cache, table.long(), n),
+              (q, cache, table[:1], n), (q, cache, table.cpu(), n), (q, cache, table, n.cpu()),
+              (q[..., :32], cache, table, n), (q[:, :, :3], cache, table, n),
+              (q, cache, table.t().contiguous().t(), n), (q, cache, table[0], n)]
+    for args in attend:
+        with pytest.raises(ValueError):
+            mfa.flash_attn_with_kv4cache(*args)
+    for args in ((kv[:, :, :1], kv[:, :, :1], table, n), (kv[..., :32], kv[..., :32], table, n),
+                 (kv, kv, table, n.long()), (kv, kv, table, n, n.long()), (kv, kv.cpu(), table, n)):
+        with pytest.raises(ValueError):
+            mfa.kv4_append(cache, *args)
+    with pytest.raises(ValueError):
+        mfa.kv4_gather(cache, table, n, 4, starts=n.long())
+    out = mfa.flash_attn_with_kv4cache(q.requires_grad_(), cache, table, n)
+    with pytest.raises(NotImplementedError):
+        out.float().sum().backward()
+
+
+# ----------------------------------------------------------------------------- as they are used
+def test_serving_loop():
+    """Prompt, then token by token: norm and rotation, append, attention with a window and first
+    tokens, against the same steps in 64 bits on the held values; the prompt's own attention is
+    the framework's dense forward with the same mask."""
+    B, Hq, Hkv, D, page, prompt = 2, 8, 2, 128, 16, 45
+    steps, window, sink = 20, (24, -1), 3
+    g = torch.Generator(device=DEV).manual_seed(11)
+    table, pages = table_of(B, 5)
+    cache = dirty(mfa.kv4_cache(pages, page, Hkv, D, DEV))
+    f = 1e4 ** (-torch.arange(0, D, 2, device=DEV, dtype=torch.float64) / D)
+    angle = torch.arange(100, device=DEV, dtype=torch.float64)[:, None] * f
+    cos, sin = angle.cos().float(), angle.sin().float()
+    lens = i32(0, 0)
+    for step in range(steps):
+        n = prompt if step == 0 else 1
+        qkv = torch.randn(B, n, Hq + 2 * Hkv, D, device=DEV, generator=g).bfloat16()
+        pos = lens[:, None] + torch.arange(n, device=DEV)
+        q, k = mfa.qk_norm_rope(qkv[:, :, :Hq], qkv[:, :, Hq:Hq + Hkv], None, None, cos, sin, pos)
+        v = qkv[:, :, Hq + Hkv:]
+        mfa.kv4_append(cache, k, v, table, lens)
+        lens += n
+        out = mfa.flash_attn_with_kv4cache(q, cache, table, lens, causal=True, window_size=window,
+                                           sink_tokens=sink)
+        m = prompt + step
+        hk, hv = mfa.kv4_gather(cache, table, lens, m)
+        dense = mfa.flash_attn_func(q, hk, hv, causal=True, window_size=window, sink_tokens=sink)
+        for b in range(B):
+            assert torch.equal(hk[b, m - n:].double(), ref.held(k[b]))
+            want = ref.attention(q[b], hk[b], hv[b], True, window, sink=sink)
+            check(out[b], want, hv[b])
+        # the dense forward rounds its probabilities to bf16 (half a step each) and its output once
+        top = float(hv.abs().max())
+        torch.testing.assert_close(out, dense, atol=2 * top * 2**-8, rtol=2**-7)
+    _kernel.check_device_errors()
+
+
+def test_captured_steps_replayed_together():
+    """Two decode steps with splits, captured on one stream, replayed on two: each graph has its
+    own workspace, and lengths are read at replay."""
+    lens = (6000,)
+    sets = []
+    for seed in (1, 2):
+        cache, table, g = filled((6100,), 64, 2, 128, seed=seed)
+        q = torch.randn(1, 1, 16, 128, device=DEV, generator=g).bfloat16()
+        kv = torch.randn(1, 1, 2, 128, device=DEV, generator=g).bfloat16()
+        sets.append((cache, table, q, kv, i32(*lens)))
+
+    def step(cache, table, q, kv, n):
+        mfa.kv4_append(cache, kv, kv, table, n)
+        n += 1
+        return mfa.flash_attn_with_kv4cache(q, cache, table, n, causal=True)
+
+    side = torch.cuda.Stream()
+    graphs, outs = [], []
+    for s in sets:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            outs.append(step(*s))
+        graphs.append(graph)
+    for s in sets:
+        s[4].fill_(lens[0])  # capture ran nothing
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    for _ in range(30):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for (cache, table, q, kv, n), out in zip(sets, outs):
+        assert n.item() == lens[0] + 30
+        want = mfa.flash_attn_with_kv4cache(q, cache, table, n, causal=True)
+        assert torch.equal(out, want)
+        k, v = (ref.tokens(cache, table[0], n.item(), keys) for keys in (True, False))
+        assert torch.equal(k[-30:], ref.held(kv[0]).expand(30, -1, -1))
+        check(out[0], ref.attention(q[0], k, v, True), v)
+    _kernel.check_device_errors()
+
+
+def test_two_threads_on_two_streams():
+    import threading
+    cache, table, g = filled((5000,), 64, 2, 64, seed=12)
+    qs = [torch.randn(1, 1, 8, 64, device=DEV, generator=g).half() for _ in range(2)]
+    n = i32(5000)
+    want = [mfa.flash_attn_with_kv4cache(q, cache, table, n) for q in qs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(100):
+                out = mfa.flash_attn_with_kv4cache(qs[i], cache, table, n)
+                torch.cuda.current_stream().synchronize()
+                if not torch.equal(out, want[i]):
+                    wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
