@@ -331,7 +331,7 @@ int mfa_kv4_gather(const mfa_kv4_cache* c, const mfa_kv4_rows* r, void* cuda_str
 
 typedef struct mfa_kv4_fwd_params {
   const void* q;      /* [B, Lq, Hq, D], any (batch, seq, head) strides, last dim stride 1 */
-  void* o;            /* [B, Lq, Hq, D] */
+  void* o;            /* [B, Lq, Hq, D], 8-byte aligned, strides multiples of 4 elements */
   int64_t q_stride[3];
   int64_t o_stride[3];
   const int32_t* seqlens; /* device [B]: keys of each sequence, the Lq newest rows' among them */

@@ -69,6 +69,13 @@ __device__ __forceinline__ uint32_t e4m3x2_f16(uint32_t two_bytes) {
       : "r"(two_bytes));
   return d;
 }
+// The scales in a word's four bytes as two pairs of fp16.
+__device__ __forceinline__ void e4m3x4_f16(uint32_t w, uint32_t* d) {
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %1, hi;\n\t}"
+      : "=r"(d[0]), "=r"(d[1])
+      : "r"(w));
+}
 __device__ __forceinline__ float f16_lo(uint32_t h2) {
   return __low2float(*reinterpret_cast<const __half2*>(&h2));
 }
@@ -216,6 +223,13 @@ __global__ void __launch_bounds__(128) kv4_gather_kernel(const Kv4Cache c, const
 //           scale is added up, so the key scales cost no rounding.
 //   values: the scale of (token, group) multiplies the probability, in fp16, before the
 //           instruction of that group (its rounding, 2^-11 of each term, is that of fp16 P).
+//
+// A CTA is four consumer warps and a producer warp. The producer copies blocks of 64 tokens (codes
+// and scales, one bulk copy each per page piece) into a ring; each consumer takes 16 of the tokens.
+// Work is shared out by blocks, not by sequences: the blocks of every (sequence, KV head, tile of
+// query rows) that has visible keys stand in one line, which the CTAs of one wave cut into equal
+// shares. A share that covers a whole unit writes its rows; one that does not leaves a partial
+// result, and kv4_join adds those up. Lengths are read on the device.
 struct Kv4Args {
   Kv4Cache c;
   const void* q;
@@ -223,35 +237,131 @@ struct Kv4Args {
   int64_t q_sb, q_ss, q_sh, o_sb, o_ss, o_sh;
   const int* seqlens;
   int Lq, Hq, group, bf16;
+  int q_vec8;  // every 4 dims of a query row can be read at once
   float scale_l2;  // scale * k_unit * log2(e) (softcap: scale * k_unit / softcap)
   float softcap;
   int causal, wl, wr, sink;
   const float* alibi;
-  int row_blocks, splits;
-  float* ws_o;    // [split][B * Lq * Hq][D], each normalised by its own sum
-  float* ws_lse;  // [split][B * Lq * Hq], log2
+  int row_blocks;
+  // workspace: [0] blocks per CTA, then where each sequence's blocks begin; partial sums of two
+  // units per CTA, [CTA][2][rows][D], and their references and sums [CTA][2][rows]
+  int* ws_line;
+  float *ws_o, *ws_m, *ws_l;
 };
 
-constexpr int kAttnWarps = 4;
+constexpr int kAttnWarps = 4;                  // consumer warps
+constexpr int kAttnThreads = 32 * kAttnWarps + 32;
+constexpr int kBlockTokens = 16 * kAttnWarps;  // tokens of a block
+constexpr int kAttnStages = 4;
+constexpr int kMinShare = 4;   // blocks per CTA at least: below, joining costs more than it gives
+#ifndef KV4_UNIT
+#define KV4_UNIT 4
+#endif
+constexpr int kUnitCost = KV4_UNIT;  // beginning and ending a unit takes about as long as so many blocks
+#ifndef KV4_C1
+#define KV4_C1 3
+#endif
+#ifndef KV4_C2
+#define KV4_C2 3
+#endif
+__host__ __device__ constexpr int kv4_ctas(int nt) { return nt == 1 ? KV4_C1 : KV4_C2; }  // per SM
 constexpr float kGrow = 7.f;   // a row's reference is renewed when a score passes it by 2^7
 constexpr float kBelow = 3.f;  // and is then set 2^3 below the new maximum
 
 struct Kv4Range {
   int lo, hi, sk;
 };
-// Keys that the row at position i sees: [lo, hi) and [0, sk).
+// Keys that the row at position i < Lq sees: [lo, hi) and [0, sk). Written so that nothing passes
+// 32 bits: the row's centre i + len - Lq is below len.
 __device__ __forceinline__ Kv4Range kv4_range(const Kv4Args& a, int len, int i) {
-  const int64_t centre = (int64_t)i + len - a.Lq;
-  int64_t lo = a.wl >= 0 ? centre - a.wl : 0, hi = len;
-  if (a.causal) hi = min(hi, centre + 1);
-  if (a.wr >= 0) hi = min(hi, centre + a.wr + 1);
-  hi = max(hi, (int64_t)0);
+  const int centre = len - (a.Lq - i);
   Kv4Range r;
-  r.lo = (int)min(max(lo, (int64_t)0), (int64_t)len);
-  r.hi = (int)hi;
-  r.sk = (int)min((int64_t)a.sink, hi);
+  r.lo = a.wl >= 0 && centre > a.wl ? centre - a.wl : 0;
+  r.hi = a.causal ? centre + 1 : len;
+  if (a.wr >= 0 && a.wr < len - 1 - centre) r.hi = min(r.hi, centre + a.wr + 1);
+  r.hi = max(r.hi, 0);
+  r.sk = min(a.sink, r.hi);
   return r;
 }
+
+__device__ __forceinline__ int kv4_length(const Kv4Args& a, int b) {
+  const int room = a.c.max_pages << a.c.page_shift;  // below 2^31
+  const int len = a.seqlens[b];
+  return len < 0 ? 0 : min(len, room);
+}
+
+// The blocks that a tile of query rows sees: [0, s1) hold first keys, [w0, w0 + n - s1) the window.
+struct Kv4Span {
+  Kv4Range first, last;  // of the tile's first and last row
+  int s1, w0, n;
+  __device__ __forceinline__ int at(int j) const { return j < s1 ? j : w0 + j - s1; }
+};
+template <int kRows>
+__device__ __forceinline__ Kv4Span kv4_span(const Kv4Args& a, int len, int rb) {
+  const int rows = a.Lq * a.group, r0 = rb * kRows;
+  Kv4Span s;
+  s.first = kv4_range(a, len, r0 / a.group);
+  s.last = kv4_range(a, len, (min(r0 + kRows, rows) - 1) / a.group);
+  constexpr unsigned kT = kBlockTokens;
+  const bool any = s.last.hi > s.first.lo;
+  s.w0 = (unsigned)(any ? s.first.lo : s.first.lo + (int)kT - 1) / kT;
+  const int w1 = any ? (int)((unsigned)(s.last.hi + (int)kT - 1) / kT) : s.w0;
+  s.s1 = min((int)((unsigned)(s.last.sk + (int)kT - 1) / kT), s.w0);
+  s.n = s.s1 + w1 - s.w0;
+  return s;
+}
+// A unit's room in the line: its cost, then its blocks.
+__device__ __forceinline__ int kv4_room(int n) { return n > 0 ? n + kUnitCost : 0; }
+// Room of one KV head of a sequence.
+template <int kRows>
+__device__ __forceinline__ int kv4_head_room(const Kv4Args& a, int len) {
+  int n = 0;
+#pragma unroll 1
+  for (int rb = 0; rb < a.row_blocks; ++rb) n += kv4_room(kv4_span<kRows>(a, len, rb).n);
+  return n;
+}
+
+// Where a CTA stands in the line of blocks.
+template <int kRows>
+struct Kv4Walk {
+  int b, hk, rb, j;  // unit, block within it (below 0: the unit's cost is not paid yet)
+  int left;          // what is left of the share
+  int len;
+  Kv4Span span;
+  int take;          // blocks of this unit that are this CTA's: [j, j + take)
+
+  __device__ __forceinline__ void look(const Kv4Args& a) {
+    len = kv4_length(a, b);
+    span = kv4_span<kRows>(a, len, rb);
+    take = 0;
+    if (span.n > 0) {
+      if (j < 0) {
+        left += j;
+        j = 0;
+      }
+      take = max(0, min(span.n - j, left));
+    }
+  }
+  __device__ __forceinline__ void next(const Kv4Args& a) {
+    left -= take;
+    take = 0;
+#pragma unroll 1
+    while (left > 0 && take == 0) {
+      j = -kUnitCost;
+      if (++rb == a.row_blocks) {
+        rb = 0;
+        if (++hk == a.c.Hkv) {
+          hk = 0;
+          if (++b >= a.c.B) {
+            left = 0;
+            return;
+          }
+        }
+      }
+      look(a);
+    }
+  }
+};
 
 // tanh from its exponential form; 2^inf and 2^-inf give 1 and -1, a NaN stays one.
 __device__ __forceinline__ float tanh_any(float y) {
@@ -277,8 +387,23 @@ __device__ __forceinline__ uint32_t h2mul(uint32_t a, uint32_t b) {
   const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
   return *reinterpret_cast<const uint32_t*>(&v);
 }
+// Untiled bulk copy (no multicast) of n bytes, completing on an mbarrier; both sides 16-byte
+// aligned, n a multiple of 16.
+__device__ __forceinline__ void bulk_load(uint8_t* dst, const uint8_t* src, uint32_t n,
+                                          uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          smem_u32(dst)),
+      "l"(src), "r"(n), "r"(smem_u32(bar))
+      : "memory");
+}
 
-// N bytes (4, 8 or 16) to words.
+// Whether one of four e4m3 bytes is NaN (0x7f, 0xff).
+__device__ __forceinline__ bool has_nan_scale(uint32_t w) {
+  return (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
+}
+
+// N bytes (4, 8 or 16) of shared memory to words.
 template <int N>
 __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* w) {
   if constexpr (N == 16) {
@@ -292,341 +417,594 @@ __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* w) {
   }
 }
 
-// A lane's share of 16 tokens: keys of tokens g and g + 8, values of tokens 2t, 2t + 1, 2t + 8 and
-// 2t + 9 (lane = 4 g + t).
-template <int D>
-struct Kv4Tile {
-  uint32_t k[2][D / 32], v[4][D / 64], ks[2][D / 64], vs[4][D / 64];
-  int token;  // first token
-  bool ok;    // its page exists
-};
-
-template <int D>
-__device__ __forceinline__ void load_tile(const Kv4Args& a, int b, int hk, int tile, int lane,
-                                          Kv4Tile<D>& f) {
-  const Kv4Cache& c = a.c;
-  const int g = lane >> 2, t = lane & 3;
-  f.token = tile * 16;
-  const int64_t row = kv4_row(c, b, f.token);
-  f.ok = row >= 0;
-  if (!f.ok) {
-    if (lane == 0) kv4_report(c);
-#pragma unroll
-    for (int i = 0; i < D / 64; ++i) {
-      f.k[0][2 * i] = f.k[0][2 * i + 1] = f.k[1][2 * i] = f.k[1][2 * i + 1] = 0;
-      f.ks[0][i] = f.ks[1][i] = 0;
-#pragma unroll
-      for (int n = 0; n < 4; ++n) f.v[n][i] = f.vs[n][i] = 0;
-    }
-    return;
+// Four columns of an output row from their weighted sums and the sum of the weights.
+__device__ __forceinline__ void kv4_store(const Kv4Args& a, int64_t at, float4 val, float sum) {
+  const float f = sum == 0.f ? 0.f : a.c.v_unit / sum;
+  if (sum == 0.f) val = make_float4(0.f, 0.f, 0.f, 0.f);
+  uint2 w;
+  if (a.bf16) {
+    w.x = pack2<true>(val.x * f, val.y * f);
+    w.y = pack2<true>(val.z * f, val.w * f);
+  } else {
+    w.x = pack2<false>(val.x * f, val.y * f);
+    w.y = pack2<false>(val.z * f, val.w * f);
   }
-  const int64_t r0 = row + ((int64_t)hk << c.page_shift);
-#pragma unroll
-  for (int n = 0; n < 2; ++n) {
-    const int64_t r = r0 + g + 8 * n;
-    load_words<D / 8>(c.k + r * (D / 2) + t * (D / 8), f.k[n]);
-    load_words<D / 16>(c.ks + r * (D / 16), f.ks[n]);
-  }
-#pragma unroll
-  for (int n = 0; n < 4; ++n) {
-    const int64_t r = r0 + 2 * t + (n & 1) + 8 * (n >> 1);
-    load_words<D / 16>(c.v + r * (D / 2) + g * (D / 16), f.v[n]);
-    load_words<D / 16>(c.vs + r * (D / 16), f.vs[n]);
-  }
+  *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.o) + at) = w;
 }
 
-// A CTA serves 8 NT query rows of one (sequence, KV head) and one share of its visible tokens; its
-// warps take tiles of 16 tokens in turn, each with its own softmax reference, and join at the end.
 template <int D, int NT>
-__global__ void __launch_bounds__(32 * kAttnWarps) kv4_attn(const __grid_constant__ Kv4Args a) {
+struct Kv4Smem {
+  static constexpr int kRows = 8 * NT;
+  static constexpr uint32_t kCodes = kBlockTokens * D / 2, kScales = kBlockTokens * D / 16;
+  static constexpr uint32_t kStage = 2 * kCodes + 2 * kScales;  // K, V, K scales, V scales
+  alignas(128) uint8_t ring[kAttnStages][kStage];
+  float o[kAttnWarps][kRows][D + 4];  // the warps' sums, to be joined
+  float m[kAttnWarps][kRows], l[kAttnWarps][kRows];
+  uint64_t full[kAttnStages], empty[kAttnStages];
+  int bad[kAttnStages];  // bit i: the page of the block's tokens [16 i, 16 i + 16) does not exist
+  int scan[kAttnThreads / 32];
+  int b, hk, rb, j, share;
+  int abort;
+};
+
+template <int D, int NT>
+__global__ void __launch_bounds__(kAttnThreads, kv4_ctas(NT))
+    kv4_attn(const __grid_constant__ Kv4Args a) {
   constexpr int NG = D / 16, kRows = 8 * NT;
-  __shared__ float s_o[kAttnWarps][kRows][D + 4];
-  __shared__ float s_m[kAttnWarps][kRows], s_l[kAttnWarps][kRows];
+  using Smem = Kv4Smem<D, NT>;
+  extern __shared__ uint8_t smem_raw[];
+  Smem& sm = *reinterpret_cast<Smem*>(smem_raw + (((smem_u32(smem_raw) + 127u) & ~127u) -
+                                                  smem_u32(smem_raw)));
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const Kv4Cache& c = a.c;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  int idx = blockIdx.x;
-  const int rb = idx % a.row_blocks;
-  idx /= a.row_blocks;
-  const int split = idx % a.splits;
-  idx /= a.splits;
-  const int hk = idx % c.Hkv, b = idx / c.Hkv;
-  const int rows = a.Lq * a.group, r0 = rb * kRows;
-  const int64_t room = (int64_t)c.max_pages << c.page_shift;
-  int len = a.seqlens[b];
-  if (len < 0 || len > room) {
-    if (threadIdx.x == 0) kv4_report(c);
-    len = len < 0 ? 0 : (int)room;
-  }
-  // tiles of 16 tokens: [0, s1) hold first keys, [w0, w0 + n - s1) the window
-  const int i_last = (min(r0 + kRows, rows) - 1) / a.group;
-  const Kv4Range first = kv4_range(a, len, r0 / a.group), last = kv4_range(a, len, i_last);
-  const bool any = last.hi > first.lo;
-  const int w0 = any ? first.lo / 16 : (first.lo + 15) / 16;
-  const int w1 = any ? (last.hi + 15) / 16 : w0;
-  const int s1 = min((last.sk + 15) / 16, w0);
-  const int n = s1 + w1 - w0;
-  const int per = (n + a.splits - 1) / a.splits;
-  const int j0 = min(n, split * per), j1 = min(n, j0 + per);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  // query fragments: lane (g, t) has dims 16 i + 4 t .. + 3 of row g of each tile of 8 rows
-  uint32_t qf[NT][NG][2];
-  float inv_f[NT];  // what a row was multiplied by, inverted
+  // ---- where this CTA's share begins: sums over the sequences, each thread a run of them
+  {
+    const int run = (c.B + kAttnThreads - 1) / kAttnThreads;
+    const int b0 = min(c.B, (int)threadIdx.x * run), b1 = min(c.B, b0 + run);
+    int mine = 0;
+    for (int b = b0; b < b1; ++b)
+      mine += kv4_head_room<kRows>(a, kv4_length(a, b)) * c.Hkv;  // below 2^31 in all
+    int upto = mine;
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int r = r0 + nt * 8 + g;
-    float x[NG][4];
-    float top = 0.f;
-#pragma unroll
-    for (int i = 0; i < NG; ++i) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[i][e] = 0.f;
-      if (r < rows) {
-        const int64_t at = b * a.q_sb + (r / a.group) * a.q_ss +
-                           (int64_t)(hk * a.group + r % a.group) * a.q_sh + 16 * i + 4 * t;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          x[i][e] = a.bf16 ? to_f32(reinterpret_cast<const __nv_bfloat16*>(a.q)[at + e])
-                           : to_f32(reinterpret_cast<const __half*>(a.q)[at + e]);
+    for (int d = 1; d < 32; d <<= 1) {
+      const int x = __shfl_up_sync(kFull, upto, d);
+      if (lane >= d) upto += x;
+    }
+    if (lane == 31) sm.scan[warp] = upto;
+    if (threadIdx.x == 0) {
+      sm.abort = 0;
+      for (int i = 0; i < kAttnStages; ++i) {
+        mbar_init(&sm.full[i], 1);
+        mbar_init(&sm.empty[i], kAttnWarps);
       }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(x[i][e]));
+      fence_mbar_init();
     }
-    top = fmaxf(top, __shfl_xor_sync(kFull, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(kFull, top, 2));
-    // exponent of the row's largest value; f = 2^(10 - e) brings it to [2^10, 2^11)
-    int e = (int)((__float_as_uint(top) >> 23) & 255u) - 127;
-    if (e > 127 || top == 0.f) e = 10;  // infinite, or a row of zeros: as it is
-    e = max(e, -100);
-    const float f = __uint_as_float((uint32_t)(127 + 10 - e) << 23);
-    inv_f[nt] = __uint_as_float((uint32_t)(127 - 10 + e) << 23);
+    __syncthreads();
+    int total = 0, before = upto - mine;
 #pragma unroll
-    for (int i = 0; i < NG; ++i) {
-      qf[nt][i][0] = h2(x[i][0] * f, x[i][1] * f);
-      qf[nt][i][1] = h2(x[i][2] * f, x[i][3] * f);
+    for (int w = 0; w < kAttnThreads / 32; ++w) {
+      if (w < warp) before += sm.scan[w];
+      total += sm.scan[w];
     }
+    const int share = max(kMinShare, (int)(((unsigned)total + gridDim.x - 1) / gridDim.x));
+    if (blockIdx.x == 0) {  // for kv4_join, and what is wrong with the lengths
+      if (threadIdx.x == 0) a.ws_line[0] = share;
+      int at = before;
+      for (int b = b0; b < b1; ++b) {
+        a.ws_line[1 + b] = at;
+        const int len = a.seqlens[b], held = kv4_length(a, b);
+        at += kv4_head_room<kRows>(a, held) * c.Hkv;
+        if (len != held) kv4_report(c);
+      }
+    }
+    const int64_t begin = (int64_t)share * blockIdx.x;
+    if (begin >= total) return;  // all threads alike
+    const int start = (int)begin;
+    if (start >= before && start < before + mine) {
+      int x = start - before, b = b0, len, head;
+      while (true) {
+        len = kv4_length(a, b);
+        head = kv4_head_room<kRows>(a, len);
+        if (x < head * c.Hkv) break;
+        x -= head * c.Hkv;
+        ++b;
+      }
+      sm.b = b;
+      sm.hk = (int)((unsigned)x / (unsigned)head);
+      x -= sm.hk * head;
+      int rb = 0;
+      for (int n; x >= (n = kv4_room(kv4_span<kRows>(a, len, rb).n)); ++rb) x -= n;
+      sm.rb = rb;
+      sm.j = x - kUnitCost;
+      sm.share = min(share, total - start);
+    }
+    __syncthreads();
   }
-  // this lane's score columns are rows 2t and 2t + 1 of each tile of 8
-  float sc[NT][2], slope[NT][2], m[NT][2], l[NT][2];
-  int centre[NT][2];
-  Kv4Range seen[NT][2];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      sc[nt][e] = a.scale_l2 * __shfl_sync(kFull, inv_f[nt], 4 * (2 * t + e));
-      const int r = r0 + nt * 8 + 2 * t + e;
-      seen[nt][e] = kv4_range(a, len, min(r, rows - 1) / a.group);
-      centre[nt][e] = min(r, rows - 1) / a.group + len - a.Lq;
-      slope[nt][e] = a.alibi != nullptr && r < rows
-                         ? a.alibi[(int64_t)b * a.Hq + hk * a.group + r % a.group] *
-                               1.4426950408889634f
-                         : 0.f;
-      m[nt][e] = -INFINITY;
-      l[nt][e] = 0.f;
-    }
-  float o[NT][NG][4];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int i = 0; i < NG; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[nt][i][e] = 0.f;
+  Kv4Walk<kRows> walk;
+  walk.b = sm.b;
+  walk.hk = sm.hk;
+  walk.rb = sm.rb;
+  walk.j = sm.j;
+  walk.left = sm.share;
+  walk.look(a);
+  volatile int* abort_flag = &sm.abort;
 
-  auto tile_of = [&](int j) { return j < s1 ? j : w0 + j - s1; };
-  Kv4Tile<D> f, next;
-  if (j0 + warp < j1) load_tile<D>(a, b, hk, tile_of(j0 + warp), lane, f);
-  for (int j = j0 + warp; j < j1; j += kAttnWarps) {
-    if (j + kAttnWarps < j1) load_tile<D>(a, b, hk, tile_of(j + kAttnWarps), lane, next);
-    // ---- scores of 16 tokens: s[nt][0, 1] token g, s[nt][2, 3] token g + 8
-    float s[NT][4];
+  if (warp == kAttnWarps) {
+    // ---------------------------------------------------------------- producer
+    // A block is one piece, or as many as it has pages. The lanes look up the pages of the next 32
+    // pieces at once, a batch ahead of the one whose copies are being issued.
+    const int piece = min(kBlockTokens, 1 << c.page_shift);
+    const int pshift = min(__ffs(kBlockTokens) - 1, c.page_shift);         // log2(piece)
+    const int bshift = __ffs(kBlockTokens) - 1 - pshift, batch = 32 >> bshift;  // blocks
+    auto page_of = [&](const Kv4Walk<kRows>& w) {  // of the batch that begins at w.j
+      const int j = w.j + (lane >> bshift);
+      const int t = w.span.at(j) * kBlockTokens + ((lane & ((1 << bshift) - 1)) << pshift);
+      // tokens past the length may have no page: -1 there
+      const bool on = w.take > 0 && lane < w.take << bshift && t < w.len;
+      return on ? c.table[(int64_t)w.b * c.table_stride + (t >> c.page_shift)] : -2;
+    };
+    auto skip = [&](Kv4Walk<kRows>& w) {  // to the next batch
+      if (w.take > batch) {
+        w.j += batch;
+        w.left -= batch;
+        w.take -= batch;
+      } else {
+        w.next(a);
+      }
+    };
+    int it = 0;
+    int pages = page_of(walk);
+    Kv4Walk<kRows> ahead = walk;
+    bool ok = true;
+    while (walk.take > 0 && ok) {
+      skip(ahead);
+      const int pages_next = page_of(ahead);
+      const int n = min(walk.take, batch);
+      const int64_t base_row = (int64_t)walk.hk << c.page_shift;
+#pragma unroll 1
+      for (int x = 0; x < n; ++x, ++it) {
+        const int slot = it % kAttnStages;
+        const uint32_t phase = (uint32_t)(it / kAttnStages) & 1u;
+        const int page = __shfl_sync(kFull, pages, (x << bshift) + (lane & ((1 << bshift) - 1)));
+        ok = __all_sync(kFull, mbar_wait(&sm.empty[slot], phase ^ 1u, abort_flag));
+        if (!ok) break;
+        const bool good = lane < 1 << bshift && page >= 0 && page < c.num_pages;
+        if (lane < 1 << bshift && page != -2 && !good) kv4_report(c);
+        const unsigned have = __ballot_sync(kFull, good);
+        if (lane == 0) {
+          int bad = 0;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
-#pragma unroll
-    for (int w = 0; w < NG / 2; ++w) {  // a word: two groups
-      uint32_t ka[4], kb[4];
-      e2m1x8_f16(f.k[0][w], ka);
-      e2m1x8_f16(f.k[1][w], kb);
-      const uint32_t sa = e4m3x2_f16(f.ks[0][w / 2] >> (16 * (w & 1)));
-      const uint32_t sb = e4m3x2_f16(f.ks[1][w / 2] >> (16 * (w & 1)));
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint32_t frag[4] = {ka[2 * i], kb[2 * i], ka[2 * i + 1], kb[2 * i + 1]};
-        const float fa = i ? f16_hi(sa) : f16_lo(sa), fb = i ? f16_hi(sb) : f16_lo(sb);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float x[4] = {0.f, 0.f, 0.f, 0.f};
-          mma16816(x, frag, qf[nt][2 * w + i][0], qf[nt][2 * w + i][1]);
-          s[nt][0] = fmaf(fa, x[0], s[nt][0]);
-          s[nt][1] = fmaf(fa, x[1], s[nt][1]);
-          s[nt][2] = fmaf(fb, x[2], s[nt][2]);
-          s[nt][3] = fmaf(fb, x[3], s[nt][3]);
+          for (int i = 0; i < kAttnWarps; ++i)
+            bad |= (have >> (16 * i >> pshift) & 1 ? 0 : 1) << i;
+          sm.bad[slot] = bad;
+          mbar_expect_tx(&sm.full[slot], (uint32_t)(__popc(have) << pshift) * (D + D / 8));
+        }
+        __syncwarp();
+        if (good) {
+          const int y = lane << pshift;  // the piece's first token within the block
+          const int t = walk.span.at(walk.j + x) * kBlockTokens + y;
+          const int64_t row = (((int64_t)page * c.Hkv) << c.page_shift) + base_row +
+                              (t & ((1 << c.page_shift) - 1));
+          uint8_t* dst = sm.ring[slot];
+          bulk_load(dst + y * (D / 2), c.k + row * (D / 2), piece * (D / 2), &sm.full[slot]);
+          bulk_load(dst + Smem::kCodes + y * (D / 2), c.v + row * (D / 2), piece * (D / 2),
+                    &sm.full[slot]);
+          dst += 2 * Smem::kCodes;
+          bulk_load(dst + y * (D / 16), c.ks + row * (D / 16), piece * (D / 16), &sm.full[slot]);
+          bulk_load(dst + Smem::kScales + y * (D / 16), c.vs + row * (D / 16), piece * (D / 16),
+                    &sm.full[slot]);
         }
       }
+      walk = ahead;
+      pages = pages_next;
     }
-    // ---- logits in log2 units, masks, probabilities
-    uint32_t pb[NT][2], pm[NT][2];
-    bool grow = false;
+    // every copy has landed before the CTA's shared memory is given back
+    for (int i = max(0, it - kAttnStages); i < it; ++i)
+      mbar_wait_drain(&sm.full[i % kAttnStages], (uint32_t)(i / kAttnStages) & 1u);
+    if (lane == 0 && sm.abort && c.err != nullptr) atomicExch(c.err, MFA_ERR_TIMEOUT);
+    return;
+  }
+
+  // ------------------------------------------------------------------ consumers
+  const int g = lane >> 2, t = lane & 3;
+  // Row r of a tile's 16 is token r ^ ((r >> 1) & 1): the tokens whose values a lane reads at once
+  // then lie in both halves of the banks.
+  const int key_of = g ^ ((g >> 1) & 1);
+  const int rows = a.Lq * a.group;
+  const bool general = a.softcap > 0.f || a.alibi != nullptr;
+  int it = 0;
+  bool ok = true;  // after a wait that gave up: no more tiles, but every barrier is still met
+  while (walk.take > 0) {
+    const int b = walk.b, hk = walk.hk, r0 = walk.rb * kRows, len = walk.len;
+    // query fragments: lane (g, t) has dims 16 i + 4 t .. + 3 of row g of each tile of 8 rows
+    uint32_t qf[NT][NG][2];
+    float inv_f[NT];  // what a row was multiplied by, inverted
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      bool vis[4];
+      const int r = r0 + nt * 8 + g;
+      float x[NG][4];
+      float top = 0.f;
+      const int64_t at = b * a.q_sb + (r / a.group) * a.q_ss +
+                         (int64_t)(hk * a.group + r % a.group) * a.q_sh + 4 * t;
+      const uint16_t* qp = reinterpret_cast<const uint16_t*>(a.q) + at;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int col = e & 1, key = f.token + g + 8 * (e >> 1);
-        float x = s[nt][e] * sc[nt][col];
-        if (a.softcap > 0.f) x = a.softcap * 1.4426950408889634f * tanh_any(x);
-        if (a.alibi != nullptr) x -= slope[nt][col] * fabsf((float)(centre[nt][col] - key));
-        const Kv4Range& r = seen[nt][col];
-        vis[e] = f.ok && (key >= r.lo || key < r.sk) && key < r.hi;
-        s[nt][e] = vis[e] ? x : -INFINITY;
-        grow = grow || s[nt][e] > m[nt][col] + kGrow;
+      for (int i = 0; i < NG; ++i) {
+        uint2 raw = make_uint2(0, 0);
+        if (r < rows) {
+          if (a.q_vec8) {
+            raw = *reinterpret_cast<const uint2*>(qp + 16 * i);
+          } else {
+            raw.x = qp[16 * i] | (uint32_t)qp[16 * i + 1] << 16;
+            raw.y = qp[16 * i + 2] | (uint32_t)qp[16 * i + 3] << 16;
+          }
+        }
+        if (a.bf16) {
+          x[i][0] = __uint_as_float(raw.x << 16);
+          x[i][1] = __uint_as_float(raw.x & 0xffff0000u);
+          x[i][2] = __uint_as_float(raw.y << 16);
+          x[i][3] = __uint_as_float(raw.y & 0xffff0000u);
+        } else {
+          x[i][0] = f16_lo(raw.x);
+          x[i][1] = f16_hi(raw.x);
+          x[i][2] = f16_lo(raw.y);
+          x[i][3] = f16_hi(raw.y);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(x[i][e]));
       }
-      pm[nt][0] = transpose8x8((vis[0] ? 0xffffu : 0u) | (vis[1] ? 0xffff0000u : 0u));
-      pm[nt][1] = transpose8x8((vis[2] ? 0xffffu : 0u) | (vis[3] ? 0xffff0000u : 0u));
+      top = fmaxf(top, __shfl_xor_sync(kFull, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(kFull, top, 2));
+      // exponent of the row's largest value; f = 2^(10 - e) brings it to [2^10, 2^11)
+      int e = (int)((__float_as_uint(top) >> 23) & 255u) - 127;
+      if (e > 127 || top == 0.f) e = 10;  // infinite, or a row of zeros: as it is
+      e = max(e, -100);
+      const float f = __uint_as_float((uint32_t)(127 + 10 - e) << 23);
+      inv_f[nt] = __uint_as_float((uint32_t)(127 - 10 + e) << 23);
+#pragma unroll
+      for (int i = 0; i < NG; ++i) {
+        qf[nt][i][0] = h2(x[i][0] * f, x[i][1] * f);
+        qf[nt][i][1] = h2(x[i][2] * f, x[i][3] * f);
+      }
     }
-    if (__any_sync(kFull, grow)) {
+    // this lane's score columns are rows 2t and 2t + 1 of each tile of 8; m is the reference
+    // and m_sub what is subtracted (0 while there is none)
+    float sc[NT][2], m[NT][2], m_sub[NT][2], l[NT][2];
+    float o[NT][NG][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float top = fmaxf(s[nt][e], s[nt][e + 2]);
+      for (int e = 0; e < 2; ++e) {
+        sc[nt][e] = a.scale_l2 * __shfl_sync(kFull, inv_f[nt], 4 * (2 * t + e));
+        m[nt][e] = -INFINITY;
+        m_sub[nt][e] = l[nt][e] = 0.f;
+      }
 #pragma unroll
-          for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, d));
-          if (top > m[nt][e] + kGrow) {
-            const float fresh = top - kBelow;
-            const float factor = m[nt][e] == -INFINITY ? 0.f : ex2(m[nt][e] - fresh);
-            m[nt][e] = fresh;
-            l[nt][e] *= factor;
+      for (int i = 0; i < NG; ++i)
 #pragma unroll
-            for (int i = 0; i < NG; ++i) {
-              o[nt][i][e] *= factor;
-              o[nt][i][e + 2] *= factor;
+        for (int e = 0; e < 4; ++e) o[nt][i][e] = 0.f;
+    }
+
+    for (int j = walk.j; j < walk.j + walk.take; ++j, ++it) {
+      const int slot = it % kAttnStages;
+      ok = ok && __all_sync(kFull, mbar_wait(&sm.full[slot], (uint32_t)(it / kAttnStages) & 1u,
+                                             abort_flag));
+      if (!ok) break;
+      const int token = walk.span.at(j) * kBlockTokens + 16 * warp;
+      const bool bad = sm.bad[slot] >> warp & 1;
+      const Kv4Span& see = walk.span;
+      // all rows see all 16 tokens; some row sees some
+      const bool full = !bad && token + 16 <= see.first.hi &&
+                        (token >= see.last.lo || token + 16 <= see.first.sk);
+      const bool some = !bad && token < see.last.hi &&
+                        (token + 16 > see.first.lo || token < see.last.sk);
+      const uint8_t* base = sm.ring[slot];
+
+      if (some) {
+        const bool careful = general || !full;  // alike in all lanes
+        // ---- scores of 16 tokens: s[nt][0, 1] row g of the tile, s[nt][2, 3] row g + 8
+        float s[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
+        {
+          uint32_t k0[D / 32], k1[D / 32], s0[D / 64], s1[D / 64];
+          const uint8_t* kp = base + (16 * warp + key_of) * (D / 2) + t * (D / 8);
+          load_words<D / 8>(kp, k0);
+          load_words<D / 8>(kp + 8 * (D / 2), k1);
+          const uint8_t* sp2 = base + 2 * Smem::kCodes + (16 * warp + key_of) * (D / 16);
+          load_words<D / 16>(sp2, s0);
+          load_words<D / 16>(sp2 + 8 * (D / 16), s1);
+          uint32_t fs0[NG / 2], fs1[NG / 2];
+#pragma unroll
+          for (int w = 0; w < NG / 4; ++w) {
+            e4m3x4_f16(s0[w], fs0 + 2 * w);
+            e4m3x4_f16(s1[w], fs1 + 2 * w);
+          }
+#pragma unroll
+          for (int w = 0; w < NG / 2; ++w) {  // a word: two groups
+            uint32_t ka[4], kb[4];
+            e2m1x8_f16(k0[w], ka);
+            e2m1x8_f16(k1[w], kb);
+            const uint32_t sa = fs0[w], sb = fs1[w];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t frag[4] = {ka[2 * i], kb[2 * i], ka[2 * i + 1], kb[2 * i + 1]};
+              const float fa = i ? f16_hi(sa) : f16_lo(sa), fb = i ? f16_hi(sb) : f16_lo(sb);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                float x[4] = {0.f, 0.f, 0.f, 0.f};
+                mma16816(x, frag, qf[nt][2 * w + i][0], qf[nt][2 * w + i][1]);
+                s[nt][0] = fmaf(fa, x[0], s[nt][0]);
+                s[nt][1] = fmaf(fa, x[1], s[nt][1]);
+                s[nt][2] = fmaf(fb, x[2], s[nt][2]);
+                s[nt][3] = fmaf(fb, x[3], s[nt][3]);
+              }
             }
           }
         }
-    }
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float p[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float ref = m[nt][e & 1] == -INFINITY ? 0.f : m[nt][e & 1];
-        p[e] = ex2(s[nt][e] - ref);
-        l[nt][e & 1] += p[e];
-      }
-      pb[nt][0] = transpose8x8(h2(p[0], p[1]));  // tokens 2t, 2t + 1 of row g
-      pb[nt][1] = transpose8x8(h2(p[2], p[3]));  // tokens 2t + 8, 2t + 9
-    }
-    // ---- values: a byte of two tokens' codes of one dim makes one operand register
-#pragma unroll
-    for (int w = 0; w < NG / 4; ++w) {  // a word: four groups
-      uint32_t va[4], vb[4], vc[4], vd[4];
-      const uint32_t x0 = f.v[0][w], x1 = f.v[1][w], x2 = f.v[2][w], x3 = f.v[3][w];
-      e2m1x8_f16((x0 & 0x0f0f0f0fu) | ((x1 << 4) & 0xf0f0f0f0u), va);  // dim g, tokens 2t, 2t + 1
-      e2m1x8_f16(((x0 >> 4) & 0x0f0f0f0fu) | (x1 & 0xf0f0f0f0u), vb);  // dim g + 8
-      e2m1x8_f16((x2 & 0x0f0f0f0fu) | ((x3 << 4) & 0xf0f0f0f0u), vc);  // tokens 2t + 8, 2t + 9
-      e2m1x8_f16(((x2 >> 4) & 0x0f0f0f0fu) | (x3 & 0xf0f0f0f0u), vd);
-      const uint32_t s01 = __byte_perm(f.vs[0][w], f.vs[1][w], 0x5140);  // groups 4w, 4w + 1
-      const uint32_t s23 = __byte_perm(f.vs[0][w], f.vs[1][w], 0x7362);
-      const uint32_t t01 = __byte_perm(f.vs[2][w], f.vs[3][w], 0x5140);
-      const uint32_t t23 = __byte_perm(f.vs[2][w], f.vs[3][w], 0x7362);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t sp = e4m3x2_f16((i < 2 ? s01 : s23) >> (16 * (i & 1)));
-        const uint32_t tp = e4m3x2_f16((i < 2 ? t01 : t23) >> (16 * (i & 1)));
-        const uint32_t frag[4] = {va[i], vb[i], vc[i], vd[i]};
+        // ---- logits in log2 units, masks
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
-          // the mask again: a NaN scale of a token that a row does not see must not reach it
-          mma16816(o[nt][4 * w + i], frag, h2mul(pb[nt][0], sp) & pm[nt][0],
-                   h2mul(pb[nt][1], tp) & pm[nt][1]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[nt][e] *= sc[nt][e & 1];
+        unsigned hidden = 0;  // bit 4 nt + e: the row does not see the token
+        if (careful) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int r = min(r0 + nt * 8 + 2 * t + (e & 1), rows - 1), i = r / a.group;
+              const int key = token + key_of + 8 * (e >> 1);
+              float x = s[nt][e];
+              if (a.softcap > 0.f) x = a.softcap * 1.4426950408889634f * tanh_any(x);
+              if (a.alibi != nullptr)
+                x -= a.alibi[(int64_t)b * a.Hq + hk * a.group + r % a.group] *
+                     1.4426950408889634f * fabsf((float)(i + len - a.Lq - key));
+              const Kv4Range seen = kv4_range(a, len, i);
+              const bool vis = (key >= seen.lo || key < seen.sk) && key < seen.hi;
+              s[nt][e] = vis ? x : -INFINITY;
+              hidden |= (vis ? 0u : 1u) << (4 * nt + e);
+            }
+        }
+        bool grow = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            grow = grow || fmaxf(s[nt][e], s[nt][e + 2]) > m[nt][e] + kGrow;
+        if (__any_sync(kFull, grow)) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float top = fmaxf(s[nt][e], s[nt][e + 2]);
+#pragma unroll
+              for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, d));
+              if (top > m[nt][e] + kGrow) {
+                const float fresh = top - kBelow;
+                const float factor = m[nt][e] == -INFINITY ? 0.f : ex2(m[nt][e] - fresh);
+                m[nt][e] = m_sub[nt][e] = fresh;
+                l[nt][e] *= factor;
+#pragma unroll
+                for (int i = 0; i < NG; ++i) {
+                  o[nt][i][e] *= factor;
+                  o[nt][i][e + 2] *= factor;
+                }
+              }
+            }
+        }
+        // ---- probabilities
+        uint32_t pb[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float p[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) p[e] = ex2(s[nt][e] - m_sub[nt][e & 1]);
+          l[nt][0] += p[0] + p[2];
+          l[nt][1] += p[1] + p[3];
+          pb[nt][0] = transpose8x8(h2(p[0], p[1]));  // rows 2t, 2t + 1 of the tile for row g of q
+          pb[nt][1] = transpose8x8(h2(p[2], p[3]));  // rows 2t + 8, 2t + 9
+        }
+        // ---- values: a byte of two tokens' codes of one dim makes one operand register
+        uint32_t v0[D / 64], v1[D / 64], v2[D / 64], v3[D / 64];
+        uint32_t z0[D / 64], z1[D / 64], z2[D / 64], z3[D / 64];
+        const int flip = t & 1;
+        const uint8_t* vp = base + Smem::kCodes + (16 * warp + 2 * t) * (D / 2) + g * (D / 16);
+        load_words<D / 16>(vp + flip * (D / 2), v0);
+        load_words<D / 16>(vp + (1 - flip) * (D / 2), v1);
+        load_words<D / 16>(vp + (8 + flip) * (D / 2), v2);
+        load_words<D / 16>(vp + (9 - flip) * (D / 2), v3);
+        const uint8_t* zp =
+            base + 2 * Smem::kCodes + Smem::kScales + (16 * warp + 2 * t) * (D / 16);
+        load_words<D / 16>(zp + flip * (D / 16), z0);
+        load_words<D / 16>(zp + (1 - flip) * (D / 16), z1);
+        load_words<D / 16>(zp + (8 + flip) * (D / 16), z2);
+        load_words<D / 16>(zp + (9 - flip) * (D / 16), z3);
+        // The NaN scale of a token must not reach a row that does not see it. Such tokens have
+        // probability 0 there, so with finite scales nothing is left to do.
+        uint32_t keep[NT][2];
+        bool clean = true;
+        if (careful) {
+          bool nan = false;
+#pragma unroll
+          for (int w = 0; w < NG / 4; ++w)
+            nan = nan || has_nan_scale(z0[w]) || has_nan_scale(z1[w]) || has_nan_scale(z2[w]) ||
+                  has_nan_scale(z3[w]);
+          clean = !__any_sync(kFull, nan);
+          if (!clean) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                keep[nt][e] = transpose8x8((hidden >> (4 * nt + 2 * e) & 1 ? 0u : 0xffffu) |
+                                           (hidden >> (4 * nt + 2 * e + 1) & 1 ? 0u : 0xffff0000u));
+          }
+        }
+#pragma unroll
+        for (int w = 0; w < NG / 4; ++w) {  // a word: four groups
+          uint32_t va[4], vb[4], vc[4], vd[4];
+          e2m1x8_f16((v0[w] & 0x0f0f0f0fu) | ((v1[w] << 4) & 0xf0f0f0f0u), va);  // dim g
+          e2m1x8_f16(((v0[w] >> 4) & 0x0f0f0f0fu) | (v1[w] & 0xf0f0f0f0u), vb);  // dim g + 8
+          e2m1x8_f16((v2[w] & 0x0f0f0f0fu) | ((v3[w] << 4) & 0xf0f0f0f0u), vc);
+          e2m1x8_f16(((v2[w] >> 4) & 0x0f0f0f0fu) | (v3[w] & 0xf0f0f0f0u), vd);
+          uint32_t sp[4], tp[4];  // pairs of tokens' scales, groups 4w .. 4w + 3
+          e4m3x4_f16(__byte_perm(z0[w], z1[w], 0x5140), sp);
+          e4m3x4_f16(__byte_perm(z0[w], z1[w], 0x7362), sp + 2);
+          e4m3x4_f16(__byte_perm(z2[w], z3[w], 0x5140), tp);
+          e4m3x4_f16(__byte_perm(z2[w], z3[w], 0x7362), tp + 2);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t frag[4] = {va[i], vb[i], vc[i], vd[i]};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              uint32_t p0 = h2mul(pb[nt][0], sp[i]), p1 = h2mul(pb[nt][1], tp[i]);
+              if (!clean) {
+                p0 &= keep[nt][0];
+                p1 &= keep[nt][1];
+              }
+              mma16816(o[nt][4 * w + i], frag, p0, p1);
+            }
+          }
+        }
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.empty[slot]);
     }
-    f = next;
-  }
 
-  // ---- join the warps
+    // ---- join the warps: a common reference per row, then their sums
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int r = nt * 8 + 2 * t + e;
+      for (int e = 0; e < 2; ++e) {
 #pragma unroll
-      for (int d = 4; d < 32; d <<= 1) l[nt][e] += __shfl_xor_sync(kFull, l[nt][e], d);
-      if (g == 0) {
-        s_m[warp][r] = m[nt][e];
-        s_l[warp][r] = l[nt][e];
+        for (int d = 4; d < 32; d <<= 1) l[nt][e] += __shfl_xor_sync(kFull, l[nt][e], d);
+        if (g == 0) sm.m[warp][nt * 8 + 2 * t + e] = m[nt][e];
       }
+    asm volatile("bar.sync 1, 128;" ::: "memory");
 #pragma unroll
-      for (int i = 0; i < NG; ++i) {
-        s_o[warp][r][16 * i + g] = o[nt][i][e];
-        s_o[warp][r][16 * i + 8 + g] = o[nt][i][e + 2];
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = nt * 8 + 2 * t + e;
+        float top = sm.m[0][r];
+#pragma unroll
+        for (int w = 1; w < kAttnWarps; ++w) top = fmaxf(top, sm.m[w][r]);
+        // a warp that saw only NaN scores has no reference, but its NaN sum, which stays
+        const float f = m[nt][e] == -INFINITY ? 0.f : ex2(m[nt][e] - top);
+        if (g == 0) sm.l[warp][r] = l[nt][e] * (l[nt][e] != l[nt][e] ? 1.f : f);
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+          sm.o[warp][r][16 * i + g] = o[nt][i][e] * f;
+          sm.o[warp][r][16 * i + 8 + g] = o[nt][i][e + 2] * f;
+        }
+      }
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    const bool whole = walk.take == walk.span.n;
+    const int64_t part = (2 * (int64_t)blockIdx.x + (walk.j == 0)) * kRows;
+    for (int x = threadIdx.x; x < kRows * (D / 4); x += 32 * kAttnWarps) {
+      const int rr = x / (D / 4), d = x % (D / 4) * 4, r = r0 + rr;
+      if (r >= rows) break;
+      float sum = 0.f;
+      float4 val = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kAttnWarps; ++w) {
+        const float4 y = *reinterpret_cast<const float4*>(&sm.o[w][rr][d]);
+        sum += sm.l[w][rr];
+        val.x += y.x;
+        val.y += y.y;
+        val.z += y.z;
+        val.w += y.w;
+      }
+      if (whole) {
+        const int i = r / a.group, h = hk * a.group + r % a.group;
+        kv4_store(a, b * a.o_sb + i * a.o_ss + (int64_t)h * a.o_sh + d, val, sum);
+      } else {
+        *reinterpret_cast<float4*>(a.ws_o + (part + rr) * D + d) = val;
+        if (d == 0) {
+          float top = sm.m[0][rr];
+#pragma unroll
+          for (int w = 1; w < kAttnWarps; ++w) top = fmaxf(top, sm.m[w][rr]);
+          a.ws_m[part + rr] = top;
+          a.ws_l[part + rr] = sum;
+        }
       }
     }
-  __syncthreads();
-  for (int x = threadIdx.x; x < kRows * D; x += 32 * kAttnWarps) {
-    const int rr = x / D, d = x % D, r = r0 + rr;
-    if (r >= rows) break;
-    float top = -INFINITY, sum = 0.f, val = 0.f;
-#pragma unroll
-    for (int w = 0; w < kAttnWarps; ++w) top = fmaxf(top, s_m[w][rr]);
-#pragma unroll
-    for (int w = 0; w < kAttnWarps; ++w) {
-      const float f2 = s_m[w][rr] == -INFINITY ? 0.f : ex2(s_m[w][rr] - top);
-      // a warp that saw only NaN scores has no maximum, but its NaN sum
-      const float weight = s_l[w][rr] != s_l[w][rr] ? s_l[w][rr] : f2;
-      sum += weight * s_l[w][rr];
-      val += weight * s_o[w][rr][d];
-    }
-    const float out = sum == 0.f ? 0.f : val / sum;
-    const int i = r / a.group, h = hk * a.group + r % a.group;
-    if (a.splits == 1) {
-      const int64_t at = b * a.o_sb + i * a.o_ss + (int64_t)h * a.o_sh + d;
-      if (a.bf16) reinterpret_cast<__nv_bfloat16*>(a.o)[at] = __float2bfloat16_rn(out * c.v_unit);
-      else reinterpret_cast<__half*>(a.o)[at] = __float2half_rn(out * c.v_unit);
-    } else {
-      const int64_t all = (int64_t)c.B * a.Lq * a.Hq;
-      const int64_t at = split * all + ((int64_t)b * a.Lq + i) * a.Hq + h;
-      a.ws_o[at * D + d] = out;
-      if (d == 0) a.ws_lse[at] = sum == 0.f ? -INFINITY : top + log2f(sum);
-    }
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    walk.next(a);
   }
 }
 
-// Joins the splits: one warp per output row, lanes over D.
-template <int D>
+// Adds up the partial results of a row: one block per output row. Rows that one CTA finished are
+// left as they are; rows without visible keys become 0.
+template <int D, int NT>
 __global__ void __launch_bounds__(128) kv4_join(const __grid_constant__ Kv4Args a) {
+  constexpr int kRows = 8 * NT, kLanes = D / 4, kAtOnce = 128 / kLanes;
+  __shared__ float4 s_val[kAtOnce][kLanes];
+  __shared__ float s_sum[kAtOnce], s_top[4];
+  const int h = (int)(blockIdx.x % a.Hq);
+  const int64_t bi = blockIdx.x / a.Hq;
+  const int i = (int)(bi % a.Lq), b = (int)(bi / a.Lq);
+  const int hk = h / a.group, r = i * a.group + h % a.group, rb = r / kRows, rr = r % kRows;
+  const int lane = threadIdx.x % kLanes, p = threadIdx.x / kLanes;
+  const int len = kv4_length(a, b);
+  int head = 0, ahead = 0;  // blocks of the head's units, and of those before this one
+  int n = 0;
+#pragma unroll 1
+  for (int x = 0; x < a.row_blocks; ++x) {
+    const int y = kv4_span<kRows>(a, len, x).n;
+    if (x < rb) ahead += kv4_room(y);
+    if (x == rb) n = y;
+    head += kv4_room(y);
+  }
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int64_t all = (int64_t)a.c.B * a.Lq * a.Hq;
-  const int64_t r = ((int64_t)blockIdx.x * 128 + threadIdx.x) >> 5;
-  const int lane = threadIdx.x & 31;
-  if (r >= all) return;
+  const unsigned share = a.ws_line[0], u0 = a.ws_line[1 + b] + hk * head + ahead + kUnitCost;
+  int c0 = 0, c1 = -1;
+  if (n > 0) {
+    c0 = u0 / share;
+    c1 = (u0 + n - 1) / share;
+    if (c0 == c1) return;
+  }
+  auto part = [&](int cta) { return (2 * (int64_t)cta + (cta == c0)) * kRows + rr; };
   float top = -INFINITY;
-  for (int s = lane; s < a.splits; s += 32) top = fmaxf(top, a.ws_lse[s * all + r]);
+  for (int x = c0 + threadIdx.x; x <= c1; x += 128) top = fmaxf(top, a.ws_m[part(x)]);
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, d));
-  float sum = 0.f, val[D / 32];
-#pragma unroll
-  for (int i = 0; i < D / 32; ++i) val[i] = 0.f;
-  for (int s = 0; s < a.splits; ++s) {
-    const float lse = a.ws_lse[s * all + r];
-    const float w = lse == -INFINITY ? 0.f : ex2(lse - (top == -INFINITY ? 0.f : top));
-    sum += w;
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i)
-      val[i] = fmaf(w, a.ws_o[(s * all + r) * D + lane + 32 * i], val[i]);
+  if (threadIdx.x % 32 == 0) s_top[threadIdx.x / 32] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
+  float sum = 0.f;
+  float4 val = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int x = c0 + p; x <= c1; x += kAtOnce) {
+    const int64_t at = part(x);
+    const float l = a.ws_l[at], m = a.ws_m[at];
+    const float f = l != l ? l : m == -INFINITY ? 0.f : ex2(m - top);
+    const float4 y = reinterpret_cast<const float4*>(a.ws_o + at * D)[lane];
+    sum = fmaf(f, l, sum);
+    val.x = fmaf(f, y.x, val.x);
+    val.y = fmaf(f, y.y, val.y);
+    val.z = fmaf(f, y.z, val.z);
+    val.w = fmaf(f, y.w, val.w);
   }
-  const int h = (int)(r % a.Hq);
-  const int64_t bi = r / a.Hq;
-  const int64_t at = bi / a.Lq * a.o_sb + bi % a.Lq * a.o_ss + h * a.o_sh;
+  s_val[p][lane] = val;
+  if (lane == 0) s_sum[p] = sum;
+  __syncthreads();
+  if (threadIdx.x >= kLanes) return;
+  sum = s_sum[0];
+  val = s_val[0][lane];
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) {
-    const float out = (sum == 0.f ? 0.f : val[i] / sum) * a.c.v_unit;
-    if (a.bf16) reinterpret_cast<__nv_bfloat16*>(a.o)[at + lane + 32 * i] = __float2bfloat16_rn(out);
-    else reinterpret_cast<__half*>(a.o)[at + lane + 32 * i] = __float2half_rn(out);
+  for (int x = 1; x < kAtOnce; ++x) {
+    const float4 y = s_val[x][lane];
+    sum += s_sum[x];
+    val.x += y.x;
+    val.y += y.y;
+    val.z += y.z;
+    val.w += y.w;
   }
+  kv4_store(a, b * a.o_sb + i * a.o_ss + (int64_t)h * a.o_sh + 4 * lane, val, sum);
 }
 
 // ------------------------------------------------------------------ host
@@ -724,54 +1102,51 @@ int check_fwd(const mfa_kv4_cache* c, const mfa_kv4_fwd_params* p) {
   if (c->B == 0 || p->Lq == 0) return MFA_OK;
   if (p->q == nullptr || p->o == nullptr || p->seqlens == nullptr) return MFA_ERR_INVALID;
   if ((int64_t)c->B * p->Lq * p->Hq >= (1ll << 31)) return MFA_ERR_UNSUPPORTED;
+  // the line is counted in 32 bits
+  const double rows = std::ceil((double)p->Lq * (p->Hq / c->Hkv) / 8);
+  if ((double)c->B * c->Hkv * rows * ((double)c->max_pages * c->page_size / 64 + 10) >= 2147483648.0)
+    return MFA_ERR_UNSUPPORTED;
+  if (reinterpret_cast<uintptr_t>(p->o) % 8 != 0) return MFA_ERR_INVALID;
+  for (int i = 0; i < 3; ++i)
+    if (p->o_stride[i] % 4 != 0) return MFA_ERR_INVALID;
   return MFA_OK;
 }
 
 struct Kv4Plan {
-  int nt, row_blocks, splits;
+  int nt, row_blocks, ctas;
+  int64_t line, o, m;  // sizes of the workspace's parts, in bytes
   size_t bytes;
 };
-// Tiles of 8 rows per CTA, and how many CTAs share the tokens of a (sequence, KV head): as many
-// as fill the SMs once, four CTAs each, with at least 16 tiles of 16 tokens apiece.
+// One wave of resident CTAs, whatever the lengths are.
 Kv4Plan plan_fwd(const mfa_kv4_cache* c, const mfa_kv4_fwd_params* p, int sms) {
   Kv4Plan k;
   const int64_t rows = (int64_t)p->Lq * (p->Hq / c->Hkv);
   k.nt = rows > 8 ? 2 : 1;
   k.row_blocks = (int)((rows + 8 * k.nt - 1) / (8 * k.nt));
-  int64_t keys = (int64_t)c->max_pages * c->page_size;
-  if (p->win_left >= 0) {  // what a row block can see at most
-    const int64_t right = p->causal ? 0 : p->win_right >= 0 ? p->win_right : keys;
-    const int64_t window = (int64_t)p->win_left + 1 + right + 8 * k.nt + 16 + (int64_t)p->sink + 16;
-    if (window < keys) keys = window;
-  }
-  const int64_t ctas = (int64_t)c->B * c->Hkv * k.row_blocks;
-  int64_t s = 4ll * sms / ctas;
-  const int64_t most = keys / 256;
-  s = s < most ? s : most;
-  k.splits = (int)(s < 1 ? 1 : s > 128 ? 128 : s);
-  const int64_t out_rows = (int64_t)c->B * p->Lq * p->Hq;
-  k.bytes = k.splits > 1 ? (size_t)k.splits * out_rows * (c->D + 1) * sizeof(float) : 0;
+  k.ctas = sms * kv4_ctas(k.nt);
+  const int64_t parts = 2ll * k.ctas * 8 * k.nt;
+  k.line = ((c->B + 1) * 4ll + 127) / 128 * 128;
+  k.o = parts * c->D * 4;
+  k.m = parts * 4;
+  k.bytes = (size_t)(k.line + k.o + 2 * k.m);
   return k;
 }
 
-template <int D>
-int launch_fwd(const Kv4Args& a, int nt, cudaStream_t st) {
-  const int64_t grid = (int64_t)a.c.B * a.c.Hkv * a.splits * a.row_blocks;
-  if (grid >= (1ll << 31)) return MFA_ERR_UNSUPPORTED;
-  if (nt == 1) kv4_attn<D, 1><<<(unsigned)grid, 32 * kAttnWarps, 0, st>>>(a);
-  else kv4_attn<D, 2><<<(unsigned)grid, 32 * kAttnWarps, 0, st>>>(a);
-  if (a.splits > 1) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(((int64_t)a.c.B * a.Lq * a.Hq + 3) / 4));
-    cfg.blockDim = dim3(128);
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    if (cudaLaunchKernelEx(&cfg, kv4_join<D>, a) != cudaSuccess) return MFA_ERR_CUDA;
-  }
+template <int D, int NT>
+int launch_fwd(const Kv4Args& a, int ctas, int dev, cudaStream_t st) {
+  constexpr int smem = (int)sizeof(Kv4Smem<D, NT>) + 128;
+  if (ensure_smem(kv4_attn<D, NT>, dev, smem) != cudaSuccess) return MFA_ERR_CUDA;
+  kv4_attn<D, NT><<<ctas, kAttnThreads, smem, st>>>(a);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((int64_t)a.c.B * a.Lq * a.Hq));
+  cfg.blockDim = dim3(128);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kv4_join<D, NT>, a) != cudaSuccess) return MFA_ERR_CUDA;
   return cudaGetLastError() == cudaSuccess ? MFA_OK : MFA_ERR_CUDA;
 }
 
@@ -822,8 +1197,8 @@ int mfa_kv4_fwd(const mfa_kv4_cache* c, const mfa_kv4_fwd_params* p, void* strea
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return MFA_ERR_NO_DEVICE;
   const mfa::Kv4Plan plan = mfa::plan_fwd(c, p, mfa::dev_info(dev).sms);
-  if (plan.bytes > 0 && (p->workspace == nullptr || p->workspace_bytes < plan.bytes))
-    return MFA_ERR_SCRATCH_TOO_SMALL;
+  if (p->workspace == nullptr || p->workspace_bytes < plan.bytes) return MFA_ERR_SCRATCH_TOO_SMALL;
+  if (!mfa::aligned16(p->workspace)) return MFA_ERR_INVALID;
   mfa::Kv4Args a;
   a.c = mfa::resolve_cache(c);
   a.q = p->q;
@@ -835,6 +1210,8 @@ int mfa_kv4_fwd(const mfa_kv4_cache* c, const mfa_kv4_fwd_params* p, void* strea
   a.Hq = p->Hq;
   a.group = p->Hq / c->Hkv;
   a.bf16 = p->dtype == MFA_BF16;
+  a.q_vec8 = reinterpret_cast<uintptr_t>(p->q) % 8 == 0;
+  for (int i = 0; i < 3; ++i) a.q_vec8 = a.q_vec8 && p->q_stride[i] % 4 == 0;
   a.softcap = p->softcap;
   a.scale_l2 = p->scale * c->k_unit *
                (p->softcap > 0.f ? 1.f / p->softcap : 1.4426950408889634f);
@@ -844,12 +1221,18 @@ int mfa_kv4_fwd(const mfa_kv4_cache* c, const mfa_kv4_fwd_params* p, void* strea
   a.sink = p->win_left >= 0 ? p->sink : 0;
   a.alibi = p->alibi;
   a.row_blocks = plan.row_blocks;
-  a.splits = plan.splits;
-  a.ws_o = static_cast<float*>(p->workspace);
-  a.ws_lse = a.ws_o + (int64_t)plan.splits * c->B * p->Lq * p->Hq * c->D;
+  uint8_t* ws = static_cast<uint8_t*>(p->workspace);
+  a.ws_line = reinterpret_cast<int*>(ws);
+  a.ws_o = reinterpret_cast<float*>(ws + plan.line);
+  a.ws_m = reinterpret_cast<float*>(ws + plan.line + plan.o);
+  a.ws_l = reinterpret_cast<float*>(ws + plan.line + plan.o + plan.m);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   (void)cudaGetLastError();
-  return c->D == 128 ? mfa::launch_fwd<128>(a, plan.nt, st) : mfa::launch_fwd<64>(a, plan.nt, st);
+  if (c->D == 128)
+    return plan.nt == 1 ? mfa::launch_fwd<128, 1>(a, plan.ctas, dev, st)
+                        : mfa::launch_fwd<128, 2>(a, plan.ctas, dev, st);
+  return plan.nt == 1 ? mfa::launch_fwd<64, 1>(a, plan.ctas, dev, st)
+                      : mfa::launch_fwd<64, 2>(a, plan.ctas, dev, st);
 }
 
 }  // extern "C"
