@@ -15,6 +15,11 @@
 namespace mfa {
 namespace {
 
+template <bool B>
+struct BoolC {
+  static constexpr bool value = B;
+};
+
 struct Kv4Cache {
   uint8_t *k, *v, *ks, *vs;
   const int* table;
@@ -417,6 +422,11 @@ __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* w) {
   }
 }
 
+// Barrier of the consumer warps.
+__device__ __forceinline__ void consumers_meet() {
+  asm volatile("bar.sync 1, %0;" ::"n"(32 * kAttnWarps) : "memory");
+}
+
 // Four columns of an output row from their weighted sums and the sum of the weights.
 __device__ __forceinline__ void kv4_store(const Kv4Args& a, int64_t at, float4 val, float sum) {
   const float f = sum == 0.f ? 0.f : a.c.v_unit / sum;
@@ -700,148 +710,153 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(NT))
       const bool some = !bad && token < see.last.hi &&
                         (token + 16 > see.first.lo || token < see.last.sk);
       const uint8_t* base = sm.ring[slot];
-
-      if (some) {
-        const bool careful = general || !full;  // alike in all lanes
-        // ---- scores of 16 tokens: s[nt][0, 1] row g of the tile, s[nt][2, 3] row g + 8
-        float s[NT][4];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
-        {
-          uint32_t k0[D / 32], k1[D / 32], s0[D / 64], s1[D / 64];
-          const uint8_t* kp = base + (16 * warp + key_of) * (D / 2) + t * (D / 8);
-          load_words<D / 8>(kp, k0);
-          load_words<D / 8>(kp + 8 * (D / 2), k1);
-          const uint8_t* sp2 = base + 2 * Smem::kCodes + (16 * warp + key_of) * (D / 16);
-          load_words<D / 16>(sp2, s0);
-          load_words<D / 16>(sp2 + 8 * (D / 16), s1);
-          uint32_t fs0[NG / 2], fs1[NG / 2];
-#pragma unroll
-          for (int w = 0; w < NG / 4; ++w) {
-            e4m3x4_f16(s0[w], fs0 + 2 * w);
-            e4m3x4_f16(s1[w], fs1 + 2 * w);
-          }
-#pragma unroll
-          for (int w = 0; w < NG / 2; ++w) {  // a word: two groups
-            uint32_t ka[4], kb[4];
-            e2m1x8_f16(k0[w], ka);
-            e2m1x8_f16(k1[w], kb);
-            const uint32_t sa = fs0[w], sb = fs1[w];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const uint32_t frag[4] = {ka[2 * i], kb[2 * i], ka[2 * i + 1], kb[2 * i + 1]};
-              const float fa = i ? f16_hi(sa) : f16_lo(sa), fb = i ? f16_hi(sb) : f16_lo(sb);
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                float x[4] = {0.f, 0.f, 0.f, 0.f};
-                mma16816(x, frag, qf[nt][2 * w + i][0], qf[nt][2 * w + i][1]);
-                s[nt][0] = fmaf(fa, x[0], s[nt][0]);
-                s[nt][1] = fmaf(fa, x[1], s[nt][1]);
-                s[nt][2] = fmaf(fb, x[2], s[nt][2]);
-                s[nt][3] = fmaf(fb, x[3], s[nt][3]);
-              }
-            }
-          }
-        }
-        // ---- logits in log2 units, masks
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[nt][e] *= sc[nt][e & 1];
-        unsigned hidden = 0;  // bit 4 nt + e: the row does not see the token
-        if (careful) {
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int r = min(r0 + nt * 8 + 2 * t + (e & 1), rows - 1), i = r / a.group;
-              const int key = token + key_of + 8 * (e >> 1);
-              float x = s[nt][e];
-              if (a.softcap > 0.f) x = a.softcap * 1.4426950408889634f * tanh_any(x);
-              if (a.alibi != nullptr)
-                x -= a.alibi[(int64_t)b * a.Hq + hk * a.group + r % a.group] *
-                     1.4426950408889634f * fabsf((float)(i + len - a.Lq - key));
-              const Kv4Range seen = kv4_range(a, len, i);
-              const bool vis = (key >= seen.lo || key < seen.sk) && key < seen.hi;
-              s[nt][e] = vis ? x : -INFINITY;
-              hidden |= (vis ? 0u : 1u) << (4 * nt + e);
-            }
-        }
-        bool grow = false;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            grow = grow || fmaxf(s[nt][e], s[nt][e + 2]) > m[nt][e] + kGrow;
-        if (__any_sync(kFull, grow)) {
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float top = fmaxf(s[nt][e], s[nt][e + 2]);
-#pragma unroll
-              for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, d));
-              if (top > m[nt][e] + kGrow) {
-                const float fresh = top - kBelow;
-                const float factor = m[nt][e] == -INFINITY ? 0.f : ex2(m[nt][e] - fresh);
-                m[nt][e] = m_sub[nt][e] = fresh;
-                l[nt][e] *= factor;
-#pragma unroll
-                for (int i = 0; i < NG; ++i) {
-                  o[nt][i][e] *= factor;
-                  o[nt][i][e + 2] *= factor;
-                }
-              }
-            }
-        }
-        // ---- probabilities
-        uint32_t pb[NT][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float p[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) p[e] = ex2(s[nt][e] - m_sub[nt][e & 1]);
-          l[nt][0] += p[0] + p[2];
-          l[nt][1] += p[1] + p[3];
-          pb[nt][0] = transpose8x8(h2(p[0], p[1]));  // rows 2t, 2t + 1 of the tile for row g of q
-          pb[nt][1] = transpose8x8(h2(p[2], p[3]));  // rows 2t + 8, 2t + 9
-        }
-        // ---- values: a byte of two tokens' codes of one dim makes one operand register
-        uint32_t v0[D / 64], v1[D / 64], v2[D / 64], v3[D / 64];
-        uint32_t z0[D / 64], z1[D / 64], z2[D / 64], z3[D / 64];
+      // this lane's codes and scales: keys of rows g and g + 8 of the tile, values of rows 2t,
+      // 2t + 1, 2t + 8 and 2t + 9; then the slot is free again
+      uint32_t k0[D / 32], k1[D / 32], y0[D / 64], y1[D / 64];
+      uint32_t v0[D / 64], v1[D / 64], v2[D / 64], v3[D / 64];
+      uint32_t z0[D / 64], z1[D / 64], z2[D / 64], z3[D / 64];
+      {
+        const uint8_t* kp = base + (16 * warp + key_of) * (D / 2) + t * (D / 8);
+        const uint8_t* yp = base + 2 * Smem::kCodes + (16 * warp + key_of) * (D / 16);
+        load_words<D / 16>(yp, y0);
+        load_words<D / 16>(yp + 8 * (D / 16), y1);
+        load_words<D / 8>(kp, k0);
+        load_words<D / 8>(kp + 8 * (D / 2), k1);
         const int flip = t & 1;
-        const uint8_t* vp = base + Smem::kCodes + (16 * warp + 2 * t) * (D / 2) + g * (D / 16);
-        load_words<D / 16>(vp + flip * (D / 2), v0);
-        load_words<D / 16>(vp + (1 - flip) * (D / 2), v1);
-        load_words<D / 16>(vp + (8 + flip) * (D / 2), v2);
-        load_words<D / 16>(vp + (9 - flip) * (D / 2), v3);
-        const uint8_t* zp =
-            base + 2 * Smem::kCodes + Smem::kScales + (16 * warp + 2 * t) * (D / 16);
-        load_words<D / 16>(zp + flip * (D / 16), z0);
-        load_words<D / 16>(zp + (1 - flip) * (D / 16), z1);
-        load_words<D / 16>(zp + (8 + flip) * (D / 16), z2);
-        load_words<D / 16>(zp + (9 - flip) * (D / 16), z3);
+        const uint8_t* vp = base + Smem::kCodes + (16 * warp + 2 * t + flip) * (D / 2) + g * (D / 16);
+        const uint8_t* zp = base + 2 * Smem::kCodes + Smem::kScales + (16 * warp + 2 * t + flip) * (D / 16);
+        const int other = 1 - 2 * flip;  // rows from a token to its partner
+        load_words<D / 16>(zp, z0);
+        load_words<D / 16>(zp + other * (D / 16), z1);
+        load_words<D / 16>(zp + 8 * (D / 16), z2);
+        load_words<D / 16>(zp + (8 + other) * (D / 16), z3);
+        load_words<D / 16>(vp, v0);
+        load_words<D / 16>(vp + other * (D / 2), v1);
+        load_words<D / 16>(vp + 8 * (D / 2), v2);
+        load_words<D / 16>(vp + (8 + other) * (D / 2), v3);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.empty[slot]);
+      if (!some) continue;
+      const bool careful = general || !full;  // alike in all lanes
+
+      // ---- scores of 16 tokens: s[nt][0, 1] row g of the tile, s[nt][2, 3] row g + 8
+      float s[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
+      {
+        uint32_t fs0[NG / 2], fs1[NG / 2];
+#pragma unroll
+        for (int w = 0; w < NG / 4; ++w) {
+          e4m3x4_f16(y0[w], fs0 + 2 * w);
+          e4m3x4_f16(y1[w], fs1 + 2 * w);
+        }
+#pragma unroll
+        for (int w = 0; w < NG / 2; ++w) {  // a word: two groups
+          uint32_t ka[4], kb[4];
+          e2m1x8_f16(k0[w], ka);
+          e2m1x8_f16(k1[w], kb);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t frag[4] = {ka[2 * i], kb[2 * i], ka[2 * i + 1], kb[2 * i + 1]};
+            const float fa = i ? f16_hi(fs0[w]) : f16_lo(fs0[w]);
+            const float fb = i ? f16_hi(fs1[w]) : f16_lo(fs1[w]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              float x[4] = {0.f, 0.f, 0.f, 0.f};
+              mma16816(x, frag, qf[nt][2 * w + i][0], qf[nt][2 * w + i][1]);
+              s[nt][0] = fmaf(fa, x[0], s[nt][0]);
+              s[nt][1] = fmaf(fa, x[1], s[nt][1]);
+              s[nt][2] = fmaf(fb, x[2], s[nt][2]);
+              s[nt][3] = fmaf(fb, x[3], s[nt][3]);
+            }
+          }
+        }
+      }
+      // ---- logits in log2 units, masks
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[nt][e] *= sc[nt][e & 1];
+      unsigned hidden = 0;  // bit 4 nt + e: the row does not see the token
+      bool clean = true;
+      if (careful) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = min(r0 + nt * 8 + 2 * t + (e & 1), rows - 1), i = r / a.group;
+            const int key = token + key_of + 8 * (e >> 1);
+            float x = s[nt][e];
+            if (a.softcap > 0.f) x = a.softcap * 1.4426950408889634f * tanh_any(x);
+            if (a.alibi != nullptr)
+              x -= a.alibi[(int64_t)b * a.Hq + hk * a.group + r % a.group] *
+                   1.4426950408889634f * fabsf((float)(i + len - a.Lq - key));
+            const Kv4Range seen = kv4_range(a, len, i);
+            const bool vis = (key >= seen.lo || key < seen.sk) && key < seen.hi;
+            s[nt][e] = vis ? x : -INFINITY;
+            hidden |= (vis ? 0u : 1u) << (4 * nt + e);
+          }
         // The NaN scale of a token must not reach a row that does not see it. Such tokens have
         // probability 0 there, so with finite scales nothing is left to do.
-        uint32_t keep[NT][2];
-        bool clean = true;
-        if (careful) {
-          bool nan = false;
+        bool nan = false;
 #pragma unroll
-          for (int w = 0; w < NG / 4; ++w)
-            nan = nan || has_nan_scale(z0[w]) || has_nan_scale(z1[w]) || has_nan_scale(z2[w]) ||
-                  has_nan_scale(z3[w]);
-          clean = !__any_sync(kFull, nan);
-          if (!clean) {
+        for (int w = 0; w < NG / 4; ++w)
+          nan = nan || has_nan_scale(z0[w]) || has_nan_scale(z1[w]) || has_nan_scale(z2[w]) ||
+                has_nan_scale(z3[w]);
+        clean = !__any_sync(kFull, nan);
+      }
+      bool grow = false;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-              for (int e = 0; e < 2; ++e)
-                keep[nt][e] = transpose8x8((hidden >> (4 * nt + 2 * e) & 1 ? 0u : 0xffffu) |
-                                           (hidden >> (4 * nt + 2 * e + 1) & 1 ? 0u : 0xffff0000u));
+        for (int e = 0; e < 2; ++e)
+          grow = grow || fmaxf(s[nt][e], s[nt][e + 2]) > m[nt][e] + kGrow;
+      if (__any_sync(kFull, grow)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float top = fmaxf(s[nt][e], s[nt][e + 2]);
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, d));
+            if (top > m[nt][e] + kGrow) {
+              const float fresh = top - kBelow;
+              const float factor = m[nt][e] == -INFINITY ? 0.f : ex2(m[nt][e] - fresh);
+              m[nt][e] = m_sub[nt][e] = fresh;
+              l[nt][e] *= factor;
+#pragma unroll
+              for (int i = 0; i < NG; ++i) {
+                o[nt][i][e] *= factor;
+                o[nt][i][e + 2] *= factor;
+              }
+            }
           }
+      }
+      // ---- probabilities
+      uint32_t pb[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float p[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) p[e] = ex2(s[nt][e] - m_sub[nt][e & 1]);
+        l[nt][0] += p[0] + p[2];
+        l[nt][1] += p[1] + p[3];
+        pb[nt][0] = transpose8x8(h2(p[0], p[1]));  // rows 2t, 2t + 1 of the tile for row g of q
+        pb[nt][1] = transpose8x8(h2(p[2], p[3]));  // rows 2t + 8, 2t + 9
+      }
+      // ---- values: a byte of two tokens' codes of one dim makes one operand register
+      auto values = [&](auto masked) {
+        uint32_t keep[NT][2];
+        if constexpr (decltype(masked)::value) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              keep[nt][e] = transpose8x8((hidden >> (4 * nt + 2 * e) & 1 ? 0u : 0xffffu) |
+                                         (hidden >> (4 * nt + 2 * e + 1) & 1 ? 0u : 0xffff0000u));
         }
 #pragma unroll
         for (int w = 0; w < NG / 4; ++w) {  // a word: four groups
@@ -861,7 +876,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(NT))
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               uint32_t p0 = h2mul(pb[nt][0], sp[i]), p1 = h2mul(pb[nt][1], tp[i]);
-              if (!clean) {
+              if constexpr (decltype(masked)::value) {
                 p0 &= keep[nt][0];
                 p1 &= keep[nt][1];
               }
@@ -869,9 +884,9 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(NT))
             }
           }
         }
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.empty[slot]);
+      };
+      if (clean) values(BoolC<false>{});
+      else values(BoolC<true>{});
     }
 
     // ---- join the warps: a common reference per row, then their sums
@@ -883,7 +898,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(NT))
         for (int d = 4; d < 32; d <<= 1) l[nt][e] += __shfl_xor_sync(kFull, l[nt][e], d);
         if (g == 0) sm.m[warp][nt * 8 + 2 * t + e] = m[nt][e];
       }
-    asm volatile("bar.sync 1, 128;" ::: "memory");
+    consumers_meet();
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -901,7 +916,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(NT))
           sm.o[warp][r][16 * i + 8 + g] = o[nt][i][e + 2] * f;
         }
       }
-    asm volatile("bar.sync 1, 128;" ::: "memory");
+    consumers_meet();
     const bool whole = walk.take == walk.span.n;
     const int64_t part = (2 * (int64_t)blockIdx.x + (walk.j == 0)) * kRows;
     for (int x = threadIdx.x; x < kRows * (D / 4); x += 32 * kAttnWarps) {
@@ -932,7 +947,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(NT))
         }
       }
     }
-    asm volatile("bar.sync 1, 128;" ::: "memory");
+    consumers_meet();
     walk.next(a);
   }
 }
@@ -1104,7 +1119,7 @@ int check_fwd(const mfa_kv4_cache* c, const mfa_kv4_fwd_params* p) {
   if ((int64_t)c->B * p->Lq * p->Hq >= (1ll << 31)) return MFA_ERR_UNSUPPORTED;
   // the line is counted in 32 bits
   const double rows = std::ceil((double)p->Lq * (p->Hq / c->Hkv) / 8);
-  if ((double)c->B * c->Hkv * rows * ((double)c->max_pages * c->page_size / 64 + 10) >= 2147483648.0)
+  if ((double)c->B * c->Hkv * rows * ((double)c->max_pages * c->page_size / kBlockTokens + 10) >= 2147483648.0)
     return MFA_ERR_UNSUPPORTED;
   if (reinterpret_cast<uintptr_t>(p->o) % 8 != 0) return MFA_ERR_INVALID;
   for (int i = 0; i < 3; ++i)
