@@ -256,11 +256,19 @@ struct Kv4Args {
 
 constexpr int kAttnWarps = 4;                  // consumer warps
 constexpr int kAttnThreads = 32 * kAttnWarps + 32;
-constexpr int kBlockTokens = 16 * kAttnWarps;  // tokens of a block
-constexpr int kAttnStages = 4;
-constexpr int kMinShare = 4;   // blocks per CTA at least: below, joining costs more than it gives
+#ifndef KV4_TILES
+#define KV4_TILES 2
+#endif
+#ifndef KV4_STAGES
+#define KV4_STAGES 3
+#endif
+constexpr int kWarpTiles = KV4_TILES;  // tiles of 16 tokens that a consumer takes of a block
+constexpr int kBlockTokens = 16 * kWarpTiles * kAttnWarps;
+constexpr int kBlockTiles = kBlockTokens / 16;
+constexpr int kAttnStages = KV4_STAGES;
+constexpr int kMinShare = 2;   // blocks per CTA at least: below, joining costs more than it gives
 #ifndef KV4_UNIT
-#define KV4_UNIT 4
+#define KV4_UNIT 3
 #endif
 constexpr int kUnitCost = KV4_UNIT;  // beginning and ending a unit takes about as long as so many blocks
 #ifndef KV4_C1
@@ -451,7 +459,7 @@ struct Kv4Smem {
   float o[kAttnWarps][kRows][D + 4];  // the warps' sums, to be joined
   float m[kAttnWarps][kRows], l[kAttnWarps][kRows];
   uint64_t full[kAttnStages], empty[kAttnStages];
-  int bad[kAttnStages];  // bit i: the page of the block's tokens [16 i, 16 i + 16) does not exist
+  unsigned bad[kAttnStages];  // bit i: tokens [16 i, 16 i + 16) of the block have no page
   int scan[kAttnThreads / 32];
   int b, hk, rb, j, share;
   int abort;
@@ -584,10 +592,10 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(NT))
         if (lane < 1 << bshift && page != -2 && !good) kv4_report(c);
         const unsigned have = __ballot_sync(kFull, good);
         if (lane == 0) {
-          int bad = 0;
+          unsigned bad = 0;
 #pragma unroll
-          for (int i = 0; i < kAttnWarps; ++i)
-            bad |= (have >> (16 * i >> pshift) & 1 ? 0 : 1) << i;
+          for (int i = 0; i < kBlockTiles; ++i)
+            bad |= (have >> (16 * i >> pshift) & 1 ? 0u : 1u) << i;
           sm.bad[slot] = bad;
           mbar_expect_tx(&sm.full[slot], (uint32_t)(__popc(have) << pshift) * (D + D / 8));
         }
@@ -696,197 +704,204 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(NT))
         for (int e = 0; e < 4; ++e) o[nt][i][e] = 0.f;
     }
 
+    // blocks whose every token all rows see: [j_full, j_full + n_full) of the window
+    const Kv4Span& see = walk.span;
+    const int j_full = see.s1 - see.w0 + (see.last.lo + kBlockTokens - 1) / kBlockTokens;
+    const unsigned n_full = max(0, see.s1 - see.w0 + see.first.hi / kBlockTokens - j_full);
+
     for (int j = walk.j; j < walk.j + walk.take; ++j, ++it) {
       const int slot = it % kAttnStages;
       ok = ok && __all_sync(kFull, mbar_wait(&sm.full[slot], (uint32_t)(it / kAttnStages) & 1u,
                                              abort_flag));
       if (!ok) break;
-      const int token = walk.span.at(j) * kBlockTokens + 16 * warp;
-      const bool bad = sm.bad[slot] >> warp & 1;
-      const Kv4Span& see = walk.span;
-      // all rows see all 16 tokens; some row sees some
-      const bool full = !bad && token + 16 <= see.first.hi &&
-                        (token >= see.last.lo || token + 16 <= see.first.sk);
-      const bool some = !bad && token < see.last.hi &&
-                        (token + 16 > see.first.lo || token < see.last.sk);
+      const unsigned bad = sm.bad[slot];
+      const bool easy = (unsigned)(j - j_full) < n_full && bad == 0 && !general;
       const uint8_t* base = sm.ring[slot];
-      // this lane's codes and scales: keys of rows g and g + 8 of the tile, values of rows 2t,
-      // 2t + 1, 2t + 8 and 2t + 9; then the slot is free again
-      uint32_t k0[D / 32], k1[D / 32], y0[D / 64], y1[D / 64];
-      uint32_t v0[D / 64], v1[D / 64], v2[D / 64], v3[D / 64];
-      uint32_t z0[D / 64], z1[D / 64], z2[D / 64], z3[D / 64];
-      {
-        const uint8_t* kp = base + (16 * warp + key_of) * (D / 2) + t * (D / 8);
-        const uint8_t* yp = base + 2 * Smem::kCodes + (16 * warp + key_of) * (D / 16);
-        load_words<D / 16>(yp, y0);
-        load_words<D / 16>(yp + 8 * (D / 16), y1);
-        load_words<D / 8>(kp, k0);
-        load_words<D / 8>(kp + 8 * (D / 2), k1);
-        const int flip = t & 1;
-        const uint8_t* vp = base + Smem::kCodes + (16 * warp + 2 * t + flip) * (D / 2) + g * (D / 16);
-        const uint8_t* zp = base + 2 * Smem::kCodes + Smem::kScales + (16 * warp + 2 * t + flip) * (D / 16);
-        const int other = 1 - 2 * flip;  // rows from a token to its partner
-        load_words<D / 16>(zp, z0);
-        load_words<D / 16>(zp + other * (D / 16), z1);
-        load_words<D / 16>(zp + 8 * (D / 16), z2);
-        load_words<D / 16>(zp + (8 + other) * (D / 16), z3);
-        load_words<D / 16>(vp, v0);
-        load_words<D / 16>(vp + other * (D / 2), v1);
-        load_words<D / 16>(vp + 8 * (D / 2), v2);
-        load_words<D / 16>(vp + (8 + other) * (D / 2), v3);
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.empty[slot]);
-      if (!some) continue;
-      const bool careful = general || !full;  // alike in all lanes
-
-      // ---- scores of 16 tokens: s[nt][0, 1] row g of the tile, s[nt][2, 3] row g + 8
-      float s[NT][4];
+      // this lane's codes and scales: keys of rows g and g + 8 of each tile, values of rows 2t,
+      // 2t + 1, 2t + 8 and 2t + 9
+      const int tile0 = 16 * kWarpTiles * warp;  // this warp's tokens within the block
+      const int flip = t & 1, other = 1 - 2 * flip;  // rows from a token to its partner
+      const uint8_t* kp = base + (tile0 + key_of) * (D / 2) + t * (D / 8);
+      const uint8_t* yp = base + 2 * Smem::kCodes + (tile0 + key_of) * (D / 16);
+      const uint8_t* vp = base + Smem::kCodes + (tile0 + 2 * t + flip) * (D / 2) + g * (D / 16);
+      const uint8_t* zp = base + 2 * Smem::kCodes + Smem::kScales + (tile0 + 2 * t + flip) * (D / 16);
+      const int v_other = other * (D / 2), z_other = other * (D / 16);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
-      {
-        uint32_t fs0[NG / 2], fs1[NG / 2];
-#pragma unroll
-        for (int w = 0; w < NG / 4; ++w) {
-          e4m3x4_f16(y0[w], fs0 + 2 * w);
-          e4m3x4_f16(y1[w], fs1 + 2 * w);
+      for (int h = 0; h < kWarpTiles; ++h) {
+        uint32_t k0[D / 32], k1[D / 32], y0[D / 64], y1[D / 64];
+        uint32_t v0[D / 64], v1[D / 64], v2[D / 64], v3[D / 64];
+        uint32_t z0[D / 64], z1[D / 64], z2[D / 64], z3[D / 64];
+        load_words<D / 16>(yp + 16 * h * (D / 16), y0);
+        load_words<D / 16>(yp + (16 * h + 8) * (D / 16), y1);
+        load_words<D / 8>(kp + 16 * h * (D / 2), k0);
+        load_words<D / 8>(kp + (16 * h + 8) * (D / 2), k1);
+        load_words<D / 16>(zp + 16 * h * (D / 16), z0);
+        load_words<D / 16>(zp + z_other + 16 * h * (D / 16), z1);
+        load_words<D / 16>(zp + (16 * h + 8) * (D / 16), z2);
+        load_words<D / 16>(zp + z_other + (16 * h + 8) * (D / 16), z3);
+        load_words<D / 16>(vp + 16 * h * (D / 2), v0);
+        load_words<D / 16>(vp + v_other + 16 * h * (D / 2), v1);
+        load_words<D / 16>(vp + (16 * h + 8) * (D / 2), v2);
+        load_words<D / 16>(vp + v_other + (16 * h + 8) * (D / 2), v3);
+        if (h == kWarpTiles - 1) {  // the slot is free again
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.empty[slot]);
         }
-#pragma unroll
-        for (int w = 0; w < NG / 2; ++w) {  // a word: two groups
-          uint32_t ka[4], kb[4];
-          e2m1x8_f16(k0[w], ka);
-          e2m1x8_f16(k1[w], kb);
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint32_t frag[4] = {ka[2 * i], kb[2 * i], ka[2 * i + 1], kb[2 * i + 1]};
-            const float fa = i ? f16_hi(fs0[w]) : f16_lo(fs0[w]);
-            const float fb = i ? f16_hi(fs1[w]) : f16_lo(fs1[w]);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              float x[4] = {0.f, 0.f, 0.f, 0.f};
-              mma16816(x, frag, qf[nt][2 * w + i][0], qf[nt][2 * w + i][1]);
-              s[nt][0] = fmaf(fa, x[0], s[nt][0]);
-              s[nt][1] = fmaf(fa, x[1], s[nt][1]);
-              s[nt][2] = fmaf(fb, x[2], s[nt][2]);
-              s[nt][3] = fmaf(fb, x[3], s[nt][3]);
-            }
-          }
+        const int token = see.at(j) * kBlockTokens + tile0 + 16 * h;
+        const bool careful = !easy;  // alike in all lanes
+        if (careful) {  // does any row see any of the tile?
+          if ((bad >> (kWarpTiles * warp + h) & 1) || token >= see.last.hi ||
+              (token + 16 <= see.first.lo && token >= see.last.sk))
+            continue;
         }
-      }
-      // ---- logits in log2 units, masks
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[nt][e] *= sc[nt][e & 1];
-      unsigned hidden = 0;  // bit 4 nt + e: the row does not see the token
-      bool clean = true;
-      if (careful) {
+        // ---- scores of 16 tokens: s[nt][0, 1] row g of the tile, s[nt][2, 3] row g + 8
+        float s[NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int r = min(r0 + nt * 8 + 2 * t + (e & 1), rows - 1), i = r / a.group;
-            const int key = token + key_of + 8 * (e >> 1);
-            float x = s[nt][e];
-            if (a.softcap > 0.f) x = a.softcap * 1.4426950408889634f * tanh_any(x);
-            if (a.alibi != nullptr)
-              x -= a.alibi[(int64_t)b * a.Hq + hk * a.group + r % a.group] *
-                   1.4426950408889634f * fabsf((float)(i + len - a.Lq - key));
-            const Kv4Range seen = kv4_range(a, len, i);
-            const bool vis = (key >= seen.lo || key < seen.sk) && key < seen.hi;
-            s[nt][e] = vis ? x : -INFINITY;
-            hidden |= (vis ? 0u : 1u) << (4 * nt + e);
+          for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
+        {
+          uint32_t fs0[NG / 2], fs1[NG / 2];
+#pragma unroll
+          for (int w = 0; w < NG / 4; ++w) {
+            e4m3x4_f16(y0[w], fs0 + 2 * w);
+            e4m3x4_f16(y1[w], fs1 + 2 * w);
           }
-        // The NaN scale of a token must not reach a row that does not see it. Such tokens have
-        // probability 0 there, so with finite scales nothing is left to do.
-        bool nan = false;
 #pragma unroll
-        for (int w = 0; w < NG / 4; ++w)
-          nan = nan || has_nan_scale(z0[w]) || has_nan_scale(z1[w]) || has_nan_scale(z2[w]) ||
-                has_nan_scale(z3[w]);
-        clean = !__any_sync(kFull, nan);
-      }
-      bool grow = false;
+          for (int w = 0; w < NG / 2; ++w) {  // a word: two groups
+            uint32_t ka[4], kb[4];
+            e2m1x8_f16(k0[w], ka);
+            e2m1x8_f16(k1[w], kb);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t frag[4] = {ka[2 * i], kb[2 * i], ka[2 * i + 1], kb[2 * i + 1]};
+              const float fa = i ? f16_hi(fs0[w]) : f16_lo(fs0[w]);
+              const float fb = i ? f16_hi(fs1[w]) : f16_lo(fs1[w]);
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-          grow = grow || fmaxf(s[nt][e], s[nt][e + 2]) > m[nt][e] + kGrow;
-      if (__any_sync(kFull, grow)) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float top = fmaxf(s[nt][e], s[nt][e + 2]);
-#pragma unroll
-            for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, d));
-            if (top > m[nt][e] + kGrow) {
-              const float fresh = top - kBelow;
-              const float factor = m[nt][e] == -INFINITY ? 0.f : ex2(m[nt][e] - fresh);
-              m[nt][e] = m_sub[nt][e] = fresh;
-              l[nt][e] *= factor;
-#pragma unroll
-              for (int i = 0; i < NG; ++i) {
-                o[nt][i][e] *= factor;
-                o[nt][i][e + 2] *= factor;
+              for (int nt = 0; nt < NT; ++nt) {
+                float x[4] = {0.f, 0.f, 0.f, 0.f};
+                mma16816(x, frag, qf[nt][2 * w + i][0], qf[nt][2 * w + i][1]);
+                s[nt][0] = fmaf(fa, x[0], s[nt][0]);
+                s[nt][1] = fmaf(fa, x[1], s[nt][1]);
+                s[nt][2] = fmaf(fb, x[2], s[nt][2]);
+                s[nt][3] = fmaf(fb, x[3], s[nt][3]);
               }
             }
           }
-      }
-      // ---- probabilities
-      uint32_t pb[NT][2];
+        }
+        // ---- logits in log2 units, masks
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float p[4];
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) p[e] = ex2(s[nt][e] - m_sub[nt][e & 1]);
-        l[nt][0] += p[0] + p[2];
-        l[nt][1] += p[1] + p[3];
-        pb[nt][0] = transpose8x8(h2(p[0], p[1]));  // rows 2t, 2t + 1 of the tile for row g of q
-        pb[nt][1] = transpose8x8(h2(p[2], p[3]));  // rows 2t + 8, 2t + 9
-      }
-      // ---- values: a byte of two tokens' codes of one dim makes one operand register
-      auto values = [&](auto masked) {
-        uint32_t keep[NT][2];
-        if constexpr (decltype(masked)::value) {
+          for (int e = 0; e < 4; ++e) s[nt][e] *= sc[nt][e & 1];
+        unsigned hidden = 0;  // bit 4 nt + e: the row does not see the token
+        bool clean = true;
+        if (careful) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-              keep[nt][e] = transpose8x8((hidden >> (4 * nt + 2 * e) & 1 ? 0u : 0xffffu) |
-                                         (hidden >> (4 * nt + 2 * e + 1) & 1 ? 0u : 0xffff0000u));
+            for (int e = 0; e < 4; ++e) {
+              const int r = min(r0 + nt * 8 + 2 * t + (e & 1), rows - 1), i = r / a.group;
+              const int key = token + key_of + 8 * (e >> 1);
+              float x = s[nt][e];
+              if (a.softcap > 0.f) x = a.softcap * 1.4426950408889634f * tanh_any(x);
+              if (a.alibi != nullptr)
+                x -= a.alibi[(int64_t)b * a.Hq + hk * a.group + r % a.group] *
+                     1.4426950408889634f * fabsf((float)(i + len - a.Lq - key));
+              const Kv4Range seen = kv4_range(a, len, i);
+              const bool vis = (key >= seen.lo || key < seen.sk) && key < seen.hi;
+              s[nt][e] = vis ? x : -INFINITY;
+              hidden |= (vis ? 0u : 1u) << (4 * nt + e);
+            }
+          // The NaN scale of a token must not reach a row that does not see it. Such tokens have
+          // probability 0 there, so with finite scales nothing is left to do.
+          bool nan = false;
+#pragma unroll
+          for (int w = 0; w < NG / 4; ++w)
+            nan = nan || has_nan_scale(z0[w]) || has_nan_scale(z1[w]) || has_nan_scale(z2[w]) ||
+                  has_nan_scale(z3[w]);
+          clean = !__any_sync(kFull, nan);
         }
+        bool grow = false;
 #pragma unroll
-        for (int w = 0; w < NG / 4; ++w) {  // a word: four groups
-          uint32_t va[4], vb[4], vc[4], vd[4];
-          e2m1x8_f16((v0[w] & 0x0f0f0f0fu) | ((v1[w] << 4) & 0xf0f0f0f0u), va);  // dim g
-          e2m1x8_f16(((v0[w] >> 4) & 0x0f0f0f0fu) | (v1[w] & 0xf0f0f0f0u), vb);  // dim g + 8
-          e2m1x8_f16((v2[w] & 0x0f0f0f0fu) | ((v3[w] << 4) & 0xf0f0f0f0u), vc);
-          e2m1x8_f16(((v2[w] >> 4) & 0x0f0f0f0fu) | (v3[w] & 0xf0f0f0f0u), vd);
-          uint32_t sp[4], tp[4];  // pairs of tokens' scales, groups 4w .. 4w + 3
-          e4m3x4_f16(__byte_perm(z0[w], z1[w], 0x5140), sp);
-          e4m3x4_f16(__byte_perm(z0[w], z1[w], 0x7362), sp + 2);
-          e4m3x4_f16(__byte_perm(z2[w], z3[w], 0x5140), tp);
-          e4m3x4_f16(__byte_perm(z2[w], z3[w], 0x7362), tp + 2);
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t frag[4] = {va[i], vb[i], vc[i], vd[i]};
+          for (int e = 0; e < 2; ++e)
+            grow = grow || fmaxf(s[nt][e], s[nt][e + 2]) > m[nt][e] + kGrow;
+        if (__any_sync(kFull, grow)) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              uint32_t p0 = h2mul(pb[nt][0], sp[i]), p1 = h2mul(pb[nt][1], tp[i]);
-              if constexpr (decltype(masked)::value) {
-                p0 &= keep[nt][0];
-                p1 &= keep[nt][1];
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float top = fmaxf(s[nt][e], s[nt][e + 2]);
+#pragma unroll
+              for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, d));
+              if (top > m[nt][e] + kGrow) {
+                const float fresh = top - kBelow;
+                const float factor = m[nt][e] == -INFINITY ? 0.f : ex2(m[nt][e] - fresh);
+                m[nt][e] = m_sub[nt][e] = fresh;
+                l[nt][e] *= factor;
+#pragma unroll
+                for (int i = 0; i < NG; ++i) {
+                  o[nt][i][e] *= factor;
+                  o[nt][i][e + 2] *= factor;
+                }
               }
-              mma16816(o[nt][4 * w + i], frag, p0, p1);
+            }
+        }
+        // ---- probabilities
+        uint32_t pb[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float p[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) p[e] = ex2(s[nt][e] - m_sub[nt][e & 1]);
+          l[nt][0] += p[0] + p[2];
+          l[nt][1] += p[1] + p[3];
+          pb[nt][0] = transpose8x8(h2(p[0], p[1]));  // rows 2t, 2t + 1 of the tile for row g of q
+          pb[nt][1] = transpose8x8(h2(p[2], p[3]));  // rows 2t + 8, 2t + 9
+        }
+        // ---- values: a byte of two tokens' codes of one dim makes one operand register
+        auto values = [&](auto masked) {
+          uint32_t keep[NT][2];
+          if constexpr (decltype(masked)::value) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                keep[nt][e] = transpose8x8((hidden >> (4 * nt + 2 * e) & 1 ? 0u : 0xffffu) |
+                                           (hidden >> (4 * nt + 2 * e + 1) & 1 ? 0u : 0xffff0000u));
+          }
+#pragma unroll
+          for (int w = 0; w < NG / 4; ++w) {  // a word: four groups
+            uint32_t va[4], vb[4], vc[4], vd[4];
+            e2m1x8_f16((v0[w] & 0x0f0f0f0fu) | ((v1[w] << 4) & 0xf0f0f0f0u), va);  // dim g
+            e2m1x8_f16(((v0[w] >> 4) & 0x0f0f0f0fu) | (v1[w] & 0xf0f0f0f0u), vb);  // dim g + 8
+            e2m1x8_f16((v2[w] & 0x0f0f0f0fu) | ((v3[w] << 4) & 0xf0f0f0f0u), vc);
+            e2m1x8_f16(((v2[w] >> 4) & 0x0f0f0f0fu) | (v3[w] & 0xf0f0f0f0u), vd);
+            uint32_t sp[4], tp[4];  // pairs of tokens' scales, groups 4w .. 4w + 3
+            e4m3x4_f16(__byte_perm(z0[w], z1[w], 0x5140), sp);
+            e4m3x4_f16(__byte_perm(z0[w], z1[w], 0x7362), sp + 2);
+            e4m3x4_f16(__byte_perm(z2[w], z3[w], 0x5140), tp);
+            e4m3x4_f16(__byte_perm(z2[w], z3[w], 0x7362), tp + 2);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t frag[4] = {va[i], vb[i], vc[i], vd[i]};
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                uint32_t p0 = h2mul(pb[nt][0], sp[i]), p1 = h2mul(pb[nt][1], tp[i]);
+                if constexpr (decltype(masked)::value) {
+                  p0 &= keep[nt][0];
+                  p1 &= keep[nt][1];
+                }
+                mma16816(o[nt][4 * w + i], frag, p0, p1);
+              }
             }
           }
-        }
-      };
-      if (clean) values(BoolC<false>{});
-      else values(BoolC<true>{});
+        };
+        if (clean) values(BoolC<false>{});
+        else values(BoolC<true>{});
+      }
     }
 
     // ---- join the warps: a common reference per row, then their sums
@@ -953,19 +968,22 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(NT))
 }
 
 // Adds up the partial results of a row: one block per output row. Rows that one CTA finished are
-// left as they are; rows without visible keys become 0.
+// left as they are; rows without visible keys become 0. The parts' weights are made first, all at
+// once, so that the long loop only loads and adds.
+constexpr int kJoinThreads = 256;
+constexpr int kJoinParts = 512;  // weights held at a time
 template <int D, int NT>
-__global__ void __launch_bounds__(128) kv4_join(const __grid_constant__ Kv4Args a) {
-  constexpr int kRows = 8 * NT, kLanes = D / 4, kAtOnce = 128 / kLanes;
+__global__ void __launch_bounds__(kJoinThreads) kv4_join(const __grid_constant__ Kv4Args a) {
+  constexpr int kRows = 8 * NT, kLanes = D / 4, kAtOnce = kJoinThreads / kLanes;
   __shared__ float4 s_val[kAtOnce][kLanes];
-  __shared__ float s_sum[kAtOnce], s_top[4];
+  __shared__ float s_weight[kJoinParts], s_red[2][kJoinThreads / 32];
   const int h = (int)(blockIdx.x % a.Hq);
   const int64_t bi = blockIdx.x / a.Hq;
   const int i = (int)(bi % a.Lq), b = (int)(bi / a.Lq);
   const int hk = h / a.group, r = i * a.group + h % a.group, rb = r / kRows, rr = r % kRows;
   const int lane = threadIdx.x % kLanes, p = threadIdx.x / kLanes;
   const int len = kv4_length(a, b);
-  int head = 0, ahead = 0;  // blocks of the head's units, and of those before this one
+  int head = 0, ahead = 0;  // room of the head's units, and of those before this one
   int n = 0;
 #pragma unroll 1
   for (int x = 0; x < a.row_blocks; ++x) {
@@ -984,36 +1002,48 @@ __global__ void __launch_bounds__(128) kv4_join(const __grid_constant__ Kv4Args 
   }
   auto part = [&](int cta) { return (2 * (int64_t)cta + (cta == c0)) * kRows + rr; };
   float top = -INFINITY;
-  for (int x = c0 + threadIdx.x; x <= c1; x += 128) top = fmaxf(top, a.ws_m[part(x)]);
+  for (int x = c0 + threadIdx.x; x <= c1; x += kJoinThreads) top = fmaxf(top, a.ws_m[part(x)]);
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, d));
-  if (threadIdx.x % 32 == 0) s_top[threadIdx.x / 32] = top;
+  if (threadIdx.x % 32 == 0) s_red[0][threadIdx.x / 32] = top;
   __syncthreads();
-  top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
+#pragma unroll
+  for (int w = 0; w < kJoinThreads / 32; ++w) top = fmaxf(top, s_red[0][w]);
   float sum = 0.f;
   float4 val = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int x = c0 + p; x <= c1; x += kAtOnce) {
-    const int64_t at = part(x);
-    const float l = a.ws_l[at], m = a.ws_m[at];
-    const float f = l != l ? l : m == -INFINITY ? 0.f : ex2(m - top);
-    const float4 y = reinterpret_cast<const float4*>(a.ws_o + at * D)[lane];
-    sum = fmaf(f, l, sum);
-    val.x = fmaf(f, y.x, val.x);
-    val.y = fmaf(f, y.y, val.y);
-    val.z = fmaf(f, y.z, val.z);
-    val.w = fmaf(f, y.w, val.w);
+  for (int from = c0; from <= c1; from += kJoinParts) {
+    const int to = min(c1 + 1, from + kJoinParts);
+    if (from > c0) __syncthreads();
+    for (int x = from + threadIdx.x; x < to; x += kJoinThreads) {
+      const float l = a.ws_l[part(x)], m = a.ws_m[part(x)];
+      const float f = l != l ? l : m == -INFINITY ? 0.f : ex2(m - top);
+      s_weight[x - from] = f;
+      sum = fmaf(f, l, sum);
+    }
+    __syncthreads();
+#pragma unroll 8
+    for (int x = from + p; x < to; x += kAtOnce) {
+      const float f = s_weight[x - from];
+      const float4 y = reinterpret_cast<const float4*>(a.ws_o + part(x) * D)[lane];
+      val.x = fmaf(f, y.x, val.x);
+      val.y = fmaf(f, y.y, val.y);
+      val.z = fmaf(f, y.z, val.z);
+      val.w = fmaf(f, y.w, val.w);
+    }
   }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(kFull, sum, d);
+  if (threadIdx.x % 32 == 0) s_red[1][threadIdx.x / 32] = sum;
   s_val[p][lane] = val;
-  if (lane == 0) s_sum[p] = sum;
   __syncthreads();
   if (threadIdx.x >= kLanes) return;
-  sum = s_sum[0];
+  sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < kJoinThreads / 32; ++w) sum += s_red[1][w];
   val = s_val[0][lane];
 #pragma unroll
   for (int x = 1; x < kAtOnce; ++x) {
     const float4 y = s_val[x][lane];
-    sum += s_sum[x];
     val.x += y.x;
     val.y += y.y;
     val.z += y.z;
@@ -1154,7 +1184,7 @@ int launch_fwd(const Kv4Args& a, int ctas, int dev, cudaStream_t st) {
   kv4_attn<D, NT><<<ctas, kAttnThreads, smem, st>>>(a);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((int64_t)a.c.B * a.Lq * a.Hq));
-  cfg.blockDim = dim3(128);
+  cfg.blockDim = dim3(kJoinThreads);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
