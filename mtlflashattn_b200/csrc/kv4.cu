@@ -242,7 +242,7 @@ struct Kv4Args {
   int64_t q_sb, q_ss, q_sh, o_sb, o_ss, o_sh;
   const int* seqlens;
   int Lq, Hq, group, bf16;
-  int q_vec8;  // every 4 dims of a query row can be read at once
+  uint32_t group_mul, group_shift;  // r / group = (umulhi(r, mul) + r) >> shift, r < 2^31
   float scale_l2;  // scale * k_unit * log2(e) (softcap: scale * k_unit / softcap)
   float softcap;
   int causal, wl, wr, sink;
@@ -281,6 +281,10 @@ __host__ __device__ constexpr int kv4_ctas(int nt) { return nt == 1 ? KV4_C1 : K
 constexpr float kGrow = 7.f;   // a row's reference is renewed when a score passes it by 2^7
 constexpr float kBelow = 3.f;  // and is then set 2^3 below the new maximum
 
+__device__ __forceinline__ int kv4_pos(const Kv4Args& a, int r) {  // r / group
+  return (int)((__umulhi((uint32_t)r, a.group_mul) + (uint32_t)r) >> a.group_shift);
+}
+
 struct Kv4Range {
   int lo, hi, sk;
 };
@@ -313,8 +317,8 @@ template <int kRows>
 __device__ __forceinline__ Kv4Span kv4_span(const Kv4Args& a, int len, int rb) {
   const int rows = a.Lq * a.group, r0 = rb * kRows;
   Kv4Span s;
-  s.first = kv4_range(a, len, r0 / a.group);
-  s.last = kv4_range(a, len, (min(r0 + kRows, rows) - 1) / a.group);
+  s.first = kv4_range(a, len, kv4_pos(a, r0));
+  s.last = kv4_range(a, len, kv4_pos(a, min(r0 + kRows, rows) - 1));
   constexpr unsigned kT = kBlockTokens;
   const bool any = s.last.hi > s.first.lo;
   s.w0 = (unsigned)(any ? s.first.lo : s.first.lo + (int)kT - 1) / kT;
@@ -456,9 +460,11 @@ struct Kv4Smem {
   static constexpr uint32_t kCodes = kBlockTokens * D / 2, kScales = kBlockTokens * D / 16;
   static constexpr uint32_t kStage = 2 * kCodes + 2 * kScales;  // K, V, K scales, V scales
   alignas(128) uint8_t ring[kAttnStages][kStage];
+  // a unit's query rows, as they are; the padding spreads 8 rows over the banks
+  alignas(16) uint16_t q[kRows][D + 16];
   float o[kAttnWarps][kRows][D + 4];  // the warps' sums, to be joined
   float m[kAttnWarps][kRows], l[kAttnWarps][kRows];
-  uint64_t full[kAttnStages], empty[kAttnStages];
+  uint64_t full[kAttnStages], empty[kAttnStages], q_full, q_empty;
   unsigned bad[kAttnStages];  // bit i: tokens [16 i, 16 i + 16) of the block have no page
   int scan[kAttnThreads / 32];
   int b, hk, rb, j, share;
@@ -497,6 +503,8 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(NT))
         mbar_init(&sm.full[i], 1);
         mbar_init(&sm.empty[i], kAttnWarps);
       }
+      mbar_init(&sm.q_full, 1);
+      mbar_init(&sm.q_empty, kAttnWarps);
       fence_mbar_init();
     }
     __syncthreads();
@@ -572,11 +580,26 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(NT))
         w.next(a);
       }
     };
-    int it = 0;
+    int it = 0, unit = 0;
     int pages = page_of(walk);
     Kv4Walk<kRows> ahead = walk;
-    bool ok = true;
+    bool ok = true, fresh = true;  // fresh: a unit begins
     while (walk.take > 0 && ok) {
+      if (fresh) {  // its query rows, one per lane
+        ok = __all_sync(kFull, mbar_wait(&sm.q_empty, (uint32_t)(unit & 1) ^ 1u, abort_flag));
+        if (!ok) break;
+        const int r0 = walk.rb * kRows, n = min(kRows, a.Lq * a.group - r0);
+        if (lane == 0) mbar_expect_tx(&sm.q_full, (uint32_t)n * D * 2);
+        __syncwarp();
+        if (lane < n) {
+          const int i = kv4_pos(a, r0 + lane), h = walk.hk * a.group + r0 + lane - i * a.group;
+          const int64_t at = walk.b * a.q_sb + i * a.q_ss + (int64_t)h * a.q_sh;
+          bulk_load(reinterpret_cast<uint8_t*>(sm.q[lane]),
+                    static_cast<const uint8_t*>(a.q) + 2 * at, D * 2, &sm.q_full);
+        }
+        ++unit;
+      }
+      fresh = walk.take <= batch;
       skip(ahead);
       const int pages_next = page_of(ahead);
       const int n = min(walk.take, batch);
@@ -621,6 +644,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(NT))
     // every copy has landed before the CTA's shared memory is given back
     for (int i = max(0, it - kAttnStages); i < it; ++i)
       mbar_wait_drain(&sm.full[i % kAttnStages], (uint32_t)(i / kAttnStages) & 1u);
+    if (unit > 0) mbar_wait_drain(&sm.q_full, (uint32_t)(unit - 1) & 1u);
     if (lane == 0 && sm.abort && c.err != nullptr) atomicExch(c.err, MFA_ERR_TIMEOUT);
     return;
   }
@@ -632,32 +656,23 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(NT))
   const int key_of = g ^ ((g >> 1) & 1);
   const int rows = a.Lq * a.group;
   const bool general = a.softcap > 0.f || a.alibi != nullptr;
-  int it = 0;
+  int it = 0, unit = 0;
   bool ok = true;  // after a wait that gave up: no more tiles, but every barrier is still met
   while (walk.take > 0) {
     const int b = walk.b, hk = walk.hk, r0 = walk.rb * kRows, len = walk.len;
     // query fragments: lane (g, t) has dims 16 i + 4 t .. + 3 of row g of each tile of 8 rows
+    ok = ok && __all_sync(kFull, mbar_wait(&sm.q_full, (uint32_t)unit & 1u, abort_flag));
+    ++unit;
     uint32_t qf[NT][NG][2];
     float inv_f[NT];  // what a row was multiplied by, inverted
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int r = r0 + nt * 8 + g;
       float x[NG][4];
       float top = 0.f;
-      const int64_t at = b * a.q_sb + (r / a.group) * a.q_ss +
-                         (int64_t)(hk * a.group + r % a.group) * a.q_sh + 4 * t;
-      const uint16_t* qp = reinterpret_cast<const uint16_t*>(a.q) + at;
 #pragma unroll
       for (int i = 0; i < NG; ++i) {
-        uint2 raw = make_uint2(0, 0);
-        if (r < rows) {
-          if (a.q_vec8) {
-            raw = *reinterpret_cast<const uint2*>(qp + 16 * i);
-          } else {
-            raw.x = qp[16 * i] | (uint32_t)qp[16 * i + 1] << 16;
-            raw.y = qp[16 * i + 2] | (uint32_t)qp[16 * i + 3] << 16;
-          }
-        }
+        uint2 raw = *reinterpret_cast<const uint2*>(&sm.q[nt * 8 + g][16 * i + 4 * t]);
+        if (r0 + nt * 8 + g >= rows) raw = make_uint2(0, 0);
         if (a.bf16) {
           x[i][0] = __uint_as_float(raw.x << 16);
           x[i][1] = __uint_as_float(raw.x & 0xffff0000u);
@@ -686,6 +701,8 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(NT))
         qf[nt][i][1] = h2(x[i][2] * f, x[i][3] * f);
       }
     }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sm.q_empty);
     // this lane's score columns are rows 2t and 2t + 1 of each tile of 8; m is the reference
     // and m_sub what is subtracted (0 while there is none)
     float sc[NT][2], m[NT][2], m_sub[NT][2], l[NT][2];
@@ -801,12 +818,12 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(NT))
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const int r = min(r0 + nt * 8 + 2 * t + (e & 1), rows - 1), i = r / a.group;
+              const int r = min(r0 + nt * 8 + 2 * t + (e & 1), rows - 1), i = kv4_pos(a, r);
               const int key = token + key_of + 8 * (e >> 1);
               float x = s[nt][e];
               if (a.softcap > 0.f) x = a.softcap * 1.4426950408889634f * tanh_any(x);
               if (a.alibi != nullptr)
-                x -= a.alibi[(int64_t)b * a.Hq + hk * a.group + r % a.group] *
+                x -= a.alibi[(int64_t)b * a.Hq + hk * a.group + r - i * a.group] *
                      1.4426950408889634f * fabsf((float)(i + len - a.Lq - key));
               const Kv4Range seen = kv4_range(a, len, i);
               const bool vis = (key >= seen.lo || key < seen.sk) && key < seen.hi;
@@ -949,7 +966,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(NT))
         val.w += y.w;
       }
       if (whole) {
-        const int i = r / a.group, h = hk * a.group + r % a.group;
+        const int i = kv4_pos(a, r), h = hk * a.group + r - i * a.group;
         kv4_store(a, b * a.o_sb + i * a.o_ss + (int64_t)h * a.o_sh + d, val, sum);
       } else {
         *reinterpret_cast<float4*>(a.ws_o + (part + rr) * D + d) = val;
@@ -1153,7 +1170,8 @@ int check_fwd(const mfa_kv4_cache* c, const mfa_kv4_fwd_params* p) {
     return MFA_ERR_UNSUPPORTED;
   if (reinterpret_cast<uintptr_t>(p->o) % 8 != 0) return MFA_ERR_INVALID;
   for (int i = 0; i < 3; ++i)
-    if (p->o_stride[i] % 4 != 0) return MFA_ERR_INVALID;
+    if (p->o_stride[i] % 4 != 0 || p->q_stride[i] % 8 != 0) return MFA_ERR_INVALID;
+  if (!aligned16(p->q)) return MFA_ERR_INVALID;
   return MFA_OK;
 }
 
@@ -1255,8 +1273,11 @@ int mfa_kv4_fwd(const mfa_kv4_cache* c, const mfa_kv4_fwd_params* p, void* strea
   a.Hq = p->Hq;
   a.group = p->Hq / c->Hkv;
   a.bf16 = p->dtype == MFA_BF16;
-  a.q_vec8 = reinterpret_cast<uintptr_t>(p->q) % 8 == 0;
-  for (int i = 0; i < 3; ++i) a.q_vec8 = a.q_vec8 && p->q_stride[i] % 4 == 0;
+  // multiplier of the exact division by the group: shift = ceil(log2(group)),
+  // mul = floor(2^32 (2^shift - group) / group) + 1
+  a.group_shift = 0;
+  while ((1u << a.group_shift) < (uint32_t)a.group) ++a.group_shift;
+  a.group_mul = (uint32_t)((((1ull << a.group_shift) - a.group) << 32) / a.group + 1);
   a.softcap = p->softcap;
   a.scale_l2 = p->scale * c->k_unit *
                (p->softcap > 0.f ? 1.f / p->softcap : 1.4426950408889634f);

@@ -246,7 +246,10 @@ def flash_attn_with_kv4cache(q, cache, block_table, cache_seqlens, softmax_scale
         if not torch.is_tensor(alibi_slopes):
             raise TypeError("mtlflashattn_b200: alibi_slopes must be a tensor of per-head slopes")
         alibi = _broadcast_alibi_slopes(alibi_slopes, B, Hq, dev)
-    x = _kernel._last_dim_contig(q)
+    x = q
+    sb, ss, sh, sd = q.stride()
+    if sd != 1 or (sb | ss | sh) % 8 or q.data_ptr() % 16:
+        x = q.clone(memory_format=torch.contiguous_format)  # rows are copied in 16-byte pieces
     out = torch.empty(q.shape, dtype=q.dtype, device=dev)
     scale = softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(D)
     far = 2**31 - 1
