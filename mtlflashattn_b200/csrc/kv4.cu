@@ -256,28 +256,13 @@ struct Kv4Args {
 
 constexpr int kAttnWarps = 4;                  // consumer warps
 constexpr int kAttnThreads = 32 * kAttnWarps + 32;
-#ifndef KV4_TILES
-#define KV4_TILES 2
-#endif
-#ifndef KV4_STAGES
-#define KV4_STAGES 3
-#endif
-constexpr int kWarpTiles = KV4_TILES;  // tiles of 16 tokens that a consumer takes of a block
+constexpr int kWarpTiles = 2;  // tiles of 16 tokens that a consumer takes of a block
 constexpr int kBlockTokens = 16 * kWarpTiles * kAttnWarps;
 constexpr int kBlockTiles = kBlockTokens / 16;
-constexpr int kAttnStages = KV4_STAGES;
+constexpr int kAttnStages = 3;
 constexpr int kMinShare = 2;   // blocks per CTA at least: below, joining costs more than it gives
-#ifndef KV4_UNIT
-#define KV4_UNIT 3
-#endif
-constexpr int kUnitCost = KV4_UNIT;  // beginning and ending a unit takes about as long as so many blocks
-#ifndef KV4_C1
-#define KV4_C1 3
-#endif
-#ifndef KV4_C2
-#define KV4_C2 3
-#endif
-__host__ __device__ constexpr int kv4_ctas(int nt) { return nt == 1 ? KV4_C1 : KV4_C2; }  // per SM
+constexpr int kUnitCost = 3;  // beginning and ending a unit takes about as long as so many blocks
+constexpr int kAttnCtas = 3;   // per SM
 constexpr float kGrow = 7.f;   // a row's reference is renewed when a score passes it by 2^7
 constexpr float kBelow = 3.f;  // and is then set 2^3 below the new maximum
 
@@ -434,11 +419,6 @@ __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* w) {
   }
 }
 
-// Barrier of the consumer warps.
-__device__ __forceinline__ void consumers_meet() {
-  asm volatile("bar.sync 1, %0;" ::"n"(32 * kAttnWarps) : "memory");
-}
-
 // Four columns of an output row from their weighted sums and the sum of the weights.
 __device__ __forceinline__ void kv4_store(const Kv4Args& a, int64_t at, float4 val, float sum) {
   const float f = sum == 0.f ? 0.f : a.c.v_unit / sum;
@@ -454,6 +434,12 @@ __device__ __forceinline__ void kv4_store(const Kv4Args& a, int64_t at, float4 v
   *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.o) + at) = w;
 }
 
+// What the consumers have to know of a unit's part: blocks [j, j + take) of its span.
+struct Kv4Unit {
+  int b, hk, r0, len, j, take;  // take = 0: there are no more
+  Kv4Span span;
+};
+
 template <int D, int NT>
 struct Kv4Smem {
   static constexpr int kRows = 8 * NT;
@@ -464,7 +450,8 @@ struct Kv4Smem {
   alignas(16) uint16_t q[kRows][D + 16];
   float o[kAttnWarps][kRows][D + 4];  // the warps' sums, to be joined
   float m[kAttnWarps][kRows], l[kAttnWarps][kRows];
-  uint64_t full[kAttnStages], empty[kAttnStages], q_full, q_empty;
+  Kv4Unit unit[2];  // this one and, while its end is being written, the next one
+  uint64_t full[kAttnStages], empty[kAttnStages], q_full, q_empty, met;
   unsigned bad[kAttnStages];  // bit i: tokens [16 i, 16 i + 16) of the block have no page
   int scan[kAttnThreads / 32];
   int b, hk, rb, j, share;
@@ -472,7 +459,7 @@ struct Kv4Smem {
 };
 
 template <int D, int NT>
-__global__ void __launch_bounds__(kAttnThreads, kv4_ctas(NT))
+__global__ void __launch_bounds__(kAttnThreads, kAttnCtas)
     kv4_attn(const __grid_constant__ Kv4Args a) {
   constexpr int NG = D / 16, kRows = 8 * NT;
   using Smem = Kv4Smem<D, NT>;
@@ -505,6 +492,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(NT))
       }
       mbar_init(&sm.q_full, 1);
       mbar_init(&sm.q_empty, kAttnWarps);
+      mbar_init(&sm.met, kAttnWarps);
       fence_mbar_init();
     }
     __syncthreads();
@@ -548,19 +536,19 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(NT))
     }
     __syncthreads();
   }
-  Kv4Walk<kRows> walk;
-  walk.b = sm.b;
-  walk.hk = sm.hk;
-  walk.rb = sm.rb;
-  walk.j = sm.j;
-  walk.left = sm.share;
-  walk.look(a);
   volatile int* abort_flag = &sm.abort;
 
   if (warp == kAttnWarps) {
     // ---------------------------------------------------------------- producer
     // A block is one piece, or as many as it has pages. The lanes look up the pages of the next 32
     // pieces at once, a batch ahead of the one whose copies are being issued.
+    Kv4Walk<kRows> walk;
+    walk.b = sm.b;
+    walk.hk = sm.hk;
+    walk.rb = sm.rb;
+    walk.j = sm.j;
+    walk.left = sm.share;
+    walk.look(a);
     const int piece = min(kBlockTokens, 1 << c.page_shift);
     const int pshift = min(__ffs(kBlockTokens) - 1, c.page_shift);         // log2(piece)
     const int bshift = __ffs(kBlockTokens) - 1 - pshift, batch = 32 >> bshift;  // blocks
@@ -584,12 +572,22 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(NT))
     int pages = page_of(walk);
     Kv4Walk<kRows> ahead = walk;
     bool ok = true, fresh = true;  // fresh: a unit begins
-    while (walk.take > 0 && ok) {
-      if (fresh) {  // its query rows, one per lane
+    while (ok) {
+      if (fresh) {  // its description, and its query rows, one per lane
         ok = __all_sync(kFull, mbar_wait(&sm.q_empty, (uint32_t)(unit & 1) ^ 1u, abort_flag));
         if (!ok) break;
-        const int r0 = walk.rb * kRows, n = min(kRows, a.Lq * a.group - r0);
-        if (lane == 0) mbar_expect_tx(&sm.q_full, (uint32_t)n * D * 2);
+        const int r0 = walk.rb * kRows, n = walk.take > 0 ? min(kRows, a.Lq * a.group - r0) : 0;
+        if (lane == 0) {
+          Kv4Unit& u = sm.unit[unit & 1];
+          u.b = walk.b;
+          u.hk = walk.hk;
+          u.r0 = r0;
+          u.len = walk.len;
+          u.j = walk.j;
+          u.take = walk.take;
+          u.span = walk.span;
+          mbar_expect_tx(&sm.q_full, (uint32_t)n * D * 2);
+        }
         __syncwarp();
         if (lane < n) {
           const int i = kv4_pos(a, r0 + lane), h = walk.hk * a.group + r0 + lane - i * a.group;
@@ -598,6 +596,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(NT))
                     static_cast<const uint8_t*>(a.q) + 2 * at, D * 2, &sm.q_full);
         }
         ++unit;
+        if (walk.take == 0) break;
       }
       fresh = walk.take <= batch;
       skip(ahead);
@@ -656,13 +655,19 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(NT))
   const int key_of = g ^ ((g >> 1) & 1);
   const int rows = a.Lq * a.group;
   const bool general = a.softcap > 0.f || a.alibi != nullptr;
-  int it = 0, unit = 0;
-  bool ok = true;  // after a wait that gave up: no more tiles, but every barrier is still met
-  while (walk.take > 0) {
-    const int b = walk.b, hk = walk.hk, r0 = walk.rb * kRows, len = walk.len;
+  int it = 0;
+  uint32_t meetings = 0;
+  auto meet = [&] {  // the consumer warps, after what each wrote to shared memory
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sm.met);
+    return __all_sync(kFull, mbar_wait(&sm.met, meetings++ & 1u, abort_flag)) != 0;
+  };
+  for (int unit = 0;; ++unit) {
+    bool ok = __all_sync(kFull, mbar_wait(&sm.q_full, (uint32_t)unit & 1u, abort_flag));
+    const Kv4Unit& u = sm.unit[unit & 1];
+    if (!ok || u.take == 0) break;
+    const int r0 = u.r0;
     // query fragments: lane (g, t) has dims 16 i + 4 t .. + 3 of row g of each tile of 8 rows
-    ok = ok && __all_sync(kFull, mbar_wait(&sm.q_full, (uint32_t)unit & 1u, abort_flag));
-    ++unit;
     uint32_t qf[NT][NG][2];
     float inv_f[NT];  // what a row was multiplied by, inverted
 #pragma unroll
@@ -722,13 +727,14 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(NT))
     }
 
     // blocks whose every token all rows see: [j_full, j_full + n_full) of the window
-    const Kv4Span& see = walk.span;
+    const Kv4Span& see = u.span;
     const int j_full = see.s1 - see.w0 + (see.last.lo + kBlockTokens - 1) / kBlockTokens;
     const unsigned n_full = max(0, see.s1 - see.w0 + see.first.hi / kBlockTokens - j_full);
 
-    for (int j = walk.j; j < walk.j + walk.take; ++j, ++it) {
+    const int j_end = u.j + u.take;
+    for (int j = u.j; j < j_end; ++j, ++it) {
       const int slot = it % kAttnStages;
-      ok = ok && __all_sync(kFull, mbar_wait(&sm.full[slot], (uint32_t)(it / kAttnStages) & 1u,
+      ok = __all_sync(kFull, mbar_wait(&sm.full[slot], (uint32_t)(it / kAttnStages) & 1u,
                                              abort_flag));
       if (!ok) break;
       const unsigned bad = sm.bad[slot];
@@ -823,9 +829,9 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(NT))
               float x = s[nt][e];
               if (a.softcap > 0.f) x = a.softcap * 1.4426950408889634f * tanh_any(x);
               if (a.alibi != nullptr)
-                x -= a.alibi[(int64_t)b * a.Hq + hk * a.group + r - i * a.group] *
-                     1.4426950408889634f * fabsf((float)(i + len - a.Lq - key));
-              const Kv4Range seen = kv4_range(a, len, i);
+                x -= a.alibi[(int64_t)u.b * a.Hq + u.hk * a.group + r - i * a.group] *
+                     1.4426950408889634f * fabsf((float)(i + u.len - a.Lq - key));
+              const Kv4Range seen = kv4_range(a, u.len, i);
               const bool vis = (key >= seen.lo || key < seen.sk) && key < seen.hi;
               s[nt][e] = vis ? x : -INFINITY;
               hidden |= (vis ? 0u : 1u) << (4 * nt + e);
@@ -921,6 +927,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(NT))
       }
     }
 
+    if (!ok) break;
     // ---- join the warps: a common reference per row, then their sums
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -930,7 +937,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(NT))
         for (int d = 4; d < 32; d <<= 1) l[nt][e] += __shfl_xor_sync(kFull, l[nt][e], d);
         if (g == 0) sm.m[warp][nt * 8 + 2 * t + e] = m[nt][e];
       }
-    consumers_meet();
+    if (!meet()) break;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -948,9 +955,9 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(NT))
           sm.o[warp][r][16 * i + 8 + g] = o[nt][i][e + 2] * f;
         }
       }
-    consumers_meet();
-    const bool whole = walk.take == walk.span.n;
-    const int64_t part = (2 * (int64_t)blockIdx.x + (walk.j == 0)) * kRows;
+    if (!meet()) break;
+    const bool whole = u.take == u.span.n;
+    const int64_t part = (2 * (int64_t)blockIdx.x + (u.j == 0)) * kRows;
     for (int x = threadIdx.x; x < kRows * (D / 4); x += 32 * kAttnWarps) {
       const int rr = x / (D / 4), d = x % (D / 4) * 4, r = r0 + rr;
       if (r >= rows) break;
@@ -966,8 +973,8 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(NT))
         val.w += y.w;
       }
       if (whole) {
-        const int i = kv4_pos(a, r), h = hk * a.group + r - i * a.group;
-        kv4_store(a, b * a.o_sb + i * a.o_ss + (int64_t)h * a.o_sh + d, val, sum);
+        const int i = kv4_pos(a, r), h = u.hk * a.group + r - i * a.group;
+        kv4_store(a, u.b * a.o_sb + i * a.o_ss + (int64_t)h * a.o_sh + d, val, sum);
       } else {
         *reinterpret_cast<float4*>(a.ws_o + (part + rr) * D + d) = val;
         if (d == 0) {
@@ -979,8 +986,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(NT))
         }
       }
     }
-    consumers_meet();
-    walk.next(a);
+    if (!meet()) break;
   }
 }
 
@@ -1186,7 +1192,7 @@ Kv4Plan plan_fwd(const mfa_kv4_cache* c, const mfa_kv4_fwd_params* p, int sms) {
   const int64_t rows = (int64_t)p->Lq * (p->Hq / c->Hkv);
   k.nt = rows > 8 ? 2 : 1;
   k.row_blocks = (int)((rows + 8 * k.nt - 1) / (8 * k.nt));
-  k.ctas = sms * kv4_ctas(k.nt);
+  k.ctas = sms * kAttnCtas;
   const int64_t parts = 2ll * k.ctas * 8 * k.nt;
   k.line = ((c->B + 1) * 4ll + 127) / 128 * 128;
   k.o = parts * c->D * 4;
