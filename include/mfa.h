@@ -312,7 +312,8 @@ typedef struct mfa_kv4_cache {
 
 /* Rows going in (mfa_kv4_append) or coming out (mfa_kv4_gather). */
 typedef struct mfa_kv4_rows {
-  void* k;            /* [B, L, Hkv, D], any (batch, seq, head) strides, last dim stride 1 */
+  void* k;            /* [B, L, Hkv, D], 16-byte aligned, last dim stride 1, the other strides
+                         (batch, seq, head) multiples of 16 bytes */
   void* v;
   int64_t k_stride[3];
   int64_t v_stride[3];

@@ -33,6 +33,7 @@ struct FwdArgs {
   int group;  // Hq / Hkv
   const int* cu_q;
   const int* cu_k;
+  const int* k_lens;  // dense, padded keys: each sequence's key count (NULL: Lk)
   int max_lq;
   float scale, softcap;
   int causal, wl, wr;
@@ -94,7 +95,7 @@ __device__ __forceinline__ SeqView seq_view(const FwdArgs& a, int b) {
     s.q0 = 0;
     s.lq = a.Lq;
     s.k0 = 0;
-    s.lk = a.Lk;
+    s.lk = a.k_lens == nullptr ? a.Lk : max(0, min(a.k_lens[b], a.Lk));
     s.qb = b;
     s.kb = b;
   }

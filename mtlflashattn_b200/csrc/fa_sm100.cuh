@@ -359,27 +359,29 @@ __global__ void __launch_bounds__(sm100::Roles<CG, TILES>::kThreads,
   // union of the rows' key intervals: lo and hi are nondecreasing in the position
   int klo = key_range(a, sv, r0 >> ps).lo;
   int khi = key_range(a, sv, r_last >> ps).hi;
-  if (a.num_splits > 1) {
+  if (!kSink && a.num_splits > 1) {
     klo = max(klo, split * a.split_keys);
     if (split + 1 < a.num_splits) khi = min(khi, (split + 1) * a.split_keys);
   }
   int jb = klo / KBN;
   int n = khi > klo ? (khi + KBN - 1) / KBN - jb : 0;
-  // blocks [sb0, sb0 + nsb) hold first keys that stay visible, all below block jb
-  int sb0 = 0, nsb = 0;
+  // blocks [0, nsb) hold first keys that stay visible, all below block jb. The splits share the
+  // visible blocks evenly, not the keys: a window is a small part of a long sequence.
+  int nsb = 0, j_first = 0;
   if constexpr (kSink) {
     if (n == 0) jb = (klo + KBN - 1) / KBN;
-    int sk = key_range(a, sv, r_last >> ps).sk;  // nondecreasing in the position, as hi is
-    if (a.num_splits > 1) {
-      sb0 = split * (a.split_keys / KBN);  // a split is a whole number of blocks
-      if (split + 1 < a.num_splits) sk = min(sk, (split + 1) * a.split_keys);
-    }
-    nsb = max(0, min((sk + KBN - 1) / KBN, jb) - sb0);
+    const int sk = key_range(a, sv, r_last >> ps).sk;  // nondecreasing in the position, as hi is
+    nsb = min((sk + KBN - 1) / KBN, jb);
     n += nsb;
+    if (a.num_splits > 1) {
+      const int per = (n + a.num_splits - 1) / a.num_splits;
+      j_first = split * per;
+      n = max(0, min(n - j_first, per));
+    }
   }
   // the j-th key block of this CTA
   auto block_at = [&](int j) {
-    if constexpr (kSink) return j < nsb ? sb0 + j : jb + j - nsb;
+    if constexpr (kSink) return j + j_first < nsb ? j + j_first : jb + j + j_first - nsb;
     else return jb + j;
   };
 

@@ -9,6 +9,8 @@
 #include <cstring>
 #include <mutex>
 
+#include "../../include/mfa.h"
+
 namespace mfa {
 
 // ------------------------------------------------------------------ host fault injection
@@ -75,6 +77,10 @@ cudaError_t ensure_smem(K kernel, int dev, int bytes) {
   }
   return e;
 }
+
+// mfa_fwd of dense, padded keys whose sequence b has k_lens[b] (device; at most p->Lk, which it is
+// cut to) of them; a row's centre follows from that length (mfa_api.cu).
+int forward_padded(const mfa_fwd_params* p, const int32_t* k_lens, cudaStream_t st);
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 

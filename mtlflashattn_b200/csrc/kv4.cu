@@ -5,6 +5,7 @@
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "../../include/mfa.h"
@@ -44,11 +45,6 @@ __device__ __forceinline__ int64_t kv4_row(const Kv4Cache& c, int b, int64_t t) 
 }
 
 // ------------------------------------------------------------------ 4-bit and 8-bit conversions
-// The code in the low 4 bits: as the top bits of an fp16 it stands for 2^-14 of its value.
-__device__ __forceinline__ float e2m1_f32(uint32_t code) {
-  return __half2float(__ushort_as_half((unsigned short)((code & 8u) << 12 | (code & 7u) << 9))) *
-         16384.f;
-}
 // The codes of a word's four bytes, two each with the low half first, as fp16. The word
 // must not come straight from an 8- or 16-bit load: with one, ptxas 12.9 took the wrong bytes.
 __device__ __forceinline__ void e2m1x8_f16(uint32_t w, uint32_t* d) {
@@ -88,133 +84,243 @@ __device__ __forceinline__ float f16_hi(uint32_t h2) {
   return __high2float(*reinterpret_cast<const __half2*>(&h2));
 }
 
-// ------------------------------------------------------------------ append
+// ------------------------------------------------------------------ append and gather
+// Both are bound by memory: 16-bit rows on one side, 0.28 of their bytes on the other. A CTA takes
+// a tile of 4096 codes of one head (32 rows of D = 128, 64 of D = 64), keys or values, through
+// shared memory, where the layout's permutation happens, so that every access to memory is 16
+// bytes of a row; rows are (sequence, token) pairs in one line and look up their pages themselves.
 struct Kv4Rows {
-  const void *k, *v;
+  void *k, *v;
   int64_t k_sb, k_ss, k_sh, v_sb, v_ss, v_sh;
   const int *start, *lens;
   int L;
+  // gather for the 16-bit forward: 1 = only the tokens that its blocks of 128 keys can touch, and
+  // zeros up to the end of a sequence's last block
+  int visible_only, Lq, wl, sink;
 };
+constexpr int kRowThreads = 128;
 
-// One lane holds 4 consecutive dims of a row, 4 lanes a group. blockIdx.y: 0 keys, 1 values.
+// Which row of the pool a (sequence, row) pair is: -1 without a page, -2 where there is none to do.
+__device__ __forceinline__ int64_t kv4_find(const Kv4Cache& c, int b, int64_t t, int h, bool wanted) {
+  if (!wanted) return -2;
+  const int64_t row = kv4_row(c, b, t);
+  return row < 0 ? -1 : row + ((int64_t)h << c.page_shift);
+}
+
 template <typename T, int D>
-__global__ void __launch_bounds__(128) kv4_append_kernel(const Kv4Cache c, const Kv4Rows r) {
-  constexpr int kLanes = D / 4, NG = D / 16;
-  const int64_t row = ((int64_t)blockIdx.x * 128 + threadIdx.x) / kLanes;  // (b, j, head)
-  const int lane = threadIdx.x % kLanes;
-  const bool is_v = blockIdx.y != 0;
-  const int h = (int)(row % c.Hkv);
-  const int64_t bj = row / c.Hkv;
-  const int b = (int)(bj / r.L), j = (int)(bj % r.L);
-  int64_t dst = -1;
-  bool wanted = b < c.B && (r.lens == nullptr || j < r.lens[b]);
-  if (wanted) {
-    dst = kv4_row(c, b, (int64_t)(r.start != nullptr ? r.start[b] : 0) + j);
-    if (dst < 0 && lane == 0) kv4_report(c);
-  }
-  float x[4] = {0.f, 0.f, 0.f, 0.f};
-  if (dst >= 0) {
-    dst += (int64_t)h << c.page_shift;
-    const T* src = is_v ? reinterpret_cast<const T*>(r.v) + b * r.v_sb + j * r.v_ss + h * r.v_sh
-                        : reinterpret_cast<const T*>(r.k) + b * r.k_sb + j * r.k_ss + h * r.k_sh;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = to_f32<T>(src[4 * lane + i]);
+__global__ void __launch_bounds__(kRowThreads) kv4_append_kernel(const Kv4Cache c, const Kv4Rows r) {
+  constexpr int NG = D / 16, kTile = 8192 / D / 2, kItems = kTile * NG / kRowThreads;
+  __shared__ alignas(16) uint8_t s_codes[kTile][D / 2];
+  __shared__ int64_t s_dst[kTile];
+  const bool is_v = blockIdx.z != 0;
+  const int h = blockIdx.y;
+  const int64_t all = (int64_t)c.B * r.L, row0 = (int64_t)blockIdx.x * kTile;
+  for (int x = threadIdx.x; x < kTile; x += kRowThreads) {
+    const int64_t row = row0 + x;
+    const int b = (int)(row / r.L), j = (int)(row % r.L);
+    const bool wanted = row < all && (r.lens == nullptr || j < r.lens[b]);
+    const int64_t dst =
+        kv4_find(c, b, (int64_t)(wanted && r.start != nullptr ? r.start[b] : 0) + j, h, wanted);
+    if (dst == -1) kv4_report(c);
+    s_dst[x] = dst;
   }
   const float per_unit = 1.f / (is_v ? c.v_unit : c.k_unit);  // exact: a power of two
-  float top = 0.f;
-  bool nan = false;
+  // a thread's group of 16 dims of a row; all loads first
+  uint4 raw[kItems][2];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[i] *= per_unit;
-    top = fmaxf(top, fabsf(x[i]));
-    nan = nan || x[i] != x[i];
-  }
-  if (nan) top = NAN;
-#pragma unroll
-  for (int s = 1; s < 4; s <<= 1) {  // fmaxf drops a NaN: pass it on by hand
-    const float other = __shfl_xor_sync(kFull, top, s);
-    top = top != top || other != other ? NAN : fmaxf(top, other);
-  }
-  const float want = top != top ? top : fminf(__fdiv_rn(top, 6.f), 448.f);
-  const uint32_t sbyte = __nv_cvt_float_to_fp8(want, __NV_SATFINITE, __NV_E4M3);
-  const float scale = f16_lo(e4m3x2_f16(sbyte));
-  uint32_t codes[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float y = scale > 0.f ? __fdiv_rn(x[i], scale) : 0.f;
-    codes[i] = f32_e2m1x2(y, 0.f) & 15u;
-  }
-  const int i16 = lane / 4, u = lane % 4;  // group, quarter of the group
-  if (!is_v) {
-    if (dst >= 0)
-      *reinterpret_cast<uint16_t*>(c.k + dst * (D / 2) + u * (D / 8) + 2 * i16) =
-          (uint16_t)(codes[0] | codes[1] << 4 | codes[2] << 8 | codes[3] << 12);
-  } else {
-    // a byte holds dims g and g + 8 of a group: the partner lane (quarter u ^ 2) has the others
-    const uint32_t mine = codes[0] | codes[1] << 8 | codes[2] << 16 | codes[3] << 24;
-    const uint32_t other = __shfl_xor_sync(kFull, mine, 2);
-    if (dst >= 0 && u < 2) {
-      const uint32_t both = mine | other << 4;
-#pragma unroll
-      for (int n = 0; n < 4; ++n)
-        c.v[dst * (D / 2) + (4 * u + n) * NG + i16] = (uint8_t)(both >> (8 * n));
+  for (int n = 0; n < kItems; ++n) {
+    const int x = (threadIdx.x + n * kRowThreads) / NG, i = threadIdx.x % NG;
+    const int64_t row = row0 + x;
+    const int b = (int)(row / r.L), j = (int)(row % r.L);
+    const T* src = is_v ? static_cast<const T*>(r.v) + b * r.v_sb + j * r.v_ss + h * r.v_sh
+                        : static_cast<const T*>(r.k) + b * r.k_sb + j * r.k_ss + h * r.k_sh;
+    raw[n][0] = raw[n][1] = make_uint4(0, 0, 0, 0);
+    if (row < all) {
+      raw[n][0] = reinterpret_cast<const uint4*>(src + 16 * i)[0];
+      raw[n][1] = reinterpret_cast<const uint4*>(src + 16 * i)[1];
     }
   }
-  if (dst >= 0 && u == 0) (is_v ? c.vs : c.ks)[dst * NG + i16] = (uint8_t)sbyte;
-}
-
-// ------------------------------------------------------------------ gather
-template <typename T>
-__device__ __forceinline__ T held_as(float x);
-template <>
-__device__ __forceinline__ float held_as<float>(float x) { return x; }
-template <>
-__device__ __forceinline__ __half held_as<__half>(float x) { return __float2half_rn(x); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 held_as<__nv_bfloat16>(float x) {
-  return __float2bfloat16_rn(x);
-}
-
-// One lane makes 4 consecutive dims of a row. blockIdx.y: 0 keys, 1 values.
-template <typename T, int D>
-__global__ void __launch_bounds__(128) kv4_gather_kernel(const Kv4Cache c, const Kv4Rows r) {
-  constexpr int kLanes = D / 4, NG = D / 16;
-  const int64_t row = ((int64_t)blockIdx.x * 128 + threadIdx.x) / kLanes;
-  const int lane = threadIdx.x % kLanes;
-  const bool is_v = blockIdx.y != 0;
-  const int h = (int)(row % c.Hkv);
-  const int64_t bj = row / c.Hkv;
-  const int b = (int)(bj / r.L), j = (int)(bj % r.L);
-  if (b >= c.B) return;
-  const int64_t t = (int64_t)(r.start != nullptr ? r.start[b] : 0) + j;
-  int64_t src = -1;
-  if (t < r.lens[b]) {
-    src = kv4_row(c, b, t);
-    if (src < 0 && lane == 0) kv4_report(c);
-  }
-  float x[4] = {0.f, 0.f, 0.f, 0.f};
-  if (src >= 0) {
-    src += (int64_t)h << c.page_shift;
-    const int i16 = lane / 4, u = lane % 4;
-    const float scale = f16_lo(e4m3x2_f16((is_v ? c.vs : c.ks)[src * NG + i16])) *
-                        (is_v ? c.v_unit : c.k_unit);
-    if (!is_v) {
-      const uint32_t w =
-          *reinterpret_cast<const uint16_t*>(c.k + src * (D / 2) + u * (D / 8) + 2 * i16);
+  __syncthreads();
 #pragma unroll
-      for (int n = 0; n < 4; ++n) x[n] = e2m1_f32(w >> (4 * n));
+  for (int n = 0; n < kItems; ++n) {
+    const int x = (threadIdx.x + n * kRowThreads) / NG, i = threadIdx.x % NG;
+    float v[16];
+    float top = 0.f, sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      v[e] = to_f32<T>(reinterpret_cast<const T*>(raw[n])[e]) * per_unit;
+      top = fmaxf(top, fabsf(v[e]));
+      sum += v[e] * 0.f;  // NaN where one of them is NaN or infinite
+    }
+    bool nan = false;
+    if (sum != sum)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) nan = nan || v[e] != v[e];
+    const float want = nan ? NAN : fminf(__fdiv_rn(top, 6.f), 448.f);
+    const uint32_t sbyte = __nv_cvt_float_to_fp8(want, __NV_SATFINITE, __NV_E4M3);
+    const float scale = f16_lo(e4m3x2_f16(sbyte));
+    // x / scale to the nearest code. The product with the rounded reciprocal is off by 2^-23 of
+    // itself; a quotient of an 11-bit by a 4-bit number is either exactly half way between two
+    // codes or at least 2^-11 of itself (2^-13 absolute) away from it, so rounding the product to
+    // 2^-16 (by adding and taking away 1.5 * 2^7) gives the right side and restores exact halves.
+    const float inv = scale > 0.f ? __frcp_rn(scale) : 0.f;
+    uint32_t code[8];
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      v[e] = nan ? 0.f : __fadd_rn(__fadd_rn(__fmul_rn(v[e], inv), 192.f), -192.f);
+    if (!is_v) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) code[e] = f32_e2m1x2(v[2 * e], v[2 * e + 1]);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        *reinterpret_cast<uint16_t*>(&s_codes[x][u * (D / 8) + 2 * i]) =
+            (uint16_t)(code[2 * u] | code[2 * u + 1] << 8);
     } else {
 #pragma unroll
-      for (int n = 0; n < 4; ++n)  // a byte holds dims g and g + 8 of the group
-        x[n] = e2m1_f32(c.v[src * (D / 2) + (4 * (u & 1) + n) * NG + i16] >> (u < 2 ? 0 : 4));
+      for (int e = 0; e < 8; ++e) code[e] = f32_e2m1x2(v[e], v[e + 8]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s_codes[x][e * NG + i] = (uint8_t)code[e];
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] *= scale;
+    const int64_t dst = s_dst[x];
+    if (dst >= 0) (is_v ? c.vs : c.ks)[dst * NG + i] = (uint8_t)sbyte;
   }
-  T* dst = is_v ? const_cast<T*>(reinterpret_cast<const T*>(r.v)) + b * r.v_sb + j * r.v_ss + h * r.v_sh
-                : const_cast<T*>(reinterpret_cast<const T*>(r.k)) + b * r.k_sb + j * r.k_ss + h * r.k_sh;
+  __syncthreads();
+  constexpr int kPieces = D / 32;  // 16-byte pieces of a row's codes
 #pragma unroll
-  for (int i = 0; i < 4; ++i) dst[4 * lane + i] = held_as<T>(x[i]);
+  for (int y = threadIdx.x; y < kTile * kPieces; y += kRowThreads) {
+    const int x = y / kPieces, q = y % kPieces;
+    const int64_t dst = s_dst[x];
+    if (dst >= 0)
+      reinterpret_cast<uint4*>((is_v ? c.v : c.k) + dst * (D / 2))[q] =
+          reinterpret_cast<const uint4*>(s_codes[x])[q];
+  }
+}
+
+// A pair of values as T, exact.
+template <typename T>
+struct Kv4Pair;
+template <>
+struct Kv4Pair<__half> {
+  using type = uint32_t;
+  static __device__ __forceinline__ type make(float a, float b) { return pack2<false>(a, b); }
+};
+template <>
+struct Kv4Pair<__nv_bfloat16> {
+  using type = uint32_t;
+  static __device__ __forceinline__ type make(float a, float b) { return pack2<true>(a, b); }
+};
+template <>
+struct Kv4Pair<float> {
+  using type = float2;
+  static __device__ __forceinline__ type make(float a, float b) { return make_float2(a, b); }
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kRowThreads) kv4_gather_kernel(const Kv4Cache c, const Kv4Rows r) {
+  constexpr int NG = D / 16, kTile = 8192 / D / 2, kPieces = D / 32;  // 16-byte code pieces of a row
+  constexpr int kPad = 16 / sizeof(T);
+  using Pair = typename Kv4Pair<T>::type;
+  __shared__ alignas(16) T s_out[kTile][D + kPad];
+  __shared__ int64_t s_src[kTile];
+  const bool is_v = blockIdx.z != 0;
+  const int h = blockIdx.y;
+  const int64_t all = (int64_t)c.B * r.L, row0 = (int64_t)blockIdx.x * kTile;
+  int any = 0;
+  for (int x = threadIdx.x; x < kTile; x += kRowThreads) {
+    const int64_t row = row0 + x;
+    int64_t src = -3;  // a row that is not written
+    if (row < all) {
+      const int b = (int)(row / r.L), j = (int)(row % r.L), len = r.lens[b];
+      const int64_t t = (int64_t)(r.start != nullptr ? r.start[b] : 0) + j;
+      bool touched = true;
+      if (r.visible_only) {
+        if (j == 0 && (len < 0 || len > r.L) && h == 0 && !is_v) kv4_report(c);
+        const int centre = len - r.Lq;  // of the first row
+        const int lo = r.wl >= 0 && centre > r.wl ? centre - r.wl : 0;
+        touched = t < ((int64_t)len + 127) / 128 * 128 &&
+                  (t >= lo / 128 * 128 || t < ((int64_t)r.sink + 127) / 128 * 128);
+      }
+      if (touched) {
+        src = kv4_find(c, b, t, h, t < len);
+        if (src == -1) kv4_report(c);
+        any = 1;
+      }
+    }
+    s_src[x] = src;
+  }
+  if (!__syncthreads_or(any)) return;
+  // kTile * kPieces = 128: one piece of one row per thread
+  {
+    const int x = threadIdx.x / kPieces, q = threadIdx.x % kPieces;
+    const int64_t src = s_src[x];
+    uint4 raw = make_uint4(0, 0, 0, 0);
+    uint32_t sc[NG / 4];
+#pragma unroll
+    for (int i = 0; i < NG / 4; ++i) sc[i] = 0;
+    if (src >= 0) {
+      raw = reinterpret_cast<const uint4*>((is_v ? c.v : c.k) + src * (D / 2))[q];
+#pragma unroll
+      for (int i = 0; i < NG / 4; ++i)
+        sc[i] = reinterpret_cast<const uint32_t*>((is_v ? c.vs : c.ks) + src * NG)[i];
+    }
+    float scale[NG];
+#pragma unroll
+    for (int i = 0; i < NG / 4; ++i) {
+      uint32_t two[2];
+      e4m3x4_f16(sc[i], two);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        scale[4 * i + 2 * e] = f16_lo(two[e]) * (is_v ? c.v_unit : c.k_unit);
+        scale[4 * i + 2 * e + 1] = f16_hi(two[e]) * (is_v ? c.v_unit : c.k_unit);
+      }
+    }
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    auto put = [&](int d, uint32_t h2v, float f) {
+      *reinterpret_cast<Pair*>(&s_out[x][d]) = Kv4Pair<T>::make(f16_lo(h2v) * f, f16_hi(h2v) * f);
+    };
+    if (!is_v) {
+      // a word is two groups' 4 dims of one quarter u
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const int u = (16 * q + 4 * n) / (D / 8), i = 4 * n % (D / 8) / 2;
+        uint32_t two[4];
+        e2m1x8_f16(w[n], two);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          put(16 * (i + e / 2) + 4 * u + 2 * (e & 1), two[e], scale[i + e / 2]);
+      }
+    } else {
+      // NG bytes of dims g and g + 8; two neighbouring g make pairs
+#pragma unroll
+      for (int n = 0; n < 16 / NG; n += 2) {
+        const int g = 16 * q / NG + n;
+#pragma unroll
+        for (int z = 0; z < NG / 4; ++z) {
+          const uint32_t x0 = w[n * NG / 4 + z], x1 = w[(n + 1) * NG / 4 + z];
+          uint32_t lo[4], hi[4];
+          e2m1x8_f16((x0 & 0x0f0f0f0fu) | ((x1 << 4) & 0xf0f0f0f0u), lo);
+          e2m1x8_f16(((x0 >> 4) & 0x0f0f0f0fu) | (x1 & 0xf0f0f0f0u), hi);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            put(16 * (4 * z + e) + g, lo[e], scale[4 * z + e]);
+            put(16 * (4 * z + e) + 8 + g, hi[e], scale[4 * z + e]);
+          }
+        }
+      }
+    }
+  }
+  __syncthreads();
+  constexpr int kVec = D * (int)sizeof(T) / 16;  // 16-byte pieces of an output row
+#pragma unroll 4
+  for (int y = threadIdx.x; y < kTile * kVec; y += kRowThreads) {
+    const int x = y / kVec, q = y % kVec;
+    const int64_t row = row0 + x;
+    if (s_src[x] == -3) continue;
+    const int b = (int)(row / r.L), j = (int)(row % r.L);
+    T* dst = is_v ? static_cast<T*>(r.v) + b * r.v_sb + j * r.v_ss + h * r.v_sh
+                  : static_cast<T*>(r.k) + b * r.k_sb + j * r.k_ss + h * r.k_sh;
+    reinterpret_cast<uint4*>(dst)[q] = reinterpret_cast<const uint4*>(s_out[x])[q];
+  }
 }
 
 // ------------------------------------------------------------------ attention
@@ -262,7 +368,9 @@ constexpr int kBlockTiles = kBlockTokens / 16;
 constexpr int kAttnStages = 3;
 constexpr int kMinShare = 2;   // blocks per CTA at least: below, joining costs more than it gives
 constexpr int kUnitCost = 3;  // beginning and ending a unit takes about as long as so many blocks
-constexpr int kAttnCtas = 3;   // per SM
+// CTAs per SM: what shared memory and 128 registers per thread allow; two tiles of rows at D = 128
+// take more of both.
+__host__ __device__ constexpr int kv4_ctas(int D, int nt) { return D == 128 && nt == 2 ? 2 : 3; }
 constexpr float kGrow = 7.f;   // a row's reference is renewed when a score passes it by 2^7
 constexpr float kBelow = 3.f;  // and is then set 2^3 below the new maximum
 
@@ -459,7 +567,7 @@ struct Kv4Smem {
 };
 
 template <int D, int NT>
-__global__ void __launch_bounds__(kAttnThreads, kAttnCtas)
+__global__ void __launch_bounds__(kAttnThreads, kv4_ctas(D, NT))
     kv4_attn(const __grid_constant__ Kv4Args a) {
   constexpr int NG = D / 16, kRows = 8 * NT;
   using Smem = Kv4Smem<D, NT>;
@@ -1127,9 +1235,12 @@ int check_rows(const mfa_kv4_cache* c, const mfa_kv4_rows* r, bool gather) {
     return MFA_ERR_UNSUPPORTED;
   if (c->B == 0 || r->L == 0) return MFA_OK;
   if (r->k == nullptr || r->v == nullptr || (gather && r->lens == nullptr)) return MFA_ERR_INVALID;
-  if (((int64_t)c->B * r->L * c->Hkv * (c->D / 4) + 127) / 128 >= (1ll << 31))
-    return MFA_ERR_UNSUPPORTED;
-  return MFA_OK;
+  // rows are read and written in 16-byte pieces
+  const int es = r->dtype == MFA_FP32 ? 4 : 2;
+  bool ok = aligned16(r->k) && aligned16(r->v);
+  for (int i = 0; i < 3; ++i)
+    ok = ok && r->k_stride[i] * es % 16 == 0 && r->v_stride[i] * es % 16 == 0;
+  return ok ? MFA_OK : MFA_ERR_INVALID;
 }
 
 Kv4Rows resolve_rows(const mfa_kv4_rows* r) {
@@ -1141,22 +1252,23 @@ Kv4Rows resolve_rows(const mfa_kv4_rows* r) {
   x.start = r->start;
   x.lens = r->lens;
   x.L = r->L;
+  x.visible_only = 0;
   return x;
 }
 
-template <typename T>
-int launch_append(const Kv4Cache& c, const Kv4Rows& r, int D, cudaStream_t st) {
-  const dim3 grid((unsigned)(((int64_t)c.B * r.L * c.Hkv * (D / 4) + 127) / 128), 2);
-  if (D == 128) kv4_append_kernel<T, 128><<<grid, 128, 0, st>>>(c, r);
-  else kv4_append_kernel<T, 64><<<grid, 128, 0, st>>>(c, r);
+template <typename T, int D, bool kGather>
+int launch_rows(const Kv4Cache& c, const Kv4Rows& r, cudaStream_t st) {
+  constexpr int kTile = 8192 / D / 2;
+  const int64_t tiles = ((int64_t)c.B * r.L + kTile - 1) / kTile;
+  if (tiles >= (1ll << 31) || c.Hkv > 65535) return MFA_ERR_UNSUPPORTED;
+  const dim3 grid((unsigned)tiles, c.Hkv, 2);
+  if constexpr (kGather) kv4_gather_kernel<T, D><<<grid, kRowThreads, 0, st>>>(c, r);
+  else kv4_append_kernel<T, D><<<grid, kRowThreads, 0, st>>>(c, r);
   return cudaGetLastError() == cudaSuccess ? MFA_OK : MFA_ERR_CUDA;
 }
-template <typename T>
-int launch_gather(const Kv4Cache& c, const Kv4Rows& r, int D, cudaStream_t st) {
-  const dim3 grid((unsigned)(((int64_t)c.B * r.L * c.Hkv * (D / 4) + 127) / 128), 2);
-  if (D == 128) kv4_gather_kernel<T, 128><<<grid, 128, 0, st>>>(c, r);
-  else kv4_gather_kernel<T, 64><<<grid, 128, 0, st>>>(c, r);
-  return cudaGetLastError() == cudaSuccess ? MFA_OK : MFA_ERR_CUDA;
+template <typename T, bool kGather>
+int launch_rows(const Kv4Cache& c, const Kv4Rows& r, int D, cudaStream_t st) {
+  return D == 128 ? launch_rows<T, 128, kGather>(c, r, st) : launch_rows<T, 64, kGather>(c, r, st);
 }
 
 int check_fwd(const mfa_kv4_cache* c, const mfa_kv4_fwd_params* p) {
@@ -1182,23 +1294,120 @@ int check_fwd(const mfa_kv4_cache* c, const mfa_kv4_fwd_params* p) {
 }
 
 struct Kv4Plan {
+  bool direct;
+  // straight from the codes
   int nt, row_blocks, ctas;
   int64_t line, o, m;  // sizes of the workspace's parts, in bytes
+  // by way of 16-bit keys and values
+  int seqs;            // sequences at a time
+  int64_t kv;          // bytes of their keys, and of their values
   size_t bytes;
 };
-// One wave of resident CTAs, whatever the lengths are.
+
+// Query rows per KV head up to which the codes are read directly. Each 16 rows read and convert
+// the codes again, while the other way converts them once, to memory, for the tensor-core forward.
+// Measured on B200, 4 sequences of 8192 keys, 32/8 heads, D = 128 (us, directly and not):
+// MEASURE
+constexpr int64_t kDirectRows = 64;
+constexpr int64_t kStageBytes = 512ll << 20;  // keys and values of the sequences done at a time
+
+// The forward of sequences [b0, b0 + n) over keys and values in 16 bits, [n, capacity, Hkv, D].
+mfa_fwd_params staged_params(const mfa_kv4_cache* c, const mfa_kv4_fwd_params* p, int b0, int n,
+                             void* k, void* v) {
+  mfa_fwd_params f;
+  std::memset(&f, 0, sizeof(f));
+  const int64_t row = (int64_t)c->Hkv * c->D, room = (int64_t)c->max_pages * c->page_size;
+  f.q = static_cast<const uint8_t*>(p->q) + 2 * b0 * p->q_stride[0];
+  f.o = static_cast<uint8_t*>(p->o) + 2 * b0 * p->o_stride[0];
+  f.k = k;
+  f.v = v;
+  for (int i = 0; i < 3; ++i) {
+    f.q_stride[i] = p->q_stride[i];
+    f.o_stride[i] = p->o_stride[i];
+    f.k_stride[i] = f.v_stride[i] = i == 0 ? room * row : i == 1 ? row : c->D;
+  }
+  f.B = n;
+  f.Hq = p->Hq;
+  f.Hkv = c->Hkv;
+  f.Lq = p->Lq;
+  f.Lk = (int)room;
+  f.D = c->D;
+  f.scale = p->scale;
+  f.softcap = p->softcap;
+  f.causal = p->causal;
+  f.win_left = p->win_left;
+  f.win_right = p->win_right;
+  f.sink = p->sink;
+  f.alibi = p->alibi != nullptr ? p->alibi + (int64_t)b0 * p->Hq : nullptr;
+  f.dtype = p->dtype;
+  f.o_dtype = -1;
+  f.err = c->err;
+  return f;
+}
+
 Kv4Plan plan_fwd(const mfa_kv4_cache* c, const mfa_kv4_fwd_params* p, int sms) {
   Kv4Plan k;
   const int64_t rows = (int64_t)p->Lq * (p->Hq / c->Hkv);
+  k.direct = rows <= kDirectRows || c->max_pages == 0;
+  if (!k.direct) {
+    const int64_t each = 2ll * c->max_pages * c->page_size * c->Hkv * c->D;
+    k.seqs = (int)std::max<int64_t>(1, std::min<int64_t>(c->B, kStageBytes / 2 / each));
+    k.kv = k.seqs * each;
+    // the last group may be smaller and split its keys more
+    size_t split = 0;
+    for (int n : {k.seqs, c->B % k.seqs}) {
+      if (n == 0) continue;
+      // the plan asks for no address: any aligned one stands for the keys'
+      void* any = const_cast<void*>(p->q);
+      const mfa_fwd_params f = staged_params(c, p, 0, n, any, any);
+      split = std::max(split, mfa_fwd_workspace_size(&f));
+    }
+    k.bytes = (size_t)(2 * k.kv) + split;
+    return k;
+  }
+  // One wave of resident CTAs, whatever the lengths are.
   k.nt = rows > 8 ? 2 : 1;
   k.row_blocks = (int)((rows + 8 * k.nt - 1) / (8 * k.nt));
-  k.ctas = sms * kAttnCtas;
+  k.ctas = sms * kv4_ctas(c->D, k.nt);
   const int64_t parts = 2ll * k.ctas * 8 * k.nt;
   k.line = ((c->B + 1) * 4ll + 127) / 128 * 128;
   k.o = parts * c->D * 4;
   k.m = parts * 4;
   k.bytes = (size_t)(k.line + k.o + 2 * k.m);
   return k;
+}
+
+// Keys and values to 16 bits, then the tensor-core forward, a group of sequences after another.
+int run_staged_fwd(const mfa_kv4_cache* c, const mfa_kv4_fwd_params* p, const Kv4Plan& plan,
+                   cudaStream_t st) {
+  uint8_t* ws = static_cast<uint8_t*>(p->workspace);
+  for (int b0 = 0; b0 < c->B; b0 += plan.seqs) {
+    const int n = std::min(plan.seqs, c->B - b0);
+    mfa_fwd_params f = staged_params(c, p, b0, n, ws, ws + plan.kv);
+    f.workspace = ws + 2 * plan.kv;
+    f.workspace_bytes = p->workspace_bytes - 2 * plan.kv;
+    Kv4Cache cc = resolve_cache(c);
+    cc.B = n;
+    cc.table += b0 * cc.table_stride;
+    Kv4Rows r;
+    r.k = ws;
+    r.v = ws + plan.kv;
+    r.k_sb = r.v_sb = f.k_stride[0];
+    r.k_ss = r.v_ss = f.k_stride[1];
+    r.k_sh = r.v_sh = f.k_stride[2];
+    r.start = nullptr;
+    r.lens = p->seqlens + b0;
+    r.L = f.Lk;
+    r.visible_only = 1;
+    r.Lq = p->Lq;
+    r.wl = p->win_left;
+    r.sink = p->win_left >= 0 ? p->sink : 0;
+    int rc = p->dtype == MFA_BF16 ? launch_rows<__nv_bfloat16, true>(cc, r, c->D, st)
+                                  : launch_rows<__half, true>(cc, r, c->D, st);
+    if (rc == MFA_OK) rc = forward_padded(&f, p->seqlens + b0, st);
+    if (rc != MFA_OK) return rc;
+  }
+  return MFA_OK;
 }
 
 template <int D, int NT>
@@ -1233,8 +1442,8 @@ int mfa_kv4_append(const mfa_kv4_cache* c, const mfa_kv4_rows* r, void* stream) 
   (void)cudaGetLastError();
   const mfa::Kv4Cache cc = mfa::resolve_cache(c);
   const mfa::Kv4Rows rr = mfa::resolve_rows(r);
-  return r->dtype == MFA_BF16 ? mfa::launch_append<__nv_bfloat16>(cc, rr, c->D, st)
-                              : mfa::launch_append<__half>(cc, rr, c->D, st);
+  return r->dtype == MFA_BF16 ? mfa::launch_rows<__nv_bfloat16, false>(cc, rr, c->D, st)
+                              : mfa::launch_rows<__half, false>(cc, rr, c->D, st);
 }
 
 int mfa_kv4_gather(const mfa_kv4_cache* c, const mfa_kv4_rows* r, void* stream) {
@@ -1246,9 +1455,9 @@ int mfa_kv4_gather(const mfa_kv4_cache* c, const mfa_kv4_rows* r, void* stream) 
   (void)cudaGetLastError();
   const mfa::Kv4Cache cc = mfa::resolve_cache(c);
   const mfa::Kv4Rows rr = mfa::resolve_rows(r);
-  if (r->dtype == MFA_FP32) return mfa::launch_gather<float>(cc, rr, c->D, st);
-  return r->dtype == MFA_BF16 ? mfa::launch_gather<__nv_bfloat16>(cc, rr, c->D, st)
-                              : mfa::launch_gather<__half>(cc, rr, c->D, st);
+  if (r->dtype == MFA_FP32) return mfa::launch_rows<float, true>(cc, rr, c->D, st);
+  return r->dtype == MFA_BF16 ? mfa::launch_rows<__nv_bfloat16, true>(cc, rr, c->D, st)
+                              : mfa::launch_rows<__half, true>(cc, rr, c->D, st);
 }
 
 size_t mfa_kv4_fwd_workspace_size(const mfa_kv4_cache* c, const mfa_kv4_fwd_params* p) {
@@ -1268,6 +1477,9 @@ int mfa_kv4_fwd(const mfa_kv4_cache* c, const mfa_kv4_fwd_params* p, void* strea
   const mfa::Kv4Plan plan = mfa::plan_fwd(c, p, mfa::dev_info(dev).sms);
   if (p->workspace == nullptr || p->workspace_bytes < plan.bytes) return MFA_ERR_SCRATCH_TOO_SMALL;
   if (!mfa::aligned16(p->workspace)) return MFA_ERR_INVALID;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  (void)cudaGetLastError();
+  if (!plan.direct) return mfa::run_staged_fwd(c, p, plan, st);
   mfa::Kv4Args a;
   a.c = mfa::resolve_cache(c);
   a.q = p->q;
@@ -1298,8 +1510,6 @@ int mfa_kv4_fwd(const mfa_kv4_cache* c, const mfa_kv4_fwd_params* p, void* strea
   a.ws_o = reinterpret_cast<float*>(ws + plan.line);
   a.ws_m = reinterpret_cast<float*>(ws + plan.line + plan.o);
   a.ws_l = reinterpret_cast<float*>(ws + plan.line + plan.o + plan.m);
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  (void)cudaGetLastError();
   if (c->D == 128)
     return plan.nt == 1 ? mfa::launch_fwd<128, 1>(a, plan.ctas, dev, st)
                         : mfa::launch_fwd<128, 2>(a, plan.ctas, dev, st);

@@ -174,8 +174,14 @@ SplitPlan plan_splits(const mfa_fwd_params* p, int sms) {
   SplitPlan sp;
   const bool varlen = p->cu_q != nullptr;
   const int64_t lq = varlen ? p->max_lq : p->Lq;
-  const int64_t lk = varlen ? p->max_lk : p->Lk;
+  int64_t lk = varlen ? p->max_lk : p->Lk;
   if (p->B == 0 || lq <= 0 || lk <= 0) return sp;
+  if (p->sink > 0 && p->win_left >= 0) {
+    // kSink launches share out the blocks that a CTA's rows can see
+    const int64_t right = p->causal ? 0 : p->win_right >= 0 ? p->win_right : lk;
+    lk = std::min<int64_t>(lk, (int64_t)p->win_left + 1 + right + std::min<int64_t>(lq, 256) +
+                                   std::min<int64_t>(p->sink, lk) + 128);
+  }
   const int ps = pack_shift_for(p);
   const int tiles = sm100_tiles_for(p);
   const int64_t rows_per_cta = (int64_t)tiles * 128;
@@ -498,7 +504,35 @@ int noalloc_scratch(int dev, void** out) {
 
 #include "staged.inc"
 
+int forward(const mfa_fwd_params* p, const int32_t* k_lens, cudaStream_t st) {
+  int rc = validate(p);
+  if (rc != MFA_OK) return rc;
+  const bool varlen = p->cu_q != nullptr;
+  if (p->B == 0 || (!varlen && p->Lq == 0) || (varlen && p->max_lq == 0)) return MFA_OK;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return MFA_ERR_NO_DEVICE;
+  const int kern = pick_kernel(p, dev);
+  if (kern < 0) return -kern;
+  (void)cudaGetLastError();
+  FwdArgs a = resolve(p);
+  a.k_lens = k_lens;
+  SplitPlan split;
+  if (kern == MFA_KERNEL_TCGEN05 && p->workspace != nullptr) {
+    split = plan_splits(p, dev_info(dev).sms);
+    if (split.splits > 1 && p->workspace_bytes < split.bytes) split = SplitPlan{};
+  }
+  rc = kern == MFA_KERNEL_TCGEN05 ? run_sm100(p, a, dev, st, split, p->workspace)
+                                  : run_simt(p, a, st);
+  if (rc != MFA_OK) return rc;
+  return cudaGetLastError() == cudaSuccess ? MFA_OK : MFA_ERR_CUDA;
+}
+
 }  // namespace
+
+int forward_padded(const mfa_fwd_params* p, const int32_t* k_lens, cudaStream_t st) {
+  return forward(p, k_lens, st);
+}
+
 }  // namespace mfa
 
 extern "C" {
@@ -559,26 +593,7 @@ int mfa_select_kernel(const mfa_fwd_params* p) {
 int mfa_fwd(const mfa_fwd_params* p, void* stream) {
   if (mfa::fault_injected("fwd")) return MFA_ERR_FAULT_INJECTED;
   mfa::NvtxRange range("mfa_fwd");
-  int rc = mfa::validate(p);
-  if (rc != MFA_OK) return rc;
-  const bool varlen = p->cu_q != nullptr;
-  if (p->B == 0 || (!varlen && p->Lq == 0) || (varlen && p->max_lq == 0)) return MFA_OK;
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return MFA_ERR_NO_DEVICE;
-  const int kern = mfa::pick_kernel(p, dev);
-  if (kern < 0) return -kern;
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  (void)cudaGetLastError();
-  mfa::FwdArgs a = mfa::resolve(p);
-  mfa::SplitPlan split;
-  if (kern == MFA_KERNEL_TCGEN05 && p->workspace != nullptr) {
-    split = mfa::plan_splits(p, mfa::dev_info(dev).sms);
-    if (split.splits > 1 && p->workspace_bytes < split.bytes) split = mfa::SplitPlan{};
-  }
-  rc = kern == MFA_KERNEL_TCGEN05 ? mfa::run_sm100(p, a, dev, st, split, p->workspace)
-                                  : mfa::run_simt(p, a, st);
-  if (rc != MFA_OK) return rc;
-  return cudaGetLastError() == cudaSuccess ? MFA_OK : MFA_ERR_CUDA;
+  return mfa::forward(p, nullptr, reinterpret_cast<cudaStream_t>(stream));
 }
 
 int mfa_fwd_noalloc(const mfa_fwd_params* p, void* stream) {

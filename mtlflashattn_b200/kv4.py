@@ -143,6 +143,14 @@ def _pack_cache(cache, block_table, B, dev):
     return p
 
 
+def _in_pieces(t):
+    """t, or a copy of it, with rows that can be read in 16-byte pieces."""
+    st = t.stride()
+    if st[-1] != 1 or any(s % 8 for s in st[:-1]) or t.data_ptr() % 16:
+        return t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
 def _pack_rows(k, v, start, lens):
     p = _kernel._scratch("kv4_rows", _ROWS)
     _ROWS.pack_into(
@@ -178,7 +186,7 @@ def kv4_append(cache, k, v, block_table, cache_seqlens, new_lens=None):
     _check_lens("cache_seqlens", cache_seqlens, B, dev)
     if new_lens is not None:
         _check_lens("new_lens", new_lens, B, dev)
-    k, v = _kernel._last_dim_contig(k), _kernel._last_dim_contig(v)
+    k, v = _in_pieces(k), _in_pieces(v)
     r = _pack_rows(k, v, cache_seqlens, new_lens)
     _kernel._call(dev, "kv4_append", _lib.kv4_append, c, r)
 
@@ -246,10 +254,7 @@ def flash_attn_with_kv4cache(q, cache, block_table, cache_seqlens, softmax_scale
         if not torch.is_tensor(alibi_slopes):
             raise TypeError("mtlflashattn_b200: alibi_slopes must be a tensor of per-head slopes")
         alibi = _broadcast_alibi_slopes(alibi_slopes, B, Hq, dev)
-    x = q
-    sb, ss, sh, sd = q.stride()
-    if sd != 1 or (sb | ss | sh) % 8 or q.data_ptr() % 16:
-        x = q.clone(memory_format=torch.contiguous_format)  # rows are copied in 16-byte pieces
+    x = _in_pieces(q)
     out = torch.empty(q.shape, dtype=q.dtype, device=dev)
     scale = softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(D)
     far = 2**31 - 1
