@@ -84,6 +84,12 @@ __device__ __forceinline__ float f16_hi(uint32_t h2) {
   return __high2float(*reinterpret_cast<const __half2*>(&h2));
 }
 
+// x / d for 0 <= x < 2^31, with shift = ceil(log2(d)) and mul = floor(2^32 (2^shift - d) / d) + 1
+// (divisor_of).
+__device__ __forceinline__ int kv4_div(int x, uint32_t mul, uint32_t shift) {
+  return (int)((__umulhi((uint32_t)x, mul) + (uint32_t)x) >> shift);
+}
+
 // ------------------------------------------------------------------ append and gather
 // Both are bound by memory: 16-bit rows on one side, 0.28 of their bytes on the other. A CTA takes
 // a tile of 4096 codes of one head (32 rows of D = 128, 64 of D = 64), keys or values, through
@@ -94,6 +100,7 @@ struct Kv4Rows {
   int64_t k_sb, k_ss, k_sh, v_sb, v_ss, v_sh;
   const int *start, *lens;
   int L;
+  uint32_t L_mul, L_shift;  // row / L, as kv4_div
   // gather for the 16-bit forward: 1 = only the tokens that its blocks of 128 keys can touch, and
   // zeros up to the end of a sequence's last block
   int visible_only, Lq, wl, sink;
@@ -107,6 +114,21 @@ __device__ __forceinline__ int64_t kv4_find(const Kv4Cache& c, int b, int64_t t,
   return row < 0 ? -1 : row + ((int64_t)h << c.page_shift);
 }
 
+template <typename T>
+struct Kv4Two;
+template <>
+struct Kv4Two<__half> {
+  using type = __half2;
+  static __device__ __forceinline__ float lo(type x) { return __low2float(x); }
+  static __device__ __forceinline__ float hi(type x) { return __high2float(x); }
+};
+template <>
+struct Kv4Two<__nv_bfloat16> {
+  using type = __nv_bfloat162;
+  static __device__ __forceinline__ float lo(type x) { return __low2float(x); }
+  static __device__ __forceinline__ float hi(type x) { return __high2float(x); }
+};
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kRowThreads) kv4_append_kernel(const Kv4Cache c, const Kv4Rows r) {
   constexpr int NG = D / 16, kTile = 8192 / D / 2, kItems = kTile * NG / kRowThreads;
@@ -114,24 +136,13 @@ __global__ void __launch_bounds__(kRowThreads) kv4_append_kernel(const Kv4Cache 
   __shared__ int64_t s_dst[kTile];
   const bool is_v = blockIdx.z != 0;
   const int h = blockIdx.y;
-  const int64_t all = (int64_t)c.B * r.L, row0 = (int64_t)blockIdx.x * kTile;
-  for (int x = threadIdx.x; x < kTile; x += kRowThreads) {
-    const int64_t row = row0 + x;
-    const int b = (int)(row / r.L), j = (int)(row % r.L);
-    const bool wanted = row < all && (r.lens == nullptr || j < r.lens[b]);
-    const int64_t dst =
-        kv4_find(c, b, (int64_t)(wanted && r.start != nullptr ? r.start[b] : 0) + j, h, wanted);
-    if (dst == -1) kv4_report(c);
-    s_dst[x] = dst;
-  }
-  const float per_unit = 1.f / (is_v ? c.v_unit : c.k_unit);  // exact: a power of two
-  // a thread's group of 16 dims of a row; all loads first
+  const int all = c.B * r.L, row0 = blockIdx.x * kTile;
+  // a thread's groups of 16 dims of a row; all loads first
   uint4 raw[kItems][2];
 #pragma unroll
   for (int n = 0; n < kItems; ++n) {
     const int x = (threadIdx.x + n * kRowThreads) / NG, i = threadIdx.x % NG;
-    const int64_t row = row0 + x;
-    const int b = (int)(row / r.L), j = (int)(row % r.L);
+    const int row = row0 + x, b = kv4_div(row, r.L_mul, r.L_shift), j = row - b * r.L;
     const T* src = is_v ? static_cast<const T*>(r.v) + b * r.v_sb + j * r.v_ss + h * r.v_sh
                         : static_cast<const T*>(r.k) + b * r.k_sb + j * r.k_ss + h * r.k_sh;
     raw[n][0] = raw[n][1] = make_uint4(0, 0, 0, 0);
@@ -140,34 +151,47 @@ __global__ void __launch_bounds__(kRowThreads) kv4_append_kernel(const Kv4Cache 
       raw[n][1] = reinterpret_cast<const uint4*>(src + 16 * i)[1];
     }
   }
+  for (int x = threadIdx.x; x < kTile; x += kRowThreads) {
+    const int row = row0 + x, b = kv4_div(row, r.L_mul, r.L_shift), j = row - b * r.L;
+    const bool wanted = row < all && (r.lens == nullptr || j < r.lens[b]);
+    const int64_t dst =
+        kv4_find(c, b, (int64_t)(wanted && r.start != nullptr ? r.start[b] : 0) + j, h, wanted);
+    if (dst == -1) kv4_report(c);
+    s_dst[x] = dst;
+  }
+  const float per_unit = 1.f / (is_v ? c.v_unit : c.k_unit);  // exact: a power of two
   __syncthreads();
 #pragma unroll
   for (int n = 0; n < kItems; ++n) {
     const int x = (threadIdx.x + n * kRowThreads) / NG, i = threadIdx.x % NG;
-    float v[16];
-    float top = 0.f, sum = 0.f;
+    const uint32_t w[8] = {raw[n][0].x, raw[n][0].y, raw[n][0].z, raw[n][0].w,
+                           raw[n][1].x, raw[n][1].y, raw[n][1].z, raw[n][1].w};
+    // the largest size; a NaN wins
+    using T2 = typename Kv4Two<T>::type;
+    T2 top2 = __habs2(*reinterpret_cast<const T2*>(&w[0]));
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      v[e] = to_f32<T>(reinterpret_cast<const T*>(raw[n])[e]) * per_unit;
-      top = fmaxf(top, fabsf(v[e]));
-      sum += v[e] * 0.f;  // NaN where one of them is NaN or infinite
-    }
-    bool nan = false;
-    if (sum != sum)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) nan = nan || v[e] != v[e];
-    const float want = nan ? NAN : fminf(__fdiv_rn(top, 6.f), 448.f);
+    for (int e = 1; e < 8; ++e)
+      top2 = __hmax2_nan(top2, __habs2(*reinterpret_cast<const T2*>(&w[e])));
+    const float ta = Kv4Two<T>::lo(top2), tb = Kv4Two<T>::hi(top2);
+    const bool nan = ta != ta || tb != tb;
+    const float want = nan ? NAN : fminf(__fdiv_rn(fmaxf(ta, tb) * per_unit, 6.f), 448.f);
     const uint32_t sbyte = __nv_cvt_float_to_fp8(want, __NV_SATFINITE, __NV_E4M3);
     const float scale = f16_lo(e4m3x2_f16(sbyte));
-    // x / scale to the nearest code. The product with the rounded reciprocal is off by 2^-23 of
+    // x / scale to the nearest code. With the rounded reciprocal the quotient is off by 2^-24 of
     // itself; a quotient of an 11-bit by a 4-bit number is either exactly half way between two
-    // codes or at least 2^-11 of itself (2^-13 absolute) away from it, so rounding the product to
-    // 2^-16 (by adding and taking away 1.5 * 2^7) gives the right side and restores exact halves.
-    const float inv = scale > 0.f ? __frcp_rn(scale) : 0.f;
-    uint32_t code[8];
+    // codes or at least 2^-11 of itself (2^-13 absolute) away from it, so rounding it to 2^-16 (by
+    // adding and taking away 1.5 * 2^7) gives the right side and restores exact halves.
+    const float inv = scale > 0.f ? __frcp_rn(scale) * per_unit : 0.f;
+    float v[16];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      v[2 * e] = Kv4Two<T>::lo(*reinterpret_cast<const T2*>(&w[e]));
+      v[2 * e + 1] = Kv4Two<T>::hi(*reinterpret_cast<const T2*>(&w[e]));
+    }
 #pragma unroll
     for (int e = 0; e < 16; ++e)
-      v[e] = nan ? 0.f : __fadd_rn(__fadd_rn(__fmul_rn(v[e], inv), 192.f), -192.f);
+      v[e] = nan ? 0.f : __fadd_rn(__fmaf_rn(v[e], inv, 192.f), -192.f);
+    uint32_t code[8];
     if (!is_v) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) code[e] = f32_e2m1x2(v[2 * e], v[2 * e + 1]);
@@ -221,16 +245,16 @@ __global__ void __launch_bounds__(kRowThreads) kv4_gather_kernel(const Kv4Cache 
   constexpr int kPad = 16 / sizeof(T);
   using Pair = typename Kv4Pair<T>::type;
   __shared__ alignas(16) T s_out[kTile][D + kPad];
-  __shared__ int64_t s_src[kTile];
+  __shared__ int64_t s_src[kTile], s_dst[kTile];
   const bool is_v = blockIdx.z != 0;
   const int h = blockIdx.y;
-  const int64_t all = (int64_t)c.B * r.L, row0 = (int64_t)blockIdx.x * kTile;
+  const int all = c.B * r.L, row0 = blockIdx.x * kTile;
   int any = 0;
   for (int x = threadIdx.x; x < kTile; x += kRowThreads) {
-    const int64_t row = row0 + x;
+    const int row = row0 + x;
     int64_t src = -3;  // a row that is not written
     if (row < all) {
-      const int b = (int)(row / r.L), j = (int)(row % r.L), len = r.lens[b];
+      const int b = kv4_div(row, r.L_mul, r.L_shift), j = row - b * r.L, len = r.lens[b];
       const int64_t t = (int64_t)(r.start != nullptr ? r.start[b] : 0) + j;
       bool touched = true;
       if (r.visible_only) {
@@ -245,6 +269,7 @@ __global__ void __launch_bounds__(kRowThreads) kv4_gather_kernel(const Kv4Cache 
         if (src == -1) kv4_report(c);
         any = 1;
       }
+      s_dst[x] = is_v ? b * r.v_sb + j * r.v_ss + h * r.v_sh : b * r.k_sb + j * r.k_ss + h * r.k_sh;
     }
     s_src[x] = src;
   }
@@ -314,12 +339,8 @@ __global__ void __launch_bounds__(kRowThreads) kv4_gather_kernel(const Kv4Cache 
 #pragma unroll 4
   for (int y = threadIdx.x; y < kTile * kVec; y += kRowThreads) {
     const int x = y / kVec, q = y % kVec;
-    const int64_t row = row0 + x;
     if (s_src[x] == -3) continue;
-    const int b = (int)(row / r.L), j = (int)(row % r.L);
-    T* dst = is_v ? static_cast<T*>(r.v) + b * r.v_sb + j * r.v_ss + h * r.v_sh
-                  : static_cast<T*>(r.k) + b * r.k_sb + j * r.k_ss + h * r.k_sh;
-    reinterpret_cast<uint4*>(dst)[q] = reinterpret_cast<const uint4*>(s_out[x])[q];
+    reinterpret_cast<uint4*>(static_cast<T*>(is_v ? r.v : r.k) + s_dst[x])[q] = reinterpret_cast<const uint4*>(s_out[x])[q];
   }
 }
 
@@ -348,7 +369,7 @@ struct Kv4Args {
   int64_t q_sb, q_ss, q_sh, o_sb, o_ss, o_sh;
   const int* seqlens;
   int Lq, Hq, group, bf16;
-  uint32_t group_mul, group_shift;  // r / group = (umulhi(r, mul) + r) >> shift, r < 2^31
+  uint32_t group_mul, group_shift;  // row / group, as kv4_div
   float scale_l2;  // scale * k_unit * log2(e) (softcap: scale * k_unit / softcap)
   float softcap;
   int causal, wl, wr, sink;
@@ -375,7 +396,7 @@ constexpr float kGrow = 7.f;   // a row's reference is renewed when a score pass
 constexpr float kBelow = 3.f;  // and is then set 2^3 below the new maximum
 
 __device__ __forceinline__ int kv4_pos(const Kv4Args& a, int r) {  // r / group
-  return (int)((__umulhi((uint32_t)r, a.group_mul) + (uint32_t)r) >> a.group_shift);
+  return kv4_div(r, a.group_mul, a.group_shift);
 }
 
 struct Kv4Range {
@@ -1184,6 +1205,12 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join(const __grid_constant__
 }
 
 // ------------------------------------------------------------------ host
+void divisor_of(int d, uint32_t* mul, uint32_t* shift) {
+  *shift = 0;
+  while ((1ull << *shift) < (uint64_t)d) ++*shift;
+  *mul = (uint32_t)((((1ull << *shift) - d) << 32) / d + 1);
+}
+
 bool is_unit(float u) {
   int e = 0;
   return std::frexp(u, &e) == 0.5f && e >= -13 && e <= 5;  // 2^(e - 1)
@@ -1252,6 +1279,7 @@ Kv4Rows resolve_rows(const mfa_kv4_rows* r) {
   x.start = r->start;
   x.lens = r->lens;
   x.L = r->L;
+  divisor_of(x.L > 0 ? x.L : 1, &x.L_mul, &x.L_shift);
   x.visible_only = 0;
   return x;
 }
@@ -1260,7 +1288,7 @@ template <typename T, int D, bool kGather>
 int launch_rows(const Kv4Cache& c, const Kv4Rows& r, cudaStream_t st) {
   constexpr int kTile = 8192 / D / 2;
   const int64_t tiles = ((int64_t)c.B * r.L + kTile - 1) / kTile;
-  if (tiles >= (1ll << 31) || c.Hkv > 65535) return MFA_ERR_UNSUPPORTED;
+  if ((int64_t)c.B * r.L + kTile >= (1ll << 31) || c.Hkv > 65535) return MFA_ERR_UNSUPPORTED;
   const dim3 grid((unsigned)tiles, c.Hkv, 2);
   if constexpr (kGather) kv4_gather_kernel<T, D><<<grid, kRowThreads, 0, st>>>(c, r);
   else kv4_append_kernel<T, D><<<grid, kRowThreads, 0, st>>>(c, r);
@@ -1398,6 +1426,7 @@ int run_staged_fwd(const mfa_kv4_cache* c, const mfa_kv4_fwd_params* p, const Kv
     r.start = nullptr;
     r.lens = p->seqlens + b0;
     r.L = f.Lk;
+    divisor_of(r.L, &r.L_mul, &r.L_shift);
     r.visible_only = 1;
     r.Lq = p->Lq;
     r.wl = p->win_left;
@@ -1491,11 +1520,7 @@ int mfa_kv4_fwd(const mfa_kv4_cache* c, const mfa_kv4_fwd_params* p, void* strea
   a.Hq = p->Hq;
   a.group = p->Hq / c->Hkv;
   a.bf16 = p->dtype == MFA_BF16;
-  // multiplier of the exact division by the group: shift = ceil(log2(group)),
-  // mul = floor(2^32 (2^shift - group) / group) + 1
-  a.group_shift = 0;
-  while ((1u << a.group_shift) < (uint32_t)a.group) ++a.group_shift;
-  a.group_mul = (uint32_t)((((1ull << a.group_shift) - a.group) << 32) / a.group + 1);
+  mfa::divisor_of(a.group, &a.group_mul, &a.group_shift);
   a.softcap = p->softcap;
   a.scale_l2 = p->scale * c->k_unit *
                (p->softcap > 0.f ? 1.f / p->softcap : 1.4426950408889634f);

@@ -11,6 +11,7 @@
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
+#include <type_traits>
 #include <vector>
 
 #include "../../include/mfa.h"
@@ -189,8 +190,11 @@ SplitPlan plan_splits(const mfa_fwd_params* p, int sms) {
   const int64_t row_blocks = ((lq << ps) + rows_per_cta - 1) / rows_per_cta;
   const int64_t ctas = row_blocks * (p->Hq >> ps) * p->B;
   const int64_t key_blocks = (lk + 127) / 128;
+  // kSink: an even share of a short window is worth a CTA from 4 blocks on (4 x 1 x 16384, 64/8
+  // heads, window 4095: 31 us with 4 splits of 8 blocks, 28 with 8 of 4)
+  const int64_t least = p->sink > 0 && p->win_left >= 0 ? 4 : MFA_SPLIT_MIN_BLOCKS;
   int64_t s = (slots - slots / 8) / ctas;
-  s = s < key_blocks / MFA_SPLIT_MIN_BLOCKS ? s : key_blocks / MFA_SPLIT_MIN_BLOCKS;
+  s = s < key_blocks / least ? s : key_blocks / least;
   s = s < MFA_MAX_SPLITS ? s : MFA_MAX_SPLITS;
   if (s < 2) return sp;
   const int64_t blocks_per = (key_blocks + s - 1) / s;
@@ -354,26 +358,31 @@ int launch_combine(const FwdArgs& fin, const float* ws_o, const float* ws_lse, v
   const int64_t rows = (int64_t)fin.B * fin.Hq * fin.Lq;
   if (rows == 0) return MFA_OK;
   if (rows >= (1ll << 31)) return MFA_ERR_UNSUPPORTED;
+  // launches with first visible keys or padded key counts, and many rows: a warp per row (the other
+  // launches keep their order of summation)
+  const bool by_warp = (fin.sink > 0 || fin.k_lens != nullptr) && rows >= 2048;
   // a programmatic dependent launch: the merge grid is set up while the forward drains and
   // waits (griddepcontrol.wait) for its completion before reading the partials
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)rows);
+  cfg.gridDim = dim3((unsigned)(by_warp ? (rows + kCombineThreads / 32 - 1) / (kCombineThreads / 32)
+                                        : rows));
   cfg.blockDim = dim3(kCombineThreads);
-  cfg.dynamicSmemBytes = (size_t)fin.num_splits * sizeof(float);
+  cfg.dynamicSmemBytes = by_warp ? 0 : (size_t)fin.num_splits * sizeof(float);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaError_t e;
-  if (fin.o_dtype == MFA_FP32)
-    e = cudaLaunchKernelEx(&cfg, split_combine_kernel<float>, fin, ws_o, ws_lse, (float*)o, lse);
-  else if (fin.o_dtype == MFA_BF16)
-    e = cudaLaunchKernelEx(&cfg, split_combine_kernel<__nv_bfloat16>, fin, ws_o, ws_lse,
-                           (__nv_bfloat16*)o, lse);
-  else
-    e = cudaLaunchKernelEx(&cfg, split_combine_kernel<__half>, fin, ws_o, ws_lse, (__half*)o, lse);
+  auto go = [&](auto* out) {
+    using TO = std::remove_pointer_t<decltype(out)>;
+    return cudaLaunchKernelEx(
+        &cfg, by_warp ? split_combine_rows_kernel<TO> : split_combine_kernel<TO>, fin, ws_o, ws_lse,
+        out, lse);
+  };
+  const cudaError_t e = fin.o_dtype == MFA_FP32   ? go(static_cast<float*>(o))
+                        : fin.o_dtype == MFA_BF16 ? go(static_cast<__nv_bfloat16*>(o))
+                                                  : go(static_cast<__half*>(o));
   return e == cudaSuccess ? MFA_OK : MFA_ERR_CUDA;
 }
 
