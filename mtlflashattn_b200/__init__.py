@@ -173,7 +173,8 @@ def flash_attn_varlen_func(
         raise ValueError("mtlflashattn_b200: k/v total token count mismatch")
 
     cu_q = cu_seqlens_q.tolist()
-    cu_k = cu_seqlens_k.tolist()
+    # self-attention passes one tensor twice: each host read waits for the stream
+    cu_k = cu_q if cu_seqlens_k is cu_seqlens_q else cu_seqlens_k.tolist()
     if cu_q[-1] != q.shape[0]:
         raise ValueError(f"mtlflashattn_b200: cu_seqlens_q[-1]={cu_q[-1]} != total_q={q.shape[0]}")
     if cu_k[-1] != k.shape[0]:

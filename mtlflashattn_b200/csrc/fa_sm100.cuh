@@ -623,9 +623,44 @@ __global__ void __launch_bounds__(sm100::Roles<CG, TILES>::kThreads,
     const int tile_lo_max = key_range(a, sv, (r0 + t * BM + BM - 1) >> ps).lo;
     const int tile_hi_min = key_range(a, sv, (r0 + t * BM) >> ps).hi;
     const int tile_sk_min = kSink ? key_range(a, sv, (r0 + t * BM) >> ps).sk : 0;
-    auto masked = [&](int kl) {
-      if constexpr (kSink) return (kl < kr.lo && kl >= kr.sk) || kl >= kr.hi;
-      else return kl < kr.lo || kl >= kr.hi;
+    const int tile_sk_max = kSink ? key_range(a, sv, (r0 + t * BM + BM - 1) >> ps).sk : 0;
+    const int tile_lo_min = kSink ? key_range(a, sv, (r0 + t * BM) >> ps).lo : 0;
+    // Hides what the row does not see among x[0..NC), whose first key is c0. With kSink most blocks
+    // that need it need one comparison per score: past the window's end, before its start, or past
+    // the first keys; which one is the same for the tile's rows.
+    auto hide = [&](float* x, int c0, int kb0) {
+      if constexpr (kSink) {
+        const bool past = kb0 + KBN > tile_hi_min, before = kb0 < tile_lo_max;
+        if (!before) {
+          const int to = kr.hi - c0;
+#pragma unroll
+          for (int i = 0; i < NC; ++i) x[i] = i < to ? x[i] : -INFINITY;
+          return;
+        }
+        if (!past && kb0 >= tile_sk_max) {
+          const int from = kr.lo - c0;
+#pragma unroll
+          for (int i = 0; i < NC; ++i) x[i] = i >= from ? x[i] : -INFINITY;
+          return;
+        }
+        if (!past && kb0 + KBN <= tile_lo_min) {
+          const int to = kr.sk - c0;
+#pragma unroll
+          for (int i = 0; i < NC; ++i) x[i] = i < to ? x[i] : -INFINITY;
+          return;
+        }
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+          const int kl = c0 + i;
+          if ((kl < kr.lo && kl >= kr.sk) || kl >= kr.hi) x[i] = -INFINITY;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+          const int kl = c0 + i;
+          if (kl < kr.lo || kl >= kr.hi) x[i] = -INFINITY;
+        }
+      }
     };
     constexpr float kLog2e = 1.4426950408889634f;
     // x (the values kept in registers) times c is the logit in log2 units
@@ -690,13 +725,7 @@ __global__ void __launch_bounds__(sm100::Roles<CG, TILES>::kThreads,
           const uint64_t b2 = ffma2(sl2, f2pack((float)i, (float)(i + 1)), base2);
           f2unpack(ffma2(s2, sc2, b2), x[i], x[i + 1]);
         }
-        if (need_mask) {
-#pragma unroll
-          for (int i = 0; i < NC; ++i) {
-            const int kl = c0 + i;
-            if (masked(kl)) x[i] = -INFINITY;
-          }
-        }
+        if (need_mask) hide(x, c0, kb0);
       } else if constexpr (kGeneral) {
         // x = log2(e) * (softcap(s * scale) - slope * |centre - key|)
         const float d0 = centre - (float)(c0 + a.k_pos_offset);  // centre - key for i = 0
@@ -742,19 +771,17 @@ __global__ void __launch_bounds__(sm100::Roles<CG, TILES>::kThreads,
           }
           f2unpack(x2, x[i], x[i + 1]);
         }
-        if (need_mask) {
-#pragma unroll
-          for (int i = 0; i < NC; ++i) {
-            const int kl = c0 + i;
-            if (masked(kl)) x[i] = -INFINITY;
-          }
-        }
+        if (need_mask) hide(x, c0, kb0);
       } else {
-        if (need_mask) {
+        if constexpr (kSink) {
+#pragma unroll
+          for (int i = 0; i < NC; ++i) x[i] = __uint_as_float(r[i]);
+          if (need_mask) hide(x, c0, kb0);
+        } else if (need_mask) {
 #pragma unroll
           for (int i = 0; i < NC; ++i) {
             const int kl = c0 + i;
-            x[i] = masked(kl) ? -INFINITY : __uint_as_float(r[i]);
+            x[i] = (kl < kr.lo || kl >= kr.hi) ? -INFINITY : __uint_as_float(r[i]);
           }
         } else {
 #pragma unroll

@@ -126,6 +126,15 @@ int sm100_gen(const mfa_fwd_params* p) {
   return p->softcap > 0.f ? 2 : (!(p->scale > 0.f) || p->alibi != nullptr) ? 1 : 0;
 }
 int sm100_tiles_rt(bool wide, int gen);
+bool sm100_sink(const mfa_fwd_params* p) { return p->sink > 0 && p->win_left >= 0; }
+// First visible keys and a short window: one-tile CTAs also at D = 128. A 128-row tile walks a
+// block less than a 256-row pair, its blocks at the window's ends are masked while the other CTA of
+// the SM computes, and the shorter CTAs fill the last wave better; a long window would rather
+// fetch each K/V block once for two tiles. B200, 16 heads, L = 8192, one tile / two: window 128
+// 56 / 66 us, 1024 107 / 111, 4096 231 / 216.
+bool sm100_sink_one(const mfa_fwd_params* p) {
+  return sm100_sink(p) && p->win_left < 2048 && (p->causal || p->win_right >= 0);
+}
 
 // Query heads packed per KV head (log2; 0 = none). Decode-like launches (fewer than 128 query
 // rows per sequence) of a GQA/MQA model put the query heads of one KV group into the rows of one
@@ -154,7 +163,7 @@ bool sm100_short(const mfa_fwd_params* p) {
 }
 // Tiles per CTA of the tcgen05 kernel for these params.
 int sm100_tiles_for(const mfa_fwd_params* p) {
-  return sm100_short(p) ? 1 : sm100_tiles_rt(p->D > 64, sm100_gen(p));
+  return sm100_short(p) || sm100_sink_one(p) ? 1 : sm100_tiles_rt(p->D > 64, sm100_gen(p));
 }
 
 #ifndef MFA_MAX_SPLITS
@@ -177,7 +186,7 @@ SplitPlan plan_splits(const mfa_fwd_params* p, int sms) {
   const int64_t lq = varlen ? p->max_lq : p->Lq;
   int64_t lk = varlen ? p->max_lk : p->Lk;
   if (p->B == 0 || lq <= 0 || lk <= 0) return sp;
-  if (p->sink > 0 && p->win_left >= 0) {
+  if (sm100_sink(p)) {
     // kSink launches share out the blocks that a CTA's rows can see
     const int64_t right = p->causal ? 0 : p->win_right >= 0 ? p->win_right : lk;
     lk = std::min<int64_t>(lk, (int64_t)p->win_left + 1 + right + std::min<int64_t>(lq, 256) +
@@ -192,7 +201,7 @@ SplitPlan plan_splits(const mfa_fwd_params* p, int sms) {
   const int64_t key_blocks = (lk + 127) / 128;
   // kSink: an even share of a short window is worth a CTA from 4 blocks on (4 x 1 x 16384, 64/8
   // heads, window 4095: 31 us with 4 splits of 8 blocks, 28 with 8 of 4)
-  const int64_t least = p->sink > 0 && p->win_left >= 0 ? 4 : MFA_SPLIT_MIN_BLOCKS;
+  const int64_t least = sm100_sink(p) ? 4 : MFA_SPLIT_MIN_BLOCKS;
   int64_t s = (slots - slots / 8) / ctas;
   s = s < key_blocks / least ? s : key_blocks / least;
   s = s < MFA_MAX_SPLITS ? s : MFA_MAX_SPLITS;
@@ -405,7 +414,7 @@ int run_sm100(const mfa_fwd_params* p, FwdArgs a, int dev, cudaStream_t st,
   const int gen = sm100_gen(p);
   const bool wide = p->D > 64;
   const bool short_rows = sm100_short(p);
-  const int rows_per_cta = (short_rows ? 1 : sm100_tiles_rt(wide, gen)) * sm100::BM;
+  const int rows_per_cta = sm100_tiles_for(p) * sm100::BM;
   a.pack_shift = pack_shift_for(p);
   const int heads = p->Hq >> a.pack_shift;  // per batch: query heads, or KV heads when packed
   if (a.pack_shift > 0 &&
@@ -478,7 +487,8 @@ int run_sm100(const mfa_fwd_params* p, FwdArgs a, int dev, cudaStream_t st,
   if (grid >= (1ll << 31)) return MFA_ERR_UNSUPPORTED;
   const bool bf = p->dtype == MFA_BF16;
   rc = (a.sink > 0 ? launch_sm100_sink : launch_sm100_rt<false>)(args, dev, wide, bf, gen,
-                                                                 short_rows, grid, st);
+                                                                 short_rows, sm100_sink_one(p),
+                                                                 grid, st);
   if (rc != MFA_OK || split.splits < 2) return rc;
   return launch_combine(fin, ws_o, ws_lse, p->o, p->lse, st);
 }

@@ -8,8 +8,8 @@
 namespace mfa {
 
 int launch_sm100_sink(const Sm100Args& args, int dev, bool wide, bool bf16, int gen,
-                      bool short_rows, int64_t grid, cudaStream_t st) {
-  return launch_sm100_rt<true>(args, dev, wide, bf16, gen, short_rows, grid, st);
+                      bool short_rows, bool one, int64_t grid, cudaStream_t st) {
+  return launch_sm100_rt<true>(args, dev, wide, bf16, gen, short_rows, one, grid, st);
 }
 
 }  // namespace mfa
