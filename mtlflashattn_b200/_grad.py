@@ -18,7 +18,7 @@ class _NoBackward(torch.autograd.Function):
 
 def _guard_grad(out, *inputs):
     if torch.is_grad_enabled():
-        ts = [t for t in inputs if torch.is_tensor(t)]
-        if any(t.requires_grad for t in ts):
-            return _NoBackward.apply(out, *ts)
+        for t in inputs:
+            if torch.is_tensor(t) and t.requires_grad:
+                return _NoBackward.apply(out, *[x for x in inputs if torch.is_tensor(x)])
     return out

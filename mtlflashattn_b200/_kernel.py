@@ -265,16 +265,14 @@ def _scratch(name, fmt):
 def _call(dev, what, fn, *args):
     """Run ``fn(*args, stream)`` with ``dev`` current, on its current stream, and raise on a
     status that is not OK."""
-    ctx = torch.cuda.device(dev) if dev.index != torch.cuda.current_device() else None
-    if ctx is not None:
-        ctx.__enter__()
-    try:
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
-        if rc != _lib.OK:
-            _raise_status(rc, what)
-    finally:
-        if ctx is not None:
-            ctx.__exit__(None, None, None)
+    index = dev.index
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc != _lib.OK:
+        _raise_status(rc, what)
     if _sync_check_enabled():
         check_device_errors(dev)
 

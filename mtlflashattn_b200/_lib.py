@@ -264,6 +264,8 @@ class MfaError(RuntimeError):
 def load(path: str | None = None) -> ctypes.CDLL:
     """Load libmfa.so (once) and declare the C signatures. Raises if it is absent."""
     global _lib
+    if _lib is not None:  # set last, once everything below is done
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib

@@ -109,10 +109,10 @@ def kv4_cache(num_pages, page_size, num_heads_kv, head_dim, device=None, k_unit=
                     zeros(head_dim // 16).view(e4m3), k_unit, v_unit)
 
 
-def _check_lens(name, t, B, dev):
-    if t.dtype != _I32 or t.shape != (B,) or not t.is_contiguous():
+def _check_lens(name, t, B, index):
+    if t.dtype is not _I32 or t.shape != (B,) or not t.is_contiguous():
         raise ValueError(f"mtlflashattn_b200: {name} must be a contiguous int32 tensor of [{B}]")
-    if t.device != dev:
+    if t.get_device() != index:
         raise ValueError("mtlflashattn_b200: all tensors must be on the cache's device")
 
 
@@ -121,15 +121,17 @@ def _pack_cache(cache, block_table, B, dev):
     if not isinstance(cache, KV4Cache):
         raise TypeError("mtlflashattn_b200: cache must be a KV4Cache")
     k = cache.k
-    if not k.is_cuda:
+    index = k.get_device()
+    if index < 0:
         raise NotImplementedError(
             f"mtlflashattn_b200: device {k.device.type!r} not supported (CUDA only)")
-    if block_table.dtype != _I32 or block_table.dim() != 2 or block_table.shape[0] != B:
+    table = block_table.shape
+    if block_table.dtype is not _I32 or len(table) != 2 or table[0] != B:
         raise ValueError(f"mtlflashattn_b200: block_table must be int32 [{B}, max_pages]")
-    if k.device != dev or block_table.device != dev:
+    if dev.index != index or dev.type != "cuda" or block_table.get_device() != index:
         raise ValueError("mtlflashattn_b200: all tensors must be on the cache's device")
     pages, heads, size, half = k.shape
-    max_pages = block_table.shape[1]
+    max_pages = table[1]
     if max_pages * size >= 2**31:
         raise ValueError("mtlflashattn_b200: block_table covers 2^31 tokens or more")
     stride = block_table.stride()
@@ -145,8 +147,8 @@ def _pack_cache(cache, block_table, B, dev):
 
 def _in_pieces(t):
     """t, or a copy of it, with rows that can be read in 16-byte pieces."""
-    st = t.stride()
-    if st[-1] != 1 or any(s % 8 for s in st[:-1]) or t.data_ptr() % 16:
+    sb, ss, sh, sd = t.stride()
+    if sd != 1 or (sb | ss | sh) % 8 or t.data_ptr() % 16:
         return t.clone(memory_format=torch.contiguous_format)
     return t
 
@@ -183,9 +185,9 @@ def kv4_append(cache, k, v, block_table, cache_seqlens, new_lens=None):
         raise ValueError("mtlflashattn_b200: all tensors must be on the cache's device")
     if k.shape[2] != cache.num_heads_kv or k.shape[3] != cache.head_dim:
         raise ValueError("mtlflashattn_b200: k and v do not have the cache's heads and head_dim")
-    _check_lens("cache_seqlens", cache_seqlens, B, dev)
+    _check_lens("cache_seqlens", cache_seqlens, B, dev.index)
     if new_lens is not None:
-        _check_lens("new_lens", new_lens, B, dev)
+        _check_lens("new_lens", new_lens, B, dev.index)
     k, v = _in_pieces(k), _in_pieces(v)
     r = _pack_rows(k, v, cache_seqlens, new_lens)
     _kernel._call(dev, "kv4_append", _lib.kv4_append, c, r)
@@ -203,9 +205,9 @@ def kv4_gather(cache, block_table, cache_seqlens, max_seqlen, starts=None, dtype
         raise ValueError("mtlflashattn_b200: max_seqlen must be an int >= 0")
     B, dev = block_table.shape[0], block_table.device
     c = _pack_cache(cache, block_table, B, dev)
-    _check_lens("cache_seqlens", cache_seqlens, B, dev)
+    _check_lens("cache_seqlens", cache_seqlens, B, dev.index)
     if starts is not None:
-        _check_lens("starts", starts, B, dev)
+        _check_lens("starts", starts, B, dev.index)
     shape = (B, max_seqlen, cache.num_heads_kv, cache.head_dim)
     k = torch.empty(shape, dtype=dtype, device=dev)
     v = torch.empty(shape, dtype=dtype, device=dev)
@@ -248,7 +250,7 @@ def flash_attn_with_kv4cache(q, cache, block_table, cache_seqlens, softmax_scale
         raise ValueError("mtlflashattn_b200: q does not have the cache's head_dim")
     if Hq == 0 or Hq % Hkv != 0:
         raise ValueError(f"mtlflashattn_b200: num_heads_kv ({Hkv}) must divide num_heads_q ({Hq})")
-    _check_lens("cache_seqlens", cache_seqlens, B, dev)
+    _check_lens("cache_seqlens", cache_seqlens, B, dev.index)
     alibi = None
     if alibi_slopes is not None:
         if not torch.is_tensor(alibi_slopes):
