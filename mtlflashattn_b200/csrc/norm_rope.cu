@@ -2,13 +2,16 @@
 // (mfa_qk_norm_rope, include/mfa.h). For a head row x of D values, all in fp32:
 //   y = x / sqrt(mean(x^2) + eps) * w
 //   (a, b) -> (a cos - b sin, a sin + b cos) over the pairs (i, i + R/2) or (2i, 2i + 1), i < R/2
-// and one rounding to the tensor's type at the end. Built without fast math: the square root,
-// the division and the mean are IEEE fp32.
+// and one rounding to the tensor's type at the end. 1 / sqrt is the hardware's, off by 2^-22 at
+// most, the rest IEEE fp32 (built without fast math).
 #include <cuda_runtime.h>
+
+#include <type_traits>
 
 #include "../../include/mfa.h"
 #include "common.cuh"
 #include "host.cuh"
+#include "ptx.cuh"
 
 namespace mfa {
 namespace {
@@ -22,8 +25,9 @@ struct NormRopeArgs {
   const void* positions;
   int64_t pos_sb, pos_ss;
   int B, L, Hq, Hkv, D, R, max_pos, pos64, w_fp32, rot_fp32, interleaved;
+  int w_vec, rot_vec;  // weights and tables can be read 16 bytes at a time (vector kernel)
   int segments;  // warps that share one token's heads (vector kernel)
-  float eps;
+  float eps, inv_D;
   int* err;
 };
 
@@ -55,29 +59,49 @@ __device__ __forceinline__ float load_any(const void* p, int64_t i, int fp32) {
   return fp32 ? reinterpret_cast<const float*>(p)[i] : to_f32<T>(reinterpret_cast<const T*>(p)[i]);
 }
 
-// N consecutive values as fp32, from 16-byte aligned memory.
-template <typename T, int N>
-__device__ __forceinline__ void load_vec(const T* p, float* out) {
-  constexpr int kPer = 16 / (int)sizeof(T);
-  static_assert(N % kPer == 0, "whole 16-byte loads");
+// 8 consecutive values in 16-byte aligned memory, as they are and as fp32.
+template <typename T>
+struct Eight {
+  uint4 raw[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-  for (int c = 0; c < N / kPer; ++c) {
-    const uint4 raw = reinterpret_cast<const uint4*>(p)[c];
-    const T* e = reinterpret_cast<const T*>(&raw);
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) out[c * kPer + i] = to_f32<T>(e[i]);
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[i] = reinterpret_cast<const uint4*>(p)[i];
   }
-}
-template <typename T, int N>
-__device__ __forceinline__ void store_vec(T* p, const float* v) {
-  constexpr int kPer = 16 / (int)sizeof(T);
+  __device__ __forceinline__ void store(T* p) const {
 #pragma unroll
-  for (int c = 0; c < N / kPer; ++c) {
-    uint4 raw;
-    T* e = reinterpret_cast<T*>(&raw);
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = raw[i];
+  }
+  __device__ __forceinline__ void get(float* v) const {
+    const T* e = reinterpret_cast<const T*>(raw);
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) e[i] = from_f32<T>(v[c * kPer + i]);
-    reinterpret_cast<uint4*>(p)[c] = raw;
+    for (int i = 0; i < 8; ++i) v[i] = to_f32<T>(e[i]);
+  }
+  __device__ __forceinline__ void set(const float* v) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) reinterpret_cast<T*>(raw)[i] = v[i];
+    } else {
+      constexpr bool kBF16 = std::is_same_v<T, __nv_bfloat16>;
+      raw[0] = make_uint4(pack2<kBF16>(v[0], v[1]), pack2<kBF16>(v[2], v[3]),
+                          pack2<kBF16>(v[4], v[5]), pack2<kBF16>(v[6], v[7]));
+    }
+  }
+};
+
+// 8 consecutive values of a table or weight from index i on.
+template <typename T>
+__device__ __forceinline__ void load_eight(const void* p, int64_t i, int fp32, int vec, float* out) {
+  if (vec && fp32) {
+    Eight<float> e;
+    e.load(static_cast<const float*>(p) + i);
+    e.get(out);
+  } else if (vec) {
+    Eight<T> e;
+    e.load(static_cast<const T*>(p) + i);
+    e.get(out);
+  } else {
+#pragma unroll
+    for (int n = 0; n < 8; ++n) out[n] = load_any<T>(p, i + n, fp32);
   }
 }
 
@@ -111,7 +135,7 @@ __global__ void __launch_bounds__(128) norm_rope_any(const __grid_constant__ Nor
   }
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
-  const float inv = 1.f / sqrtf(sum / (float)a.D + a.eps);
+  const float inv = rsqrtf(fmaf(sum, a.inv_D, a.eps));
   auto y = [&](int d) {
     const float v = to_f32<T>(x[d]) * inv;
     return weight != nullptr ? v * load_any<T>(weight, d, a.w_fp32) : v;
@@ -135,21 +159,42 @@ __global__ void __launch_bounds__(128) norm_rope_any(const __grid_constant__ Nor
 // D % 16 == 0 and 16-byte aligned rows. A row is LP lanes (D / 16 of them at work), each with two
 // chunks of 8 values: with split halves the chunks p and p + R/16 that rotate with each other
 // (R % 16 == 0), interleaved any two (R % 8 == 0), so no value crosses lanes but the sum of
-// squares. A warp walks heads of one token and keeps its cosines, sines and weights in registers.
+// squares. A warp takes groups of heads of one token, first of q and then of k, and keeps the
+// token's cosines and sines in registers; the next group's rows are on their way while one is
+// worked on. Per value there are few bytes and many instructions: the arithmetic is in
+// packed pairs and the registers are kept at 80 for 16-bit rows (16384 tokens, 32/8 heads, D = 128,
+// bf16: 65 us, 5.3 TB/s; with scalar arithmetic 77; 64 registers: 82).
 template <typename T, bool kInterleaved, int LP>
-__global__ void __launch_bounds__(128) norm_rope_vec(const __grid_constant__ NormRopeArgs a) {
+__global__ void __launch_bounds__(128, sizeof(T) == 2 ? 6 : 5)
+    norm_rope_vec(const __grid_constant__ NormRopeArgs a) {
   constexpr int kRows = 32 / LP;  // heads a warp holds at once
-  const int64_t w = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+  const int w = (blockIdx.x * 128 + threadIdx.x) >> 5;
   const int lane = threadIdx.x & 31, sub = lane % LP;
-  const int64_t token = w / a.segments;
-  const int seg = (int)(w % a.segments);
-  if (token >= (int64_t)a.B * a.L) return;
-  const int b = (int)(token / a.L), l = (int)(token % a.L);
+  const int token = w / a.segments, seg = w - token * a.segments;
+  if (token >= a.B * a.L) return;
+  const int b = token / a.L, l = token - b * a.L;
   const bool active = sub < a.D / 16;
   const int pairs = kInterleaved ? 0 : a.R / 16;  // leading lanes whose chunks rotate together
   const int c0 = 8 * (kInterleaved || sub >= pairs ? 2 * sub : sub);
   const int c1 = kInterleaved || sub >= pairs ? c0 + 8 : c0 + a.R / 2;
   const bool rot0 = active && c0 < a.R, rot1 = active && c1 < a.R;
+  const int gq = (a.Hq + kRows - 1) / kRows, all = gq + (a.Hkv + kRows - 1) / kRows;
+  const int per = (all + a.segments - 1) / a.segments;
+  const int g_end = min(all, (seg + 1) * per);
+  const T* q = static_cast<const T*>(a.q) + b * a.q_sb + l * a.q_ss;
+  const T* k = static_cast<const T*>(a.k) + b * a.k_sb + l * a.k_ss;
+  T* qo = static_cast<T*>(a.q_out) + (int64_t)token * a.Hq * a.D;
+  T* ko = static_cast<T*>(a.k_out) + (int64_t)token * a.Hkv * a.D;
+  Eight<T> lo, hi;
+  auto fetch = [&](int g) {
+    const bool is_k = g >= gq;
+    const int h = (is_k ? g - gq : g) * kRows + lane / LP;
+    if (!active || g >= g_end || h >= (is_k ? a.Hkv : a.Hq)) return;
+    const T* src = is_k ? k + h * a.k_sh : q + h * a.q_sh;
+    lo.load(src + c0);
+    hi.load(src + c1);
+  };
+  fetch(seg * per);
   int64_t row = 0;
   const bool bad = a.R > 0 && (row = table_row(a, b, l)) < 0;
   float cs[8], sn[8];
@@ -159,63 +204,87 @@ __global__ void __launch_bounds__(128) norm_rope_vec(const __grid_constant__ Nor
     sn[i] = 0.f;
   }
   if (!bad) {
+    // the angles of the lane's 8 pairs stand side by side; interleaved, the last lane that
+    // rotates may have 4 of them
+    const int p = kInterleaved ? c0 / 2 : c0;
+    if (rot0 && (rot1 || !kInterleaved)) {
+      load_eight<T>(a.cos, row * a.cos_row + p, a.rot_fp32, a.rot_vec, cs);
+      load_eight<T>(a.sin, row * a.sin_row + p, a.rot_fp32, a.rot_vec, sn);
+    } else if (rot0) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const bool rot = kInterleaved ? (i < 4 ? rot0 : rot1) : rot0;
-      const int p = kInterleaved ? (i < 4 ? c0 : c1) / 2 + (i & 3) : c0 + i;
-      if (rot) {
-        cs[i] = load_any<T>(a.cos, row * a.cos_row + p, a.rot_fp32);
-        sn[i] = load_any<T>(a.sin, row * a.sin_row + p, a.rot_fp32);
+      for (int i = 0; i < 4; ++i) {
+        cs[i] = load_any<T>(a.cos, row * a.cos_row + p + i, a.rot_fp32);
+        sn[i] = load_any<T>(a.sin, row * a.sin_row + p + i, a.rot_fp32);
       }
     }
   } else if (lane == 0 && seg == 0 && a.err != nullptr) {
     atomicExch(a.err, MFA_ERR_INVALID);
   }
-  const int H = a.Hq + a.Hkv;
-  const int per = (H + a.segments * kRows - 1) / (a.segments * kRows) * kRows;
-  const int h_end = min(H, (seg + 1) * per);
-  float wt[16];
-  int wt_of = -1;  // whose weights wt holds: 0 the queries', 1 the keys'
-  for (int h0 = seg * per; h0 < h_end; h0 += kRows) {  // the warp's lanes stay together
-    const int hh = h0 + lane / LP;
-    const bool on = active && hh < h_end;
-    const int is_k = hh >= a.Hq;
-    const int h = is_k ? hh - a.Hq : hh;
-    float x[16];
-    float sum = 0.f;
-    if (on) {
-      const T* src = is_k ? reinterpret_cast<const T*>(a.k) + b * a.k_sb + l * a.k_ss + h * a.k_sh
-                          : reinterpret_cast<const T*>(a.q) + b * a.q_sb + l * a.q_ss + h * a.q_sh;
-      load_vec<T, 8>(src + c0, x);
-      load_vec<T, 8>(src + c1, x + 8);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) sum = fmaf(x[i], x[i], sum);
-    }
-#pragma unroll
-    for (int s = LP / 2; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
-    if (!on) continue;
-    if (wt_of != is_k) {
-      wt_of = is_k;
+  uint64_t wt[8];  // weights, in pairs
+  for (int g = seg * per; g < g_end; ++g) {
+    const bool is_k = g >= gq;
+    const int h = (is_k ? g - gq : g) * kRows + lane / LP;
+    const bool on = active && h < (is_k ? a.Hkv : a.Hq);
+    if (g == seg * per || g == gq) {  // whose weights change
       const void* weight = is_k ? a.k_weight : a.q_weight;
+      float v[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        wt[i] = weight != nullptr ? load_any<T>(weight, (i < 8 ? c0 : c1 - 8) + i, a.w_fp32) : 1.f;
+      for (int i = 0; i < 16; ++i) v[i] = 1.f;
+      if (weight != nullptr && active) {
+        load_eight<T>(weight, c0, a.w_fp32, a.w_vec, v);
+        load_eight<T>(weight, c1, a.w_fp32, a.w_vec, v + 8);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) wt[i] = f2pack(v[2 * i], v[2 * i + 1]);
     }
-    const float inv = 1.f / sqrtf(sum / (float)a.D + a.eps);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = bad ? 0.f : x[i] * inv * wt[i];
+    float v[16];
+    lo.get(v);
+    hi.get(v + 8);
+    fetch(g + 1);
+    uint64_t x[8], sum2 = f2pack(0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      float& u = x[kInterleaved ? 2 * i : i];
-      float& v = x[kInterleaved ? 2 * i + 1 : i + 8];
-      const float y0 = u * cs[i] - v * sn[i], y1 = u * sn[i] + v * cs[i];
-      u = y0;
-      v = y1;
+      x[i] = f2pack(v[2 * i], v[2 * i + 1]);
+      sum2 = ffma2(x[i], x[i], sum2);
     }
-    T* o = is_k ? reinterpret_cast<T*>(a.k_out) + (token * a.Hkv + h) * a.D
-                : reinterpret_cast<T*>(a.q_out) + (token * a.Hq + h) * a.D;
-    store_vec<T, 8>(o + c0, x);
-    store_vec<T, 8>(o + c1, x + 8);
+    float sum, odd;
+    f2unpack(sum2, sum, odd);
+    sum = on ? sum + odd : 0.f;
+#pragma unroll
+    for (int s = LP / 2; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+    const float inv = rsqrtf(fmaf(sum, a.inv_D, a.eps));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = fmul2(fmul2(x[i], f2pack(inv, inv)), wt[i]);
+    if (!kInterleaved) {  // pairs of pairs: (u0, u1) and (v0, v1) turn by two angles
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint64_t c = f2pack(cs[2 * i], cs[2 * i + 1]), s = f2pack(sn[2 * i], sn[2 * i + 1]);
+        const uint64_t u = x[i], t = x[i + 4];
+        x[i] = fsub2(fmul2(u, c), fmul2(t, s));
+        x[i + 4] = ffma2(u, s, fmul2(t, c));
+        f2unpack(x[i], v[2 * i], v[2 * i + 1]);
+        f2unpack(x[i + 4], v[8 + 2 * i], v[8 + 2 * i + 1]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float u, t;
+        f2unpack(x[i], u, t);
+        v[2 * i] = u * cs[i] - t * sn[i];
+        v[2 * i + 1] = u * sn[i] + t * cs[i];
+      }
+    }
+    if (bad)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = 0.f;
+    if (on) {
+      T* o = (is_k ? ko : qo) + h * a.D;
+      Eight<T> out;
+      out.set(v);
+      out.store(o + c0);
+      out.set(v + 8);
+      out.store(o + c1);
+    }
   }
 }
 
@@ -234,10 +303,10 @@ int launch_norm_rope(NormRopeArgs a, bool vec, cudaStream_t st) {
   const int rows = a.D > 64 ? 4 : a.D > 32 ? 8 : 16;  // heads a warp holds at once
   // few tokens: spread each one's heads over warps until every SM has 16
   a.segments = 1;
-  const int most = (H + rows - 1) / rows;
+  const int most = (a.Hq + rows - 1) / rows + (a.Hkv + rows - 1) / rows;
   while (a.segments < most && tokens * a.segments < 148 * 16) ++a.segments;
   const int64_t warps = vec ? tokens * a.segments : tokens * H;
-  if ((warps + 3) / 4 >= (1ll << 31)) return MFA_ERR_UNSUPPORTED;
+  if (warps >= (1ll << 31)) return MFA_ERR_UNSUPPORTED;
   if (!vec) norm_rope_any<T><<<(unsigned)((warps + 3) / 4), 128, 0, st>>>(a);
   else if (a.interleaved) launch_vec<T, true>(a, warps, st);
   else launch_vec<T, false>(a, warps, st);
@@ -280,12 +349,17 @@ extern "C" int mfa_qk_norm_rope(const mfa_norm_rope_params* p, void* stream) {
   a.interleaved = p->interleaved ? 1 : 0;
   a.segments = 1;
   a.eps = p->eps;
+  a.inv_D = 1.f / (float)p->D;
   a.err = p->err;
   const int es = p->dtype == MFA_FP32 ? 4 : 2;
   bool vec = p->D % 16 == 0 && p->R % (p->interleaved ? 8 : 16) == 0 && mfa::aligned16(p->q) &&
              mfa::aligned16(p->k) && mfa::aligned16(p->q_out) && mfa::aligned16(p->k_out);
   for (int i = 0; i < 3; ++i)
     vec = vec && p->q_stride[i] * es % 16 == 0 && p->k_stride[i] * es % 16 == 0;
+  const int rs = p->rot_dtype == MFA_FP32 ? 4 : 2;
+  a.w_vec = mfa::aligned16(p->q_weight) && mfa::aligned16(p->k_weight);
+  a.rot_vec = mfa::aligned16(p->cos) && mfa::aligned16(p->sin) && p->cos_stride * rs % 16 == 0 &&
+              p->sin_stride * rs % 16 == 0;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   (void)cudaGetLastError();
   if (p->dtype == MFA_FP32) return mfa::launch_norm_rope<float>(a, vec, st);
