@@ -577,7 +577,8 @@ struct Kv4Smem {
   alignas(128) uint8_t ring[kAttnStages][kStage];
   // a unit's query rows, as they are; the padding spreads 8 rows over the banks
   alignas(16) uint16_t q[kRows][D + 16];
-  float o[kAttnWarps][kRows][D + 4];  // the warps' sums, to be joined
+  // the warps' sums, to be joined; until then, each warp's scales of a block
+  alignas(16) float o[kAttnWarps][kRows][D + 4];
   float m[kAttnWarps][kRows], l[kAttnWarps][kRows];
   Kv4Unit unit[2];  // this one and, while its end is being written, the next one
   uint64_t full[kAttnStages], empty[kAttnStages], q_full, q_empty, met;
@@ -869,28 +870,58 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(D, NT))
       const unsigned bad = sm.bad[slot];
       const bool easy = (unsigned)(j - j_full) < n_full && bad == 0 && !general;
       const uint8_t* base = sm.ring[slot];
-      // this lane's codes and scales: keys of rows g and g + 8 of each tile, values of rows 2t,
-      // 2t + 1, 2t + 8 and 2t + 9
+      // The warp converts the scales of its tiles once, not every lane those it needs: a key's as
+      // fp32, a value's in pairs of the tile's rows 2p, 2p + 1 as fp16.
       const int tile0 = 16 * kWarpTiles * warp;  // this warp's tokens within the block
+      float* k_scale = &sm.o[warp][0][0];                                  // [token][NG]
+      uint32_t* v_scale = reinterpret_cast<uint32_t*>(k_scale + 32 * NG);  // [tile][pair][NG]
+      bool clean = true;
+      __syncwarp();  // the last block's have been read
+      {
+        const uint8_t* yp = base + 2 * Smem::kCodes + (tile0 + lane) * NG;
+        uint32_t w[NG / 4], two[2];
+        load_words<NG>(yp, w);
+#pragma unroll
+        for (int i = 0; i < NG / 4; ++i) {
+          e4m3x4_f16(w[i], two);
+          reinterpret_cast<float4*>(k_scale + lane * NG)[i] =
+              make_float4(f16_lo(two[0]), f16_hi(two[0]), f16_lo(two[1]), f16_hi(two[1]));
+        }
+        // lane: tile, pair and (D = 128) half of the groups
+        constexpr int kHalves = NG / 4;
+        const int pair = lane / kHalves, half = lane % kHalves;  // pair: 8 tile + p
+        if (pair < 8 * kWarpTiles) {
+          const int first = 2 * pair + (pair & 1), second = 2 * pair + 1 - (pair & 1);
+          const uint8_t* zp = base + 2 * Smem::kCodes + Smem::kScales + tile0 * NG + 4 * half;
+          const uint32_t za = *reinterpret_cast<const uint32_t*>(zp + first * NG);
+          const uint32_t zb = *reinterpret_cast<const uint32_t*>(zp + second * NG);
+          uint4 out;
+          e4m3x4_f16(__byte_perm(za, zb, 0x5140), two);
+          out.x = two[0];
+          out.y = two[1];
+          e4m3x4_f16(__byte_perm(za, zb, 0x7362), two);
+          out.z = two[0];
+          out.w = two[1];
+          reinterpret_cast<uint4*>(v_scale + pair * NG)[half] = out;
+          // The NaN scale of a token must not reach a row that does not see it. Such tokens have
+          // probability 0 there, so with finite scales nothing is left to do.
+          if (!easy) clean = !(has_nan_scale(za) || has_nan_scale(zb));
+        }
+        if (!easy) clean = __all_sync(kFull, clean);
+      }
+      __syncwarp();
+      // this lane's codes: keys of rows g and g + 8 of each tile, values of rows 2t, 2t + 1, 2t + 8
+      // and 2t + 9
       const int flip = t & 1, other = 1 - 2 * flip;  // rows from a token to its partner
       const uint8_t* kp = base + (tile0 + key_of) * (D / 2) + t * (D / 8);
-      const uint8_t* yp = base + 2 * Smem::kCodes + (tile0 + key_of) * (D / 16);
       const uint8_t* vp = base + Smem::kCodes + (tile0 + 2 * t + flip) * (D / 2) + g * (D / 16);
-      const uint8_t* zp = base + 2 * Smem::kCodes + Smem::kScales + (tile0 + 2 * t + flip) * (D / 16);
-      const int v_other = other * (D / 2), z_other = other * (D / 16);
+      const int v_other = other * (D / 2);
 #pragma unroll
       for (int h = 0; h < kWarpTiles; ++h) {
-        uint32_t k0[D / 32], k1[D / 32], y0[D / 64], y1[D / 64];
+        uint32_t k0[D / 32], k1[D / 32];
         uint32_t v0[D / 64], v1[D / 64], v2[D / 64], v3[D / 64];
-        uint32_t z0[D / 64], z1[D / 64], z2[D / 64], z3[D / 64];
-        load_words<D / 16>(yp + 16 * h * (D / 16), y0);
-        load_words<D / 16>(yp + (16 * h + 8) * (D / 16), y1);
         load_words<D / 8>(kp + 16 * h * (D / 2), k0);
         load_words<D / 8>(kp + (16 * h + 8) * (D / 2), k1);
-        load_words<D / 16>(zp + 16 * h * (D / 16), z0);
-        load_words<D / 16>(zp + z_other + 16 * h * (D / 16), z1);
-        load_words<D / 16>(zp + (16 * h + 8) * (D / 16), z2);
-        load_words<D / 16>(zp + z_other + (16 * h + 8) * (D / 16), z3);
         load_words<D / 16>(vp + 16 * h * (D / 2), v0);
         load_words<D / 16>(vp + v_other + 16 * h * (D / 2), v1);
         load_words<D / 16>(vp + (16 * h + 8) * (D / 2), v2);
@@ -913,11 +944,13 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(D, NT))
 #pragma unroll
           for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
         {
-          uint32_t fs0[NG / 2], fs1[NG / 2];
+          float fa[NG], fb[NG];
 #pragma unroll
-          for (int w = 0; w < NG / 4; ++w) {
-            e4m3x4_f16(y0[w], fs0 + 2 * w);
-            e4m3x4_f16(y1[w], fs1 + 2 * w);
+          for (int i = 0; i < NG; i += 4) {
+            *reinterpret_cast<float4*>(fa + i) =
+                *reinterpret_cast<const float4*>(k_scale + (16 * h + key_of) * NG + i);
+            *reinterpret_cast<float4*>(fb + i) =
+                *reinterpret_cast<const float4*>(k_scale + (16 * h + key_of + 8) * NG + i);
           }
 #pragma unroll
           for (int w = 0; w < NG / 2; ++w) {  // a word: two groups
@@ -927,16 +960,14 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(D, NT))
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               const uint32_t frag[4] = {ka[2 * i], kb[2 * i], ka[2 * i + 1], kb[2 * i + 1]};
-              const float fa = i ? f16_hi(fs0[w]) : f16_lo(fs0[w]);
-              const float fb = i ? f16_hi(fs1[w]) : f16_lo(fs1[w]);
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
                 float x[4] = {0.f, 0.f, 0.f, 0.f};
                 mma16816(x, frag, qf[nt][2 * w + i][0], qf[nt][2 * w + i][1]);
-                s[nt][0] = fmaf(fa, x[0], s[nt][0]);
-                s[nt][1] = fmaf(fa, x[1], s[nt][1]);
-                s[nt][2] = fmaf(fb, x[2], s[nt][2]);
-                s[nt][3] = fmaf(fb, x[3], s[nt][3]);
+                s[nt][0] = fmaf(fa[2 * w + i], x[0], s[nt][0]);
+                s[nt][1] = fmaf(fa[2 * w + i], x[1], s[nt][1]);
+                s[nt][2] = fmaf(fb[2 * w + i], x[2], s[nt][2]);
+                s[nt][3] = fmaf(fb[2 * w + i], x[3], s[nt][3]);
               }
             }
           }
@@ -947,7 +978,6 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(D, NT))
 #pragma unroll
           for (int e = 0; e < 4; ++e) s[nt][e] *= sc[nt][e & 1];
         unsigned hidden = 0;  // bit 4 nt + e: the row does not see the token
-        bool clean = true;
         if (careful) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
@@ -965,14 +995,6 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(D, NT))
               s[nt][e] = vis ? x : -INFINITY;
               hidden |= (vis ? 0u : 1u) << (4 * nt + e);
             }
-          // The NaN scale of a token must not reach a row that does not see it. Such tokens have
-          // probability 0 there, so with finite scales nothing is left to do.
-          bool nan = false;
-#pragma unroll
-          for (int w = 0; w < NG / 4; ++w)
-            nan = nan || has_nan_scale(z0[w]) || has_nan_scale(z1[w]) || has_nan_scale(z2[w]) ||
-                  has_nan_scale(z3[w]);
-          clean = !__any_sync(kFull, nan);
         }
         bool grow = false;
 #pragma unroll
@@ -1031,11 +1053,10 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(D, NT))
             e2m1x8_f16(((v0[w] >> 4) & 0x0f0f0f0fu) | (v1[w] & 0xf0f0f0f0u), vb);  // dim g + 8
             e2m1x8_f16((v2[w] & 0x0f0f0f0fu) | ((v3[w] << 4) & 0xf0f0f0f0u), vc);
             e2m1x8_f16(((v2[w] >> 4) & 0x0f0f0f0fu) | (v3[w] & 0xf0f0f0f0u), vd);
-            uint32_t sp[4], tp[4];  // pairs of tokens' scales, groups 4w .. 4w + 3
-            e4m3x4_f16(__byte_perm(z0[w], z1[w], 0x5140), sp);
-            e4m3x4_f16(__byte_perm(z0[w], z1[w], 0x7362), sp + 2);
-            e4m3x4_f16(__byte_perm(z2[w], z3[w], 0x5140), tp);
-            e4m3x4_f16(__byte_perm(z2[w], z3[w], 0x7362), tp + 2);
+            // pairs of tokens' scales, groups 4w .. 4w + 3
+            const uint4 s4 = *reinterpret_cast<const uint4*>(v_scale + (8 * h + t) * NG + 4 * w);
+            const uint4 t4 = *reinterpret_cast<const uint4*>(v_scale + (8 * h + t + 4) * NG + 4 * w);
+            const uint32_t sp[4] = {s4.x, s4.y, s4.z, s4.w}, tp[4] = {t4.x, t4.y, t4.z, t4.w};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const uint32_t frag[4] = {va[i], vb[i], vc[i], vd[i]};
@@ -1334,9 +1355,10 @@ struct Kv4Plan {
 
 // Query rows per KV head up to which the codes are read directly. Each 16 rows read and convert
 // the codes again, while the other way converts them once, to memory, for the tensor-core forward.
-// Measured on B200, 4 sequences of 8192 keys, 32/8 heads, D = 128 (us, directly and not):
-// MEASURE
-constexpr int64_t kDirectRows = 64;
+// Measured on B200 (us, directly / not) at 32, 48, 64 and 96 rows: 4 x 8192 keys, 32/8 heads,
+// D = 128: 46/65, 59/71, 76/70, 104/76; 1 x 32768: 51/75, 65/78, 80/81, 112/89; and at 16 and 32
+// rows of D = 64, 16 x 2048 keys, 16/16 heads: 45/51, 69/52.
+int64_t direct_rows(int D) { return D == 128 ? 48 : 16; }
 constexpr int64_t kStageBytes = 512ll << 20;  // keys and values of the sequences done at a time
 
 // The forward of sequences [b0, b0 + n) over keys and values in 16 bits, [n, capacity, Hkv, D].
@@ -1376,7 +1398,7 @@ mfa_fwd_params staged_params(const mfa_kv4_cache* c, const mfa_kv4_fwd_params* p
 Kv4Plan plan_fwd(const mfa_kv4_cache* c, const mfa_kv4_fwd_params* p, int sms) {
   Kv4Plan k;
   const int64_t rows = (int64_t)p->Lq * (p->Hq / c->Hkv);
-  k.direct = rows <= kDirectRows || c->max_pages == 0;
+  k.direct = rows <= direct_rows(c->D) || c->max_pages == 0;
   if (!k.direct) {
     const int64_t each = 2ll * c->max_pages * c->page_size * c->Hkv * c->D;
     k.seqs = (int)std::max<int64_t>(1, std::min<int64_t>(c->B, kStageBytes / 2 / each));
