@@ -375,10 +375,11 @@ struct Kv4Args {
   int causal, wl, wr, sink;
   const float* alibi;
   int row_blocks;
-  // workspace: [0] blocks per CTA, then where each sequence's blocks begin; partial sums of two
-  // units per CTA, [CTA][2][rows][D], and their references and sums [CTA][2][rows]
-  int* ws_line;
-  float *ws_o, *ws_m, *ws_l;
+  int ctas;  // that the line is cut for
+  // workspace: partial sums of two units per CTA, [CTA][2][rows][D], and their references and sums
+  // of weights [CTA][2][rows]
+  float* ws_o;
+  float2* ws_ml;
 };
 
 constexpr int kAttnWarps = 4;                  // consumer warps
@@ -450,6 +451,11 @@ __device__ __forceinline__ int kv4_head_room(const Kv4Args& a, int len) {
 #pragma unroll 1
   for (int rb = 0; rb < a.row_blocks; ++rb) n += kv4_room(kv4_span<kRows>(a, len, rb).n);
   return n;
+}
+
+// What each CTA takes of a line of this length.
+__device__ __forceinline__ int kv4_share(const Kv4Args& a, int total) {
+  return max(kMinShare, (int)(((unsigned)total + a.ctas - 1) / a.ctas));
 }
 
 // Where a CTA stands in the line of blocks.
@@ -632,17 +638,10 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(D, NT))
       if (w < warp) before += sm.scan[w];
       total += sm.scan[w];
     }
-    const int share = max(kMinShare, (int)(((unsigned)total + gridDim.x - 1) / gridDim.x));
-    if (blockIdx.x == 0) {  // for kv4_join, and what is wrong with the lengths
-      if (threadIdx.x == 0) a.ws_line[0] = share;
-      int at = before;
-      for (int b = b0; b < b1; ++b) {
-        a.ws_line[1 + b] = at;
-        const int len = a.seqlens[b], held = kv4_length(a, b);
-        at += kv4_head_room<kRows>(a, held) * c.Hkv;
-        if (len != held) kv4_report(c);
-      }
-    }
+    const int share = kv4_share(a, total);
+    if (blockIdx.x == 0)
+      for (int b = b0; b < b1; ++b)
+        if (a.seqlens[b] != kv4_length(a, b)) kv4_report(c);
     const int64_t begin = (int64_t)share * blockIdx.x;
     if (begin >= total) return;  // all threads alike
     const int start = (int)begin;
@@ -916,143 +915,152 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(D, NT))
       const uint8_t* kp = base + (tile0 + key_of) * (D / 2) + t * (D / 8);
       const uint8_t* vp = base + Smem::kCodes + (tile0 + 2 * t + flip) * (D / 2) + g * (D / 16);
       const int v_other = other * (D / 2);
+      // ---- scores of the tiles: s[h][nt][0, 1] row g, s[h][nt][2, 3] row g + 8
+      const bool careful = !easy;  // alike in all lanes
+      float s[kWarpTiles][NT][4];
+      uint32_t v[kWarpTiles][4][D / 64];
 #pragma unroll
       for (int h = 0; h < kWarpTiles; ++h) {
         uint32_t k0[D / 32], k1[D / 32];
-        uint32_t v0[D / 64], v1[D / 64], v2[D / 64], v3[D / 64];
         load_words<D / 8>(kp + 16 * h * (D / 2), k0);
         load_words<D / 8>(kp + (16 * h + 8) * (D / 2), k1);
-        load_words<D / 16>(vp + 16 * h * (D / 2), v0);
-        load_words<D / 16>(vp + v_other + 16 * h * (D / 2), v1);
-        load_words<D / 16>(vp + (16 * h + 8) * (D / 2), v2);
-        load_words<D / 16>(vp + v_other + (16 * h + 8) * (D / 2), v3);
-        if (h == kWarpTiles - 1) {  // the slot is free again
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sm.empty[slot]);
-        }
-        const int token = see.at(j) * kBlockTokens + tile0 + 16 * h;
-        const bool careful = !easy;  // alike in all lanes
-        if (careful) {  // does any row see any of the tile?
-          if ((bad >> (kWarpTiles * warp + h) & 1) || token >= see.last.hi ||
-              (token + 16 <= see.first.lo && token >= see.last.sk))
-            continue;
-        }
-        // ---- scores of 16 tokens: s[nt][0, 1] row g of the tile, s[nt][2, 3] row g + 8
-        float s[NT][4];
+        load_words<D / 16>(vp + 16 * h * (D / 2), v[h][0]);
+        load_words<D / 16>(vp + v_other + 16 * h * (D / 2), v[h][1]);
+        load_words<D / 16>(vp + (16 * h + 8) * (D / 2), v[h][2]);
+        load_words<D / 16>(vp + v_other + (16 * h + 8) * (D / 2), v[h][3]);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
-        {
-          float fa[NG], fb[NG];
+          for (int e = 0; e < 4; ++e) s[h][nt][e] = 0.f;
+        float fa[NG], fb[NG];
 #pragma unroll
-          for (int i = 0; i < NG; i += 4) {
-            *reinterpret_cast<float4*>(fa + i) =
-                *reinterpret_cast<const float4*>(k_scale + (16 * h + key_of) * NG + i);
-            *reinterpret_cast<float4*>(fb + i) =
-                *reinterpret_cast<const float4*>(k_scale + (16 * h + key_of + 8) * NG + i);
-          }
+        for (int i = 0; i < NG; i += 4) {
+          *reinterpret_cast<float4*>(fa + i) =
+              *reinterpret_cast<const float4*>(k_scale + (16 * h + key_of) * NG + i);
+          *reinterpret_cast<float4*>(fb + i) =
+              *reinterpret_cast<const float4*>(k_scale + (16 * h + key_of + 8) * NG + i);
+        }
 #pragma unroll
-          for (int w = 0; w < NG / 2; ++w) {  // a word: two groups
-            uint32_t ka[4], kb[4];
-            e2m1x8_f16(k0[w], ka);
-            e2m1x8_f16(k1[w], kb);
+        for (int w = 0; w < NG / 2; ++w) {  // a word: two groups
+          uint32_t ka[4], kb[4];
+          e2m1x8_f16(k0[w], ka);
+          e2m1x8_f16(k1[w], kb);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const uint32_t frag[4] = {ka[2 * i], kb[2 * i], ka[2 * i + 1], kb[2 * i + 1]};
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t frag[4] = {ka[2 * i], kb[2 * i], ka[2 * i + 1], kb[2 * i + 1]};
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                float x[4] = {0.f, 0.f, 0.f, 0.f};
-                mma16816(x, frag, qf[nt][2 * w + i][0], qf[nt][2 * w + i][1]);
-                s[nt][0] = fmaf(fa[2 * w + i], x[0], s[nt][0]);
-                s[nt][1] = fmaf(fa[2 * w + i], x[1], s[nt][1]);
-                s[nt][2] = fmaf(fb[2 * w + i], x[2], s[nt][2]);
-                s[nt][3] = fmaf(fb[2 * w + i], x[3], s[nt][3]);
-              }
+            for (int nt = 0; nt < NT; ++nt) {
+              float x[4] = {0.f, 0.f, 0.f, 0.f};
+              mma16816(x, frag, qf[nt][2 * w + i][0], qf[nt][2 * w + i][1]);
+              s[h][nt][0] = fmaf(fa[2 * w + i], x[0], s[h][nt][0]);
+              s[h][nt][1] = fmaf(fa[2 * w + i], x[1], s[h][nt][1]);
+              s[h][nt][2] = fmaf(fb[2 * w + i], x[2], s[h][nt][2]);
+              s[h][nt][3] = fmaf(fb[2 * w + i], x[3], s[h][nt][3]);
             }
           }
         }
-        // ---- logits in log2 units, masks
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.empty[slot]);  // the slot is free again
+      // ---- logits in log2 units, masks
+#pragma unroll
+      for (int h = 0; h < kWarpTiles; ++h)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[nt][e] *= sc[nt][e & 1];
-        unsigned hidden = 0;  // bit 4 nt + e: the row does not see the token
-        if (careful) {
+          for (int e = 0; e < 4; ++e) s[h][nt][e] *= sc[nt][e & 1];
+      unsigned hidden[kWarpTiles] = {};  // bit 4 nt + e: the row does not see the token
+      if (careful) {
+#pragma unroll
+        for (int h = 0; h < kWarpTiles; ++h)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int r = min(r0 + nt * 8 + 2 * t + (e & 1), rows - 1), i = kv4_pos(a, r);
-              const int key = token + key_of + 8 * (e >> 1);
-              float x = s[nt][e];
+              const int key = see.at(j) * kBlockTokens + tile0 + 16 * h + key_of + 8 * (e >> 1);
+              float x = s[h][nt][e];
               if (a.softcap > 0.f) x = a.softcap * 1.4426950408889634f * tanh_any(x);
               if (a.alibi != nullptr)
                 x -= a.alibi[(int64_t)u.b * a.Hq + u.hk * a.group + r - i * a.group] *
                      1.4426950408889634f * fabsf((float)(i + u.len - a.Lq - key));
               const Kv4Range seen = kv4_range(a, u.len, i);
-              const bool vis = (key >= seen.lo || key < seen.sk) && key < seen.hi;
-              s[nt][e] = vis ? x : -INFINITY;
-              hidden |= (vis ? 0u : 1u) << (4 * nt + e);
+              const bool vis = !(bad >> (kWarpTiles * warp + h) & 1) &&
+                               (key >= seen.lo || key < seen.sk) && key < seen.hi;
+              s[h][nt][e] = vis ? x : -INFINITY;
+              hidden[h] |= (vis ? 0u : 1u) << (4 * nt + e);
             }
+      }
+      // ---- a row's reference, over the tiles
+      float top[NT][2];
+      bool grow = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          top[nt][e] = fmaxf(s[0][nt][e], s[0][nt][e + 2]);
+#pragma unroll
+          for (int h = 1; h < kWarpTiles; ++h)
+            top[nt][e] = fmax3(top[nt][e], s[h][nt][e], s[h][nt][e + 2]);
+          grow = grow || top[nt][e] > m[nt][e] + kGrow;
         }
-        bool grow = false;
+      if (__any_sync(kFull, grow)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
-            grow = grow || fmaxf(s[nt][e], s[nt][e + 2]) > m[nt][e] + kGrow;
-        if (__any_sync(kFull, grow)) {
+          for (int e = 0; e < 2; ++e) {
+            float x = top[nt][e];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+            for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(kFull, x, d));
+            if (x > m[nt][e] + kGrow) {
+              const float fresh = x - kBelow;
+              const float factor = m[nt][e] == -INFINITY ? 0.f : ex2(m[nt][e] - fresh);
+              m[nt][e] = m_sub[nt][e] = fresh;
+              l[nt][e] *= factor;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float top = fmaxf(s[nt][e], s[nt][e + 2]);
-#pragma unroll
-              for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, d));
-              if (top > m[nt][e] + kGrow) {
-                const float fresh = top - kBelow;
-                const float factor = m[nt][e] == -INFINITY ? 0.f : ex2(m[nt][e] - fresh);
-                m[nt][e] = m_sub[nt][e] = fresh;
-                l[nt][e] *= factor;
-#pragma unroll
-                for (int i = 0; i < NG; ++i) {
-                  o[nt][i][e] *= factor;
-                  o[nt][i][e + 2] *= factor;
-                }
+              for (int i = 0; i < NG; ++i) {
+                o[nt][i][e] *= factor;
+                o[nt][i][e + 2] *= factor;
               }
             }
-        }
-        // ---- probabilities
-        uint32_t pb[NT][2];
+          }
+      }
+      // ---- probabilities
+      uint32_t pb[kWarpTiles][NT][2];
+#pragma unroll
+      for (int h = 0; h < kWarpTiles; ++h)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           float p[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) p[e] = ex2(s[nt][e] - m_sub[nt][e & 1]);
+          for (int e = 0; e < 4; ++e) p[e] = ex2(s[h][nt][e] - m_sub[nt][e & 1]);
           l[nt][0] += p[0] + p[2];
           l[nt][1] += p[1] + p[3];
-          pb[nt][0] = transpose8x8(h2(p[0], p[1]));  // rows 2t, 2t + 1 of the tile for row g of q
-          pb[nt][1] = transpose8x8(h2(p[2], p[3]));  // rows 2t + 8, 2t + 9
+          pb[h][nt][0] = transpose8x8(h2(p[0], p[1]));  // rows 2t, 2t + 1 of the tile for row g of q
+          pb[h][nt][1] = transpose8x8(h2(p[2], p[3]));  // rows 2t + 8, 2t + 9
         }
-        // ---- values: a byte of two tokens' codes of one dim makes one operand register
-        auto values = [&](auto masked) {
+      // ---- values: a byte of two tokens' codes of one dim makes one operand register
+      auto values = [&](auto masked) {
+#pragma unroll
+        for (int h = 0; h < kWarpTiles; ++h) {
           uint32_t keep[NT][2];
           if constexpr (decltype(masked)::value) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
               for (int e = 0; e < 2; ++e)
-                keep[nt][e] = transpose8x8((hidden >> (4 * nt + 2 * e) & 1 ? 0u : 0xffffu) |
-                                           (hidden >> (4 * nt + 2 * e + 1) & 1 ? 0u : 0xffff0000u));
+                keep[nt][e] =
+                    transpose8x8((hidden[h] >> (4 * nt + 2 * e) & 1 ? 0u : 0xffffu) |
+                                 (hidden[h] >> (4 * nt + 2 * e + 1) & 1 ? 0u : 0xffff0000u));
           }
 #pragma unroll
           for (int w = 0; w < NG / 4; ++w) {  // a word: four groups
+            const uint32_t v0 = v[h][0][w], v1 = v[h][1][w], v2 = v[h][2][w], v3 = v[h][3][w];
             uint32_t va[4], vb[4], vc[4], vd[4];
-            e2m1x8_f16((v0[w] & 0x0f0f0f0fu) | ((v1[w] << 4) & 0xf0f0f0f0u), va);  // dim g
-            e2m1x8_f16(((v0[w] >> 4) & 0x0f0f0f0fu) | (v1[w] & 0xf0f0f0f0u), vb);  // dim g + 8
-            e2m1x8_f16((v2[w] & 0x0f0f0f0fu) | ((v3[w] << 4) & 0xf0f0f0f0u), vc);
-            e2m1x8_f16(((v2[w] >> 4) & 0x0f0f0f0fu) | (v3[w] & 0xf0f0f0f0u), vd);
+            e2m1x8_f16((v0 & 0x0f0f0f0fu) | ((v1 << 4) & 0xf0f0f0f0u), va);  // dim g
+            e2m1x8_f16(((v0 >> 4) & 0x0f0f0f0fu) | (v1 & 0xf0f0f0f0u), vb);  // dim g + 8
+            e2m1x8_f16((v2 & 0x0f0f0f0fu) | ((v3 << 4) & 0xf0f0f0f0u), vc);
+            e2m1x8_f16(((v2 >> 4) & 0x0f0f0f0fu) | (v3 & 0xf0f0f0f0u), vd);
             // pairs of tokens' scales, groups 4w .. 4w + 3
             const uint4 s4 = *reinterpret_cast<const uint4*>(v_scale + (8 * h + t) * NG + 4 * w);
             const uint4 t4 = *reinterpret_cast<const uint4*>(v_scale + (8 * h + t + 4) * NG + 4 * w);
@@ -1062,7 +1070,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(D, NT))
               const uint32_t frag[4] = {va[i], vb[i], vc[i], vd[i]};
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
-                uint32_t p0 = h2mul(pb[nt][0], sp[i]), p1 = h2mul(pb[nt][1], tp[i]);
+                uint32_t p0 = h2mul(pb[h][nt][0], sp[i]), p1 = h2mul(pb[h][nt][1], tp[i]);
                 if constexpr (decltype(masked)::value) {
                   p0 &= keep[nt][0];
                   p1 &= keep[nt][1];
@@ -1071,10 +1079,10 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(D, NT))
               }
             }
           }
-        };
-        if (clean) values(BoolC<false>{});
-        else values(BoolC<true>{});
-      }
+        }
+      };
+      if (clean) values(BoolC<false>{});
+      else values(BoolC<true>{});
     }
 
     if (!ok) break;
@@ -1131,8 +1139,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(D, NT))
           float top = sm.m[0][rr];
 #pragma unroll
           for (int w = 1; w < kAttnWarps; ++w) top = fmaxf(top, sm.m[w][rr]);
-          a.ws_m[part + rr] = top;
-          a.ws_l[part + rr] = sum;
+          a.ws_ml[part + rr] = make_float2(top, sum);
         }
       }
     }
@@ -1150,11 +1157,36 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join(const __grid_constant__
   constexpr int kRows = 8 * NT, kLanes = D / 4, kAtOnce = kJoinThreads / kLanes;
   __shared__ float4 s_val[kAtOnce][kLanes];
   __shared__ float s_weight[kJoinParts], s_red[2][kJoinThreads / 32];
+  __shared__ int s_line[2][kJoinThreads / 32];
   const int h = (int)(blockIdx.x % a.Hq);
-  const int64_t bi = blockIdx.x / a.Hq;
-  const int i = (int)(bi % a.Lq), b = (int)(bi / a.Lq);
-  const int hk = h / a.group, r = i * a.group + h % a.group, rb = r / kRows, rr = r % kRows;
+  const int bi = blockIdx.x / a.Hq, b = bi / a.Lq, i = bi - b * a.Lq;
+  const int hk = kv4_pos(a, h), r = i * a.group + h - hk * a.group, rb = r / kRows, rr = r % kRows;
   const int lane = threadIdx.x % kLanes, p = threadIdx.x / kLanes;
+  const int warp = threadIdx.x / 32;
+  // Where the row's unit stands in the line, while the last CTAs are still at work: what comes
+  // before the sequence, and the whole.
+  int before = 0, total = 0;
+  for (int x = threadIdx.x; x < a.c.B; x += kJoinThreads) {
+    const int n = kv4_head_room<kRows>(a, kv4_length(a, x)) * a.c.Hkv;
+    total += n;
+    if (x < b) before += n;
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) {
+    before += __shfl_xor_sync(kFull, before, d);
+    total += __shfl_xor_sync(kFull, total, d);
+  }
+  if (threadIdx.x % 32 == 0) {
+    s_line[0][warp] = before;
+    s_line[1][warp] = total;
+  }
+  __syncthreads();
+  before = total = 0;
+#pragma unroll
+  for (int w = 0; w < kJoinThreads / 32; ++w) {
+    before += s_line[0][w];
+    total += s_line[1][w];
+  }
   const int len = kv4_length(a, b);
   int head = 0, ahead = 0;  // room of the head's units, and of those before this one
   int n = 0;
@@ -1165,20 +1197,24 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join(const __grid_constant__
     if (x == rb) n = y;
     head += kv4_room(y);
   }
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const unsigned share = a.ws_line[0], u0 = a.ws_line[1 + b] + hk * head + ahead + kUnitCost;
+  const unsigned share = kv4_share(a, total), u0 = before + hk * head + ahead + kUnitCost;
   int c0 = 0, c1 = -1;
   if (n > 0) {
     c0 = u0 / share;
     c1 = (u0 + n - 1) / share;
-    if (c0 == c1) return;
   }
+  // every block waits, also one with nothing to add: what follows this grid relies on it
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (n > 0 && c0 == c1) return;
   auto part = [&](int cta) { return (2 * (int64_t)cta + (cta == c0)) * kRows + rr; };
-  float top = -INFINITY;
-  for (int x = c0 + threadIdx.x; x <= c1; x += kJoinThreads) top = fmaxf(top, a.ws_m[part(x)]);
+  const float2 none = make_float2(-INFINITY, 0.f);
+  const float2 mine = c0 + (int)threadIdx.x <= c1 ? a.ws_ml[part(c0 + threadIdx.x)] : none;
+  float top = mine.x;
+  for (int x = c0 + threadIdx.x + kJoinThreads; x <= c1; x += kJoinThreads)
+    top = fmaxf(top, a.ws_ml[part(x)].x);
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, d));
-  if (threadIdx.x % 32 == 0) s_red[0][threadIdx.x / 32] = top;
+  if (threadIdx.x % 32 == 0) s_red[0][warp] = top;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kJoinThreads / 32; ++w) top = fmaxf(top, s_red[0][w]);
@@ -1188,10 +1224,10 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join(const __grid_constant__
     const int to = min(c1 + 1, from + kJoinParts);
     if (from > c0) __syncthreads();
     for (int x = from + threadIdx.x; x < to; x += kJoinThreads) {
-      const float l = a.ws_l[part(x)], m = a.ws_m[part(x)];
-      const float f = l != l ? l : m == -INFINITY ? 0.f : ex2(m - top);
+      const float2 ml = x == c0 + (int)threadIdx.x ? mine : a.ws_ml[part(x)];
+      const float f = ml.y != ml.y ? ml.y : ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
       s_weight[x - from] = f;
-      sum = fmaf(f, l, sum);
+      sum = fmaf(f, ml.y, sum);
     }
     __syncthreads();
 #pragma unroll 8
@@ -1206,7 +1242,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join(const __grid_constant__
   }
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(kFull, sum, d);
-  if (threadIdx.x % 32 == 0) s_red[1][threadIdx.x / 32] = sum;
+  if (threadIdx.x % 32 == 0) s_red[1][warp] = sum;
   s_val[p][lane] = val;
   __syncthreads();
   if (threadIdx.x >= kLanes) return;
@@ -1346,7 +1382,7 @@ struct Kv4Plan {
   bool direct;
   // straight from the codes
   int nt, row_blocks, ctas;
-  int64_t line, o, m;  // sizes of the workspace's parts, in bytes
+  int64_t o;           // bytes of the partial sums
   // by way of 16-bit keys and values
   int seqs;            // sequences at a time
   int64_t kv;          // bytes of their keys, and of their values
@@ -1420,10 +1456,8 @@ Kv4Plan plan_fwd(const mfa_kv4_cache* c, const mfa_kv4_fwd_params* p, int sms) {
   k.row_blocks = (int)((rows + 8 * k.nt - 1) / (8 * k.nt));
   k.ctas = sms * kv4_ctas(c->D, k.nt);
   const int64_t parts = 2ll * k.ctas * 8 * k.nt;
-  k.line = ((c->B + 1) * 4ll + 127) / 128 * 128;
   k.o = parts * c->D * 4;
-  k.m = parts * 4;
-  k.bytes = (size_t)(k.line + k.o + 2 * k.m);
+  k.bytes = (size_t)(k.o + parts * 8);
   return k;
 }
 
@@ -1552,11 +1586,9 @@ int mfa_kv4_fwd(const mfa_kv4_cache* c, const mfa_kv4_fwd_params* p, void* strea
   a.sink = p->win_left >= 0 ? p->sink : 0;
   a.alibi = p->alibi;
   a.row_blocks = plan.row_blocks;
-  uint8_t* ws = static_cast<uint8_t*>(p->workspace);
-  a.ws_line = reinterpret_cast<int*>(ws);
-  a.ws_o = reinterpret_cast<float*>(ws + plan.line);
-  a.ws_m = reinterpret_cast<float*>(ws + plan.line + plan.o);
-  a.ws_l = reinterpret_cast<float*>(ws + plan.line + plan.o + plan.m);
+  a.ctas = plan.ctas;
+  a.ws_o = static_cast<float*>(p->workspace);
+  a.ws_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(p->workspace) + plan.o);
   if (c->D == 128)
     return plan.nt == 1 ? mfa::launch_fwd<128, 1>(a, plan.ctas, dev, st)
                         : mfa::launch_fwd<128, 2>(a, plan.ctas, dev, st);
