@@ -138,6 +138,14 @@ def _err_word(device):
     return t
 
 
+def _err_ptr(device):
+    """Address of the device's error word; 0 where the first call of all is being captured: a word
+    made then would be zeroed by every replay, and hold anything before the first."""
+    if device not in _err_words and torch.cuda.is_current_stream_capturing():
+        return 0
+    return _err_word(device).data_ptr()
+
+
 def check_device_errors(device=None):
     """Synchronise and raise if any kernel on ``device`` reported a bounded-wait timeout."""
     dev = torch.device(device) if device is not None else torch.device("cuda")
@@ -216,7 +224,7 @@ def _values(q, k, v, o, B, Hq, Hkv, Lq, Lk, D, q_st, k_st, v_st, o_st, scale, ca
             int(bias.window_left), int(bias.window_right),
             bias.alibi.data_ptr() if bias.alibi is not None else 0,
             _DTYPES[q.dtype], _DTYPES[o.dtype], int(k_pos_offset), int(lk_total), kernel,
-            _err_word(q.device).data_ptr(), 0, 0, cu_q_host, bias.sink)
+            _err_ptr(q.device), 0, 0, cu_q_host, bias.sink)
 
 
 def _params(q, k, v, o, *, B, Hq, Hkv, Lq, Lk, D, q_st, k_st, v_st, o_st, scale, causal,

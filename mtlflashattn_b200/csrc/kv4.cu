@@ -1356,6 +1356,13 @@ int launch_rows(const Kv4Cache& c, const Kv4Rows& r, int D, cudaStream_t st) {
   return D == 128 ? launch_rows<T, 128, kGather>(c, r, st) : launch_rows<T, 64, kGather>(c, r, st);
 }
 
+// Query rows per KV head up to which the codes are read directly. Each 16 rows read and convert
+// the codes again, while the other way converts them once, to memory, for the tensor-core forward.
+// Measured on B200 (us, directly / not) at 32, 48, 64 and 96 rows: 4 x 8192 keys, 32/8 heads,
+// D = 128: 46/65, 59/71, 76/70, 104/76; 1 x 32768: 51/75, 65/78, 80/81, 112/89; and at 16 and 32
+// rows of D = 64, 16 x 2048 keys, 16/16 heads: 45/51, 69/52.
+int64_t direct_rows(int D) { return D == 128 ? 48 : 16; }
+
 int check_fwd(const mfa_kv4_cache* c, const mfa_kv4_fwd_params* p) {
   const int rc = check_cache(c);
   if (rc != MFA_OK) return rc;
@@ -1367,9 +1374,11 @@ int check_fwd(const mfa_kv4_cache* c, const mfa_kv4_fwd_params* p) {
   if (c->B == 0 || p->Lq == 0) return MFA_OK;
   if (p->q == nullptr || p->o == nullptr || p->seqlens == nullptr) return MFA_ERR_INVALID;
   if ((int64_t)c->B * p->Lq * p->Hq >= (1ll << 31)) return MFA_ERR_UNSUPPORTED;
-  // the line is counted in 32 bits
-  const double rows = std::ceil((double)p->Lq * (p->Hq / c->Hkv) / 8);
-  if ((double)c->B * c->Hkv * rows * ((double)c->max_pages * c->page_size / kBlockTokens + 10) >= 2147483648.0)
+  // the direct path's line is counted in 32 bits
+  const int64_t rows = (int64_t)p->Lq * (p->Hq / c->Hkv);
+  if (rows <= direct_rows(c->D) &&
+      (double)c->B * c->Hkv * ((rows + 7) / 8) *
+              ((double)c->max_pages * c->page_size / kBlockTokens + 10) >= 2147483648.0)
     return MFA_ERR_UNSUPPORTED;
   if (reinterpret_cast<uintptr_t>(p->o) % 8 != 0) return MFA_ERR_INVALID;
   for (int i = 0; i < 3; ++i)
@@ -1389,12 +1398,6 @@ struct Kv4Plan {
   size_t bytes;
 };
 
-// Query rows per KV head up to which the codes are read directly. Each 16 rows read and convert
-// the codes again, while the other way converts them once, to memory, for the tensor-core forward.
-// Measured on B200 (us, directly / not) at 32, 48, 64 and 96 rows: 4 x 8192 keys, 32/8 heads,
-// D = 128: 46/65, 59/71, 76/70, 104/76; 1 x 32768: 51/75, 65/78, 80/81, 112/89; and at 16 and 32
-// rows of D = 64, 16 x 2048 keys, 16/16 heads: 45/51, 69/52.
-int64_t direct_rows(int D) { return D == 128 ? 48 : 16; }
 constexpr int64_t kStageBytes = 512ll << 20;  // keys and values of the sequences done at a time
 
 // The forward of sequences [b0, b0 + n) over keys and values in 16 bits, [n, capacity, Hkv, D].

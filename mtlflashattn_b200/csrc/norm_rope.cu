@@ -168,7 +168,7 @@ template <typename T, bool kInterleaved, int LP>
 __global__ void __launch_bounds__(128, sizeof(T) == 2 ? 6 : 5)
     norm_rope_vec(const __grid_constant__ NormRopeArgs a) {
   constexpr int kRows = 32 / LP;  // heads a warp holds at once
-  const int w = (blockIdx.x * 128 + threadIdx.x) >> 5;
+  const int w = blockIdx.x * 4 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31, sub = lane % LP;
   const int token = w / a.segments, seg = w - token * a.segments;
   if (token >= a.B * a.L) return;

@@ -141,7 +141,7 @@ def _pack_cache(cache, block_table, B, dev):
     _CACHE.pack_into(
         p, 0, k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
         cache.v_scale.data_ptr(), block_table.data_ptr(), stride[0], pages, size, heads, 2 * half,
-        B, max_pages, cache.k_unit, cache.v_unit, _kernel._err_word(dev).data_ptr())
+        B, max_pages, cache.k_unit, cache.v_unit, _kernel._err_ptr(dev))
     return p
 
 

@@ -138,7 +138,7 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, rotary_cos=None, rotary_sin
         p, 0, x.data_ptr(), y.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), qs[0], qs[1], qs[2],
         ks[0], ks[1], ks[2], wq, wk, cos, sin, cos_row, sin_row, pos, pos_b, pos_l, B, L, Hq, Hkv,
         D, R, min(rows, 2**31 - 1), pos64, code, w_code, rot_code, bool(interleaved), eps,
-        _kernel._err_word(dev).data_ptr())
+        _kernel._err_ptr(dev))
     _kernel._call(dev, "qk_norm_rope", _lib.qk_norm_rope, p)
     if torch.is_grad_enabled():
         extra = (q, k, q_weight, k_weight, rotary_cos, rotary_sin)
