@@ -44,7 +44,8 @@ enum mfa_status {
   MFA_ERR_TIMEOUT = 4,        /* a bounded in-kernel wait expired; output is invalid */
   MFA_ERR_NO_DEVICE = 5,      /* no usable sm_100 device for the requested kernel */
   MFA_ERR_FAULT_INJECTED = 6, /* host-side fault injection (MFA_FAULT env) fired */
-  MFA_ERR_SCRATCH_TOO_SMALL = 7, /* mfa_fwd_noalloc: the problem needs more than its scratch */
+  MFA_ERR_SCRATCH_TOO_SMALL = 7, /* mfa_fwd_noalloc: the problem needs more than its scratch;
+                                    mfa_kv4_fwd: than the workspace it was given */
   MFA_ERR_CHECK = 8             /* (in *err) a device-side bounds check of a build with
                                    -DMFA_CHECKS=1 failed; the access was skipped */
 };
@@ -294,8 +295,9 @@ int mfa_qk_norm_rope(const mfa_norm_rope_params* p, void* cuda_stream);
  *   keys    byte (j / 4) (D / 8) + 2 i + (j % 4) / 2, half (j % 4) % 2
  *   values  byte (j % 8) (D / 16) + i, half j / 8
  * Token t of sequence b is slot t % page_size of page block_table[b][t / page_size]. A page index
- * outside [0, num_pages), or a token outside [0, max_pages * page_size), is never dereferenced: it
- * is skipped and MFA_ERR_INVALID goes to *err. */
+ * outside [0, num_pages), or a token outside [0, max_pages * page_size), is never dereferenced:
+ * MFA_ERR_INVALID goes to *err, and the token is not written, read back as 0, and left out of the
+ * attention or, in calls with many query rows, attended as 0. */
 typedef struct mfa_kv4_cache {
   void* k;            /* [num_pages, Hkv, page_size, D/2] bytes, contiguous, 16-byte aligned */
   void* v;
@@ -303,7 +305,8 @@ typedef struct mfa_kv4_cache {
   void* v_scale;
   const int32_t* block_table; /* [B, max_pages], row stride table_stride (elements) */
   int64_t table_stride;
-  int32_t num_pages, page_size; /* page_size a power of two, 16 .. 1024 */
+  int32_t num_pages, page_size; /* page_size a power of two, 16 .. 1024;
+                                   max_pages * page_size <= 2^31 - 4096 */
   int32_t Hkv, D;     /* D 64 or 128 */
   int32_t B, max_pages;
   float k_unit, v_unit; /* powers of two, 2^-14 .. 2^4 */
@@ -347,7 +350,10 @@ typedef struct mfa_kv4_fwd_params {
 } mfa_kv4_fwd_params;
 
 /* Attention of the newest Lq rows of every sequence over its cached keys; the semantics of
- * mfa_fwd with Lk = seqlens[b]. A row that sees no key is 0. */
+ * mfa_fwd with Lk = seqlens[b]. A row that sees no key is 0. Up to 48 query rows per KV head (D =
+ * 128; 16 at D = 64) read the codes directly; more convert the visible keys and values to 16 bits
+ * in the workspace (512 MiB of them at a time, or one sequence's capacity where that is more) and
+ * run the tensor-core forward on them. */
 int mfa_kv4_fwd(const mfa_kv4_cache* c, const mfa_kv4_fwd_params* p, void* cuda_stream);
 size_t mfa_kv4_fwd_workspace_size(const mfa_kv4_cache* c, const mfa_kv4_fwd_params* p);
 

@@ -684,7 +684,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(D, NT))
     auto page_of = [&](const Kv4Walk<kRows>& w) {  // of the batch that begins at w.j
       const int j = w.j + (lane >> bshift);
       const int t = w.span.at(j) * kBlockTokens + ((lane & ((1 << bshift) - 1)) << pshift);
-      // tokens past the length may have no page: -1 there
+      // -2: no token of the sequence is there, and there need not be a page
       const bool on = w.take > 0 && lane < w.take << bshift && t < w.len;
       return on ? c.table[(int64_t)w.b * c.table_stride + (t >> c.page_shift)] : -2;
     };
@@ -864,7 +864,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(D, NT))
     for (int j = u.j; j < j_end; ++j, ++it) {
       const int slot = it % kAttnStages;
       ok = __all_sync(kFull, mbar_wait(&sm.full[slot], (uint32_t)(it / kAttnStages) & 1u,
-                                             abort_flag));
+                                       abort_flag));
       if (!ok) break;
       const unsigned bad = sm.bad[slot];
       const bool easy = (unsigned)(j - j_full) < n_full && bad == 0 && !general;
@@ -1279,7 +1279,8 @@ int check_cache(const mfa_kv4_cache* c) {
   if (c->page_size < 16 || c->page_size > 1024 || (c->page_size & (c->page_size - 1)) != 0)
     return MFA_ERR_UNSUPPORTED;
   if (c->num_pages < 0 || c->Hkv < 1 || c->B < 0 || c->max_pages < 0) return MFA_ERR_INVALID;
-  if ((int64_t)c->max_pages * c->page_size >= (1ll << 31)) return MFA_ERR_INVALID;
+  // token indices, and what is added to them for a block, stay within 32 bits
+  if ((int64_t)c->max_pages * c->page_size > (1ll << 31) - 4096) return MFA_ERR_INVALID;
   if (!is_unit(c->k_unit) || !is_unit(c->v_unit)) return MFA_ERR_INVALID;
   if (c->B == 0) return MFA_OK;
   if (c->num_pages > 0 && (c->k == nullptr || c->v == nullptr || c->k_scale == nullptr ||

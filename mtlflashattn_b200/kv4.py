@@ -132,8 +132,8 @@ def _pack_cache(cache, block_table, B, dev):
         raise ValueError("mtlflashattn_b200: all tensors must be on the cache's device")
     pages, heads, size, half = k.shape
     max_pages = table[1]
-    if max_pages * size >= 2**31:
-        raise ValueError("mtlflashattn_b200: block_table covers 2^31 tokens or more")
+    if max_pages * size > 2**31 - 4096:
+        raise ValueError("mtlflashattn_b200: block_table covers more than 2^31 - 4096 tokens")
     stride = block_table.stride()
     if max_pages > 1 and stride[1] != 1:
         raise ValueError("mtlflashattn_b200: block_table must have a contiguous last dimension")
@@ -271,6 +271,13 @@ def flash_attn_with_kv4cache(q, cache, block_table, cache_seqlens, softmax_scale
 
 
 def _launch(c, p, dev, stream):
+    # the stream's workspace is usually there and large enough: no need to ask first
+    ws = _kernel._workspaces.get((dev, stream))
+    if ws is not None and not torch.cuda.is_current_stream_capturing():
+        _WS.pack_into(p, _lib.KV4_FWD_WORKSPACE_OFFSET, ws.data_ptr(), ws.numel())
+        rc = _lib.kv4_fwd(c, p, stream)
+        if rc != _lib.ERR_SCRATCH_TOO_SMALL:
+            return rc
     need = _lib.kv4_fwd_workspace_size(c, p)
     if need > 0:
         ws = _kernel._workspace(dev, stream, need)

@@ -284,6 +284,35 @@ def test_chunk_with_softcap_and_alibi():
     compare(cache, table, lens, q, slopes=slopes)
 
 
+@pytest.mark.parametrize("D,Hq,Hkv,Lq,page", [
+    (64, 71, 1, 1, 64), (128, 71, 1, 1, 64),   # more heads per KV head than rows read directly
+    (128, 48, 1, 1, 16), (128, 9, 1, 5, 1024), (64, 16, 1, 1, 1024), (64, 2, 2, 16, 16),
+    (128, 7, 7, 1, 32), (128, 3, 1, 16, 128)])
+def test_row_counts_and_pages(D, Hq, Hkv, Lq, page):
+    lens = (300, 1025, Lq)
+    cache, table, g = filled(lens, page, Hkv, D, seed=Hq)
+    q = torch.randn(3, Lq, Hq, D, device=DEV, generator=g).bfloat16()
+    compare(cache, table, lens, q, causal=True)
+    compare(cache, table, lens, q, window=(70, 2), sink=3)
+    compare(cache, table, lens, q, causal=True, window=(2**40, -1), sink=10**15)
+
+
+@pytest.mark.parametrize("B,Lq", [(400, 1), (333, 2)])
+def test_more_sequences_than_threads(B, Lq):
+    lens = tuple((7 * b * b) % 90 if b % 5 else 0 for b in range(B))
+    cache, table, g = filled(lens, 16, 1, 64, seed=B)
+    q = torch.randn(B, Lq, 3, 64, device=DEV, generator=g).half()
+    compare(cache, table, lens, q, causal=True)
+
+
+def test_one_long_and_many_short_sequences():
+    """The line of blocks is cut anywhere: a unit over many CTAs next to many units in one."""
+    lens = (30000, *[1 + 13 * b % 200 for b in range(60)], 9000)
+    cache, table, g = filled(lens, 64, 2, 128, seed=31)
+    q = torch.randn(len(lens), 1, 8, 128, device=DEV, generator=g).bfloat16()
+    compare(cache, table, lens, q, causal=True)
+
+
 def test_extreme_queries():
     """Query rows far outside of fp16's range in bf16, zeros, and infinities in one row only."""
     lens = (300,)
@@ -474,6 +503,43 @@ def test_captured_steps_replayed_together():
         assert torch.equal(k[-30:], ref.held(kv[0]).expand(30, -1, -1))
         check(out[0], ref.attention(q[0], k, v, True), v)
     _kernel.check_device_errors()
+
+
+def test_first_call_of_a_process_captured():
+    """No eager call before: nothing that the capture made may be missing at replay."""
+    import os
+    import subprocess
+    import sys
+    import textwrap
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = textwrap.dedent("""
+        import torch, mtlflashattn_b200 as mfa
+        from mtlflashattn_b200 import _kernel
+        cache = mfa.kv4_cache(64, 64, 2, 128, "cuda")
+        table = torch.arange(64, device="cuda").int().view(1, 64)
+        n = torch.tensor([3000], dtype=torch.int32, device="cuda")
+        kv = torch.randn(1, 3000, 2, 128, device="cuda").bfloat16()
+        q = torch.randn(1, 1, 8, 128, device="cuda").bfloat16()
+        zero = torch.zeros(1, dtype=torch.int32, device="cuda")
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            qq, _ = mfa.qk_norm_rope(q, kv[:, :1])
+            mfa.kv4_append(cache, kv, kv, table, zero)
+            out = mfa.flash_attn_with_kv4cache(qq, cache, table, n, causal=True)
+            dense = mfa.flash_attn_func(qq, kv, kv, causal=True, window_size=(500, -1), sink_tokens=4)
+        _kernel.check_device_errors("cuda")
+        g.replay()
+        torch.cuda.synchronize()
+        qq, _ = mfa.qk_norm_rope(q, kv[:, :1])
+        assert torch.equal(out, mfa.flash_attn_with_kv4cache(qq, cache, table, n, causal=True))
+        assert torch.equal(dense, mfa.flash_attn_func(qq, kv, kv, causal=True,
+                                                      window_size=(500, -1), sink_tokens=4))
+        _kernel.check_device_errors("cuda")
+        print("same")
+    """)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=root,
+                       timeout=300)
+    assert r.returncode == 0 and "same" in r.stdout, r.stdout[-1000:] + r.stderr[-3000:]
 
 
 def test_two_threads_on_two_streams():

@@ -131,7 +131,7 @@ def cache_params(**kw):
     (dict(k_unit=0.3), _lib.ERR_INVALID), (dict(v_unit=64.0), _lib.ERR_INVALID),
     (dict(k=24), _lib.ERR_INVALID), (dict(v_scale=None), _lib.ERR_INVALID),
     (dict(block_table=None), _lib.ERR_INVALID), (dict(num_pages=-1), _lib.ERR_INVALID),
-    (dict(max_pages=2**27), _lib.ERR_INVALID), (dict(B=-1), _lib.ERR_INVALID)])
+    (dict(max_pages=2**27), _lib.ERR_INVALID), (dict(max_pages=2**27 - 255), _lib.ERR_INVALID), (dict(B=-1), _lib.ERR_INVALID)])
 def test_library_checks_the_cache(kw, rc):
     r = _lib.MfaKv4Rows(k=16, v=16, L=1, dtype=_lib.BF16, lens=4)
     p = _lib.MfaKv4FwdParams(q=16, o=16, seqlens=4, Lq=1, Hq=2, dtype=_lib.BF16, scale=1.0,
