@@ -182,15 +182,15 @@ __global__ void __launch_bounds__(kRowThreads) kv4_append_kernel(const Kv4Cache 
     // codes or at least 2^-11 of itself (2^-13 absolute) away from it, so rounding it to 2^-16 (by
     // adding and taking away 1.5 * 2^7) gives the right side and restores exact halves.
     const float inv = scale > 0.f ? __frcp_rn(scale) * per_unit : 0.f;
+    // (with a NaN scale the codes do not matter)
+    const uint64_t inv2 = f2pack(inv, inv), up = f2pack(192.f, 192.f), down = f2pack(-192.f, -192.f);
     float v[16];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      v[2 * e] = Kv4Two<T>::lo(*reinterpret_cast<const T2*>(&w[e]));
-      v[2 * e + 1] = Kv4Two<T>::hi(*reinterpret_cast<const T2*>(&w[e]));
+      const T2 x2 = *reinterpret_cast<const T2*>(&w[e]);
+      const uint64_t y = ffma2(f2pack(Kv4Two<T>::lo(x2), Kv4Two<T>::hi(x2)), inv2, up);
+      f2unpack(fadd2(y, down), v[2 * e], v[2 * e + 1]);
     }
-#pragma unroll
-    for (int e = 0; e < 16; ++e)
-      v[e] = nan ? 0.f : __fadd_rn(__fmaf_rn(v[e], inv, 192.f), -192.f);
     uint32_t code[8];
     if (!is_v) {
 #pragma unroll
