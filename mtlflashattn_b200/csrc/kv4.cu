@@ -389,7 +389,7 @@ constexpr int kBlockTokens = 16 * kWarpTiles * kAttnWarps;
 constexpr int kBlockTiles = kBlockTokens / 16;
 constexpr int kAttnStages = 3;
 constexpr int kMinShare = 2;   // blocks per CTA at least: below, joining costs more than it gives
-constexpr int kUnitCost = 3;  // beginning and ending a unit takes about as long as so many blocks
+constexpr int kUnitCost = 2;  // beginning and ending a unit takes about as long as so many blocks
 // CTAs per SM: what shared memory and 128 registers per thread allow; two tiles of rows at D = 128
 // take more of both.
 __host__ __device__ constexpr int kv4_ctas(int D, int nt) { return D == 128 && nt == 2 ? 2 : 3; }
