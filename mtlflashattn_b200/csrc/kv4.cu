@@ -91,7 +91,9 @@ __device__ __forceinline__ int kv4_div(int x, uint32_t mul, uint32_t shift) {
 }
 
 // ------------------------------------------------------------------ append and gather
-// Both are bound by memory: 16-bit rows on one side, 0.28 of their bytes on the other. A CTA takes
+// 16-bit rows on one side, 0.28 of their bytes on the other; issue slots bound both (76 % of them
+// taken in the append, 61 % in the gather) before memory does. B200, 2 x 8192 tokens, 8 heads,
+// D = 128, bf16: append 20.6 us (4.2 TB/s), gather 15.6 us (5.5 TB/s). A CTA takes
 // a tile of 4096 codes of one head (32 rows of D = 128, 64 of D = 64), keys or values, through
 // shared memory, where the layout's permutation happens, so that every access to memory is 16
 // bytes of a row; rows are (sequence, token) pairs in one line and look up their pages themselves.
@@ -356,12 +358,18 @@ __global__ void __launch_bounds__(kRowThreads) kv4_gather_kernel(const Kv4Cache 
 //   values: the scale of (token, group) multiplies the probability, in fp16, before the
 //           instruction of that group (its rounding, 2^-11 of each term, is that of fp16 P).
 //
-// A CTA is four consumer warps and a producer warp. The producer copies blocks of 64 tokens (codes
-// and scales, one bulk copy each per page piece) into a ring; each consumer takes 16 of the tokens.
+// A CTA is four consumer warps and a producer warp. The producer copies blocks of 128 tokens (codes
+// and scales, one bulk copy each per page piece) into a ring; each consumer takes two tiles of 16 of
+// the tokens, both at a time, so that one's conversions fill the other's waits.
 // Work is shared out by blocks, not by sequences: the blocks of every (sequence, KV head, tile of
 // query rows) that has visible keys stand in one line, which the CTAs of one wave cut into equal
 // shares. A share that covers a whole unit writes its rows; one that does not leaves a partial
 // result, and kv4_join adds those up. Lengths are read on the device.
+//
+// What bounds it is issue and the ALU pipe (55 % and 48 % busy), which converts the codes, before
+// memory. B200: 1 x 1 x 131072 tokens, 64/8 heads, D = 128: 38 us, 4.0 TB/s of codes and scales (62 %
+// of a copy's rate); 32 x 1 x up to 8192, 32/8 heads: 40 us; 1 x 1 x 4096: 7.4 us. The copies alone
+// took 21 us for the first, from L2. Eight warps of one tile instead of four of two: 51 us.
 struct Kv4Args {
   Kv4Cache c;
   const void* q;
@@ -388,8 +396,12 @@ constexpr int kWarpTiles = 2;  // tiles of 16 tokens that a consumer takes of a 
 constexpr int kBlockTokens = 16 * kWarpTiles * kAttnWarps;
 constexpr int kBlockTiles = kBlockTokens / 16;
 constexpr int kAttnStages = 3;
-constexpr int kMinShare = 2;   // blocks per CTA at least: below, joining costs more than it gives
-constexpr int kUnitCost = 2;  // beginning and ending a unit takes about as long as so many blocks
+// Blocks per CTA at least: more leave SMs idle in short calls. 1 x 1 x 4096, 32/8 heads, attention
+// kernel with 2 / 4 / 8 blocks: 7.4 / 8.7 / 11.8 us; 1 x 1 x 16384: 10.3 / 11.6 / 14.4.
+constexpr int kMinShare = 2;
+// Beginning and ending a unit takes about as long as so many blocks. 32 x 1 x up to 8192, a call
+// with 2 / 3 / 4: 47.5 / 48.5 / 47.7 us; 8 x 1 x 26000: 44.0 / 45.6 / 45.6.
+constexpr int kUnitCost = 2;
 // CTAs per SM: what shared memory and 128 registers per thread allow; two tiles of rows at D = 128
 // take more of both.
 __host__ __device__ constexpr int kv4_ctas(int D, int nt) { return D == 128 && nt == 2 ? 2 : 3; }
@@ -1149,7 +1161,8 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(D, NT))
 
 // Adds up the partial results of a row: one block per output row. Rows that one CTA finished are
 // left as they are; rows without visible keys become 0. The parts' weights are made first, all at
-// once, so that the long loop only loads and adds.
+// once, so that the long loop only loads and adds. Launched while kv4_attn still runs, it finds its
+// parts before the last CTAs end; 1 x 1 x 131072: a call takes 43.7 us, kv4_attn 38.0 of them.
 constexpr int kJoinThreads = 256;
 constexpr int kJoinParts = 512;  // weights held at a time
 template <int D, int NT>
@@ -1359,10 +1372,10 @@ int launch_rows(const Kv4Cache& c, const Kv4Rows& r, int D, cudaStream_t st) {
 
 // Query rows per KV head up to which the codes are read directly. Each 16 rows read and convert
 // the codes again, while the other way converts them once, to memory, for the tensor-core forward.
-// Measured on B200 (us, directly / not) at 32, 48, 64 and 96 rows: 4 x 8192 keys, 32/8 heads,
-// D = 128: 46/65, 59/71, 76/70, 104/76; 1 x 32768: 51/75, 65/78, 80/81, 112/89; and at 16 and 32
-// rows of D = 64, 16 x 2048 keys, 16/16 heads: 45/51, 69/52.
-int64_t direct_rows(int D) { return D == 128 ? 48 : 16; }
+// Measured on B200 (us a call, directly / not) at 32, 48, 64 and 96 rows: 4 x 8192 keys, 32/8
+// heads, D = 128: 42/66, 55/71, 68/69, 99/75; 1 x 32768: 47/75, 61/78, 75/81, 106/89; and at 16 and
+// 32 rows of D = 64, 16 x 2048 keys, 16/16 heads: 43/52, 74/53.
+int64_t direct_rows(int D) { return D == 128 ? 64 : 16; }
 
 int check_fwd(const mfa_kv4_cache* c, const mfa_kv4_fwd_params* p) {
   const int rc = check_cache(c);

@@ -297,6 +297,16 @@ def test_row_counts_and_pages(D, Hq, Hkv, Lq, page):
     compare(cache, table, lens, q, causal=True, window=(2**40, -1), sink=10**15)
 
 
+@pytest.mark.parametrize("Hq,Lq", [(64, 1), (65, 1), (16, 4), (13, 5), (1, 49), (7, 9)])
+def test_rows_around_the_direct_limit(Hq, Lq):
+    """The last row counts whose codes are read directly, and the first that go through 16 bits."""
+    lens = (1300, Lq, 700)
+    cache, table, g = filled(lens, 32, 1, 128, seed=Hq)
+    q = torch.randn(3, Lq, Hq, 128, device=DEV, generator=g).half()
+    compare(cache, table, lens, q, causal=True)
+    compare(cache, table, lens, q, causal=True, window=(200, -1), sink=130)
+
+
 @pytest.mark.parametrize("B,Lq", [(400, 1), (333, 2)])
 def test_more_sequences_than_threads(B, Lq):
     lens = tuple((7 * b * b) % 90 if b % 5 else 0 for b in range(B))
