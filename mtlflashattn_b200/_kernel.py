@@ -286,6 +286,10 @@ def _call(dev, what, fn, *args):
 
 
 _workspaces = {}  # (device, stream) -> uint8 tensor
+# Held from the lookup of a stream's workspace until all of the call's kernels are queued: another
+# thread's kernels on that stream must not come between one that leaves partial sums there and the
+# one that joins them.
+_workspace_lock = threading.RLock()
 
 
 def _workspace(dev, stream, need):
@@ -318,9 +322,12 @@ def _run(p, q, what, causal, trace_shape, kernel, D):
         stream = torch._C._cuda_getCurrentRawStream(dev.index)  # the current stream's handle
         need = _lib.workspace_size(p)
         if need > 0:  # few query rows: let the library split the keys over more CTAs
-            ws = _workspace(dev, stream, need)
-            _WS.pack_into(p, _lib.WORKSPACE_OFFSET, ws.data_ptr(), need)
-        rc = _lib.fwd(p, stream)
+            with _workspace_lock:
+                ws = _workspace(dev, stream, need)
+                _WS.pack_into(p, _lib.WORKSPACE_OFFSET, ws.data_ptr(), need)
+                rc = _lib.fwd(p, stream)
+        else:
+            rc = _lib.fwd(p, stream)
         if rc != _lib.OK:
             if rc == _lib.ERR_UNSUPPORTED and kernel != _lib.KERNEL_AUTO:
                 raise RuntimeError(

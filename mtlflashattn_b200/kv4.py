@@ -271,15 +271,16 @@ def flash_attn_with_kv4cache(q, cache, block_table, cache_seqlens, softmax_scale
 
 
 def _launch(c, p, dev, stream):
-    # the stream's workspace is usually there and large enough: no need to ask first
-    ws = _kernel._workspaces.get((dev, stream))
-    if ws is not None and not torch.cuda.is_current_stream_capturing():
-        _WS.pack_into(p, _lib.KV4_FWD_WORKSPACE_OFFSET, ws.data_ptr(), ws.numel())
-        rc = _lib.kv4_fwd(c, p, stream)
-        if rc != _lib.ERR_SCRATCH_TOO_SMALL:
-            return rc
-    need = _lib.kv4_fwd_workspace_size(c, p)
-    if need > 0:
-        ws = _kernel._workspace(dev, stream, need)
-        _WS.pack_into(p, _lib.KV4_FWD_WORKSPACE_OFFSET, ws.data_ptr(), need)
-    return _lib.kv4_fwd(c, p, stream)
+    with _kernel._workspace_lock:
+        # the stream's workspace is usually there and large enough: no need to ask first
+        ws = _kernel._workspaces.get((dev, stream))
+        if ws is not None and not torch.cuda.is_current_stream_capturing():
+            _WS.pack_into(p, _lib.KV4_FWD_WORKSPACE_OFFSET, ws.data_ptr(), ws.numel())
+            rc = _lib.kv4_fwd(c, p, stream)
+            if rc != _lib.ERR_SCRATCH_TOO_SMALL:
+                return rc
+        need = _lib.kv4_fwd_workspace_size(c, p)
+        if need > 0:
+            ws = _kernel._workspace(dev, stream, need)
+            _WS.pack_into(p, _lib.KV4_FWD_WORKSPACE_OFFSET, ws.data_ptr(), need)
+        return _lib.kv4_fwd(c, p, stream)

@@ -575,3 +575,46 @@ def test_two_threads_on_two_streams():
     for t in threads:
         t.join()
     assert not wrong
+
+
+def test_threads_that_share_a_stream():
+    """Two host threads whose calls share a stream, and with it the workspace that an attention
+    kernel leaves partial sums in for the kernel that joins them."""
+    import threading
+
+    lens = (5000, 900)
+    cases = []
+    for seed in (1, 2):
+        cache, table, g = filled(lens, 64, 2, 128, seed=seed)
+        q = torch.randn(2, 1, 8, 128, device=DEV, generator=g).half()
+        k = torch.randn(1, 9000, 2, 128, device=DEV, generator=g).half()
+
+        def paged(q=q, cache=cache, table=table):
+            return mfa.flash_attn_with_kv4cache(q, cache, table, i32(*lens), causal=True)
+
+        def dense(q=q, k=k):  # few rows over long keys: split as well
+            return mfa.flash_attn_func(q[:1], k, k)
+        cases += [(paged, paged()), (dense, dense())]
+    torch.cuda.synchronize()
+    wrong, stop = [], threading.Event()
+
+    def work(mine):
+        try:
+            for _ in range(300):
+                if stop.is_set():
+                    return
+                for fn, want in mine:
+                    if not torch.equal(fn(), want):
+                        wrong.append(fn)
+                        stop.set()
+        except BaseException as e:  # shown by the assertion below
+            wrong.append(e)
+            stop.set()
+
+    threads = [threading.Thread(target=work, args=(cases[i::4],)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not wrong
