@@ -448,7 +448,9 @@ int run_sm100(const mfa_fwd_params* p, FwdArgs a, int dev, cudaStream_t st,
     a.o_sb = (int64_t)p->Lq * p->Hq * p->D;
     a.o_ss = (int64_t)p->Hq * p->D;
     a.o_sh = p->D;
-    a.o_vec16 = 0;
+    // 256-byte aligned, and D % 8 == 0 here: every row segment starts on 32 bytes. With 4-byte stores
+    // 2 x 509 rows of 16 heads in two splits took 61 us instead of 45 at D = 128 (the forward alone).
+    a.o_vec16 = 1;
     a.lse = ws_lse;
     a.lse_sb = (int64_t)p->Hq * p->Lq;
     a.lse_sh = p->Lq;
