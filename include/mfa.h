@@ -350,7 +350,7 @@ typedef struct mfa_kv4_fwd_params {
 } mfa_kv4_fwd_params;
 
 /* Attention of the newest Lq rows of every sequence over its cached keys; the semantics of
- * mfa_fwd with Lk = seqlens[b]. A row that sees no key is 0. Up to 64 query rows per KV head (D =
+ * mfa_fwd with Lk = seqlens[b]. A row that sees no key is 0. Up to 48 query rows per KV head (D =
  * 128; 16 at D = 64) read the codes directly; more convert the visible keys and values to 16 bits
  * in the workspace (512 MiB of them at a time, or one sequence's capacity where that is more) and
  * run the tensor-core forward on them. */

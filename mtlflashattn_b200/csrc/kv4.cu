@@ -1373,9 +1373,9 @@ int launch_rows(const Kv4Cache& c, const Kv4Rows& r, int D, cudaStream_t st) {
 // Query rows per KV head up to which the codes are read directly. Each 16 rows read and convert
 // the codes again, while the other way converts them once, to memory, for the tensor-core forward.
 // Measured on B200 (us a call, directly / not) at 32, 48, 64 and 96 rows: 4 x 8192 keys, 32/8
-// heads, D = 128: 42/66, 55/71, 68/69, 99/75; 1 x 32768: 47/75, 61/78, 75/81, 106/89; and at 16 and
-// 32 rows of D = 64, 16 x 2048 keys, 16/16 heads: 43/52, 74/53.
-int64_t direct_rows(int D) { return D == 128 ? 64 : 16; }
+// heads, D = 128: 42/63, 54/66, 68/63, 98/65; 1 x 32768: 47/72, 61/72, 75/73, 106/76; and at 16 and
+// 32 rows of D = 64, 16 x 2048 keys, 16/16 heads: 44/52, 75/53.
+int64_t direct_rows(int D) { return D == 128 ? 48 : 16; }
 
 int check_fwd(const mfa_kv4_cache* c, const mfa_kv4_fwd_params* p) {
   const int rc = check_cache(c);

@@ -297,7 +297,7 @@ def test_row_counts_and_pages(D, Hq, Hkv, Lq, page):
     compare(cache, table, lens, q, causal=True, window=(2**40, -1), sink=10**15)
 
 
-@pytest.mark.parametrize("Hq,Lq", [(64, 1), (65, 1), (16, 4), (13, 5), (1, 49), (7, 9)])
+@pytest.mark.parametrize("Hq,Lq", [(48, 1), (49, 1), (64, 1), (65, 1), (16, 4), (13, 5), (1, 49), (7, 9)])
 def test_rows_around_the_direct_limit(Hq, Lq):
     """The last row counts whose codes are read directly, and the first that go through 16 bits."""
     lens = (1300, Lq, 700)
