@@ -352,11 +352,15 @@ __global__ void __launch_bounds__(kRowThreads) kv4_gather_kernel(const Kv4Cache 
 // wastes nothing, and A comes straight from the 4-bit codes in registers. All operands are fp16:
 // e2m1 codes are exact in it, query rows are scaled by a power of two so that their largest value
 // is below 2^11 (what falls under fp16's range then is 2^-35 of the row's largest), and
-// probabilities lie in [0, 2^7].
+// probabilities lie in [0, 2^15].
 //   scores: the k index of an instruction is one scale group; its fp32 result times the token's
 //           scale is added up, so the key scales cost no rounding.
-//   values: the scale of (token, group) multiplies the probability, in fp16, before the
-//           instruction of that group (its rounding, 2^-11 of each term, is that of fp16 P).
+//   values: the scale of (token, group) multiplies the codes. A code has 2 significant bits and a
+//           scale 4, and their product lies in [2^-10, 2688], so it is exact in fp16.
+// The one rounding to fewer bits than fp32 is that of a probability: 2^-11 of it down to 2^-25 of
+// the largest that its warp has met (fp16's normal numbers), 2^-36 of that largest below. A product
+// of probability and scale leaves fp16's range far sooner: with a first key of value 0 and 8192
+// more of 2^-23 of its weight each, values 0.03 +- 0.02, the output was off by 5 to 7 %, now 0.2 %.
 //
 // A CTA is four consumer warps and a producer warp. The producer copies blocks of 128 tokens (codes
 // and scales, one bulk copy each per page piece) into a ring; each consumer takes two tiles of 16 of
@@ -405,8 +409,8 @@ constexpr int kUnitCost = 2;
 // CTAs per SM: what shared memory and 128 registers per thread allow; two tiles of rows at D = 128
 // take more of both.
 __host__ __device__ constexpr int kv4_ctas(int D, int nt) { return D == 128 && nt == 2 ? 2 : 3; }
-constexpr float kGrow = 7.f;   // a row's reference is renewed when a score passes it by 2^7
-constexpr float kBelow = 3.f;  // and is then set 2^3 below the new maximum
+constexpr float kGrow = 15.f;   // a row's reference is renewed when a score passes it by 2^15
+constexpr float kBelow = 11.f;  // and is then set 2^11 below the new maximum
 
 __device__ __forceinline__ int kv4_pos(const Kv4Args& a, int r) {  // r / group
   return kv4_div(r, a.group_mul, a.group_shift);
@@ -535,6 +539,11 @@ __device__ __forceinline__ uint32_t h2(float lo, float hi) {
 __device__ __forceinline__ uint32_t h2mul(uint32_t a, uint32_t b) {
   const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
   return *reinterpret_cast<const uint32_t*>(&v);
+}
+// All bits set in the halves that are NaN.
+__device__ __forceinline__ uint32_t h2nan(uint32_t a) {
+  const __half2 v = *reinterpret_cast<const __half2*>(&a);
+  return __hneu2_mask(v, v);
 }
 // Untiled bulk copy (no multicast) of n bytes, completing on an mbarrier; both sides 16-byte
 // aligned, n a multiple of 16.
@@ -915,7 +924,8 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(D, NT))
           out.w = two[1];
           reinterpret_cast<uint4*>(v_scale + pair * NG)[half] = out;
           // The NaN scale of a token must not reach a row that does not see it. Such tokens have
-          // probability 0 there, so with finite scales nothing is left to do.
+          // probability 0 there, so with finite scales nothing is left to do. (In an easy block
+          // every row sees every token.)
           if (!easy) clean = !(has_nan_scale(za) || has_nan_scale(zb));
         }
         if (!easy) clean = __all_sync(kFull, clean);
@@ -1055,15 +1065,15 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(D, NT))
       auto values = [&](auto masked) {
 #pragma unroll
         for (int h = 0; h < kWarpTiles; ++h) {
-          uint32_t keep[NT][2];
+          uint32_t poison[NT][2];  // NaN where the row sees the token, else 0
           if constexpr (decltype(masked)::value) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
               for (int e = 0; e < 2; ++e)
-                keep[nt][e] =
-                    transpose8x8((hidden[h] >> (4 * nt + 2 * e) & 1 ? 0u : 0xffffu) |
-                                 (hidden[h] >> (4 * nt + 2 * e + 1) & 1 ? 0u : 0xffff0000u));
+                poison[nt][e] =
+                    transpose8x8((hidden[h] >> (4 * nt + 2 * e) & 1 ? 0u : 0x7fffu) |
+                                 (hidden[h] >> (4 * nt + 2 * e + 1) & 1 ? 0u : 0x7fff0000u));
           }
 #pragma unroll
           for (int w = 0; w < NG / 4; ++w) {  // a word: four groups
@@ -1079,16 +1089,24 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(D, NT))
             const uint32_t sp[4] = {s4.x, s4.y, s4.z, s4.w}, tp[4] = {t4.x, t4.y, t4.z, t4.w};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const uint32_t frag[4] = {va[i], vb[i], vc[i], vd[i]};
+              uint32_t s0 = sp[i], s1 = tp[i];
+              if constexpr (decltype(masked)::value) {
+                // A NaN scale makes NaN of the rows that see its token: of those alone, as a
+                // probability of 0 times a NaN value would be one in every row. It counts as 0
+                // below, and codes (finite) times NaN or 0 are added here.
+                const uint32_t n0 = h2nan(s0), n1 = h2nan(s1);
+                const uint32_t codes[4] = {va[i], vb[i], vc[i], vd[i]};
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                uint32_t p0 = h2mul(pb[h][nt][0], sp[i]), p1 = h2mul(pb[h][nt][1], tp[i]);
-                if constexpr (decltype(masked)::value) {
-                  p0 &= keep[nt][0];
-                  p1 &= keep[nt][1];
-                }
-                mma16816(o[nt][4 * w + i], frag, p0, p1);
+                for (int nt = 0; nt < NT; ++nt)
+                  mma16816(o[nt][4 * w + i], codes, n0 & poison[nt][0], n1 & poison[nt][1]);
+                s0 &= ~n0;
+                s1 &= ~n1;
               }
+              const uint32_t frag[4] = {h2mul(va[i], s0), h2mul(vb[i], s0), h2mul(vc[i], s1),
+                                        h2mul(vd[i], s1)};
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+                mma16816(o[nt][4 * w + i], frag, pb[h][nt][0], pb[h][nt][1]);
             }
           }
         }

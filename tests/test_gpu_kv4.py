@@ -323,6 +323,37 @@ def test_one_long_and_many_short_sequences():
     compare(cache, table, lens, q, causal=True)
 
 
+@pytest.mark.parametrize("Hq,Hkv,B", [(8, 8, 60), (16, 1, 450), (8, 8, 1)])
+@pytest.mark.parametrize("mean,sd", [(0.03, 0.02), (0.1, 0.05), (3.0, 2.0)])
+def test_small_values_beside_a_dominant_key(Hq, Hkv, B, mean, sd):
+    """A first key with most of the weight and the value 0, as sink tokens have it: the output is
+    what the other keys, each of about 2^-23 of its weight, add up to. With the batches one CTA
+    holds a sequence's KV head, and one warp all of what it shares with the first key."""
+    n, D, page = 8192, 128, 64
+    g = torch.Generator(device=DEV).manual_seed(B)
+    cache = mfa.kv4_cache(n // page, page, Hkv, D, DEV)
+    table = torch.arange(n // page, device=DEV).int()[None]
+    one = torch.randn(Hkv, 1, D, device=DEV, generator=g).bfloat16()  # alike in a group's heads
+    q = one.expand(Hkv, Hq // Hkv, D).reshape(1, 1, Hq, D)
+    k = torch.randn(1, n, Hkv, D, device=DEV, generator=g)
+    v = mean + sd * torch.randn(1, n, Hkv, D, device=DEV, generator=g)
+    u = one[:, 0].float()
+    k[0, 0] = u * (16 * D**0.5 / u.square().sum(-1, keepdim=True))  # a logit of 16
+    v[0, 0] = 0
+    mfa.kv4_append(cache, k.bfloat16(), v.bfloat16(), table, i32(0))
+    out = mfa.flash_attn_with_kv4cache(q.expand(B, 1, Hq, D), cache, table.expand(B, -1),
+                                       torch.full((B,), n, dtype=torch.int32, device=DEV))
+    want = ref.attention(q[0], ref.tokens(cache, table[0], n, True),
+                         ref.tokens(cache, table[0], n, False))
+    # Relative to the output, in the 2-norm: 2^-9 of its rounding to bf16; 2^-11 of that of the
+    # probabilities, which are normal fp16 numbers here; 2^-13 and 2^-14 of what moves the first
+    # key's logit and another's (fp32 sums, 2^-17 of sum|q k| / sqrt(D) = 16 and about 7)
+    for b in {0, B // 2, B - 1}:
+        off = (out[b].double() - want).norm() / want.norm()
+        assert off <= 2**-9 + 2**-11 + 2**-13 + 2**-14, (b, off)
+    _kernel.check_device_errors()
+
+
 def test_extreme_queries():
     """Query rows far outside of fp16's range in bf16, zeros, and infinities in one row only."""
     lens = (300,)
