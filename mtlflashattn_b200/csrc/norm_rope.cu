@@ -255,13 +255,16 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 ? 6 : 5)
     const float inv = rsqrtf(fmaf(sum, a.inv_D, a.eps));
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = fmul2(fmul2(x[i], f2pack(inv, inv)), wt[i]);
+    // Dims that do not rotate stay as they are: turned by an angle of 0, one that is not finite
+    // would make NaN of the other of its pair.
     if (!kInterleaved) {  // pairs of pairs: (u0, u1) and (v0, v1) turn by two angles
+      const uint64_t turns = rot0 ? ~0ull : 0ull;  // of the other, nothing is added
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint64_t c = f2pack(cs[2 * i], cs[2 * i + 1]), s = f2pack(sn[2 * i], sn[2 * i + 1]);
         const uint64_t u = x[i], t = x[i + 4];
-        x[i] = fsub2(fmul2(u, c), fmul2(t, s));
-        x[i + 4] = ffma2(u, s, fmul2(t, c));
+        x[i] = fsub2(fmul2(u, c), fmul2(t & turns, s));
+        x[i + 4] = ffma2(u & turns, s, fmul2(t, c));
         f2unpack(x[i], v[2 * i], v[2 * i + 1]);
         f2unpack(x[i + 4], v[8 + 2 * i], v[8 + 2 * i + 1]);
       }
@@ -270,8 +273,9 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 ? 6 : 5)
       for (int i = 0; i < 8; ++i) {
         float u, t;
         f2unpack(x[i], u, t);
-        v[2 * i] = u * cs[i] - t * sn[i];
-        v[2 * i + 1] = u * sn[i] + t * cs[i];
+        const bool turns = i < 4 ? rot0 : rot1;
+        v[2 * i] = u * cs[i] - (turns ? t : 0.f) * sn[i];
+        v[2 * i + 1] = (turns ? u : 0.f) * sn[i] + t * cs[i];
       }
     }
     if (bad)

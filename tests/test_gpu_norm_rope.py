@@ -138,6 +138,34 @@ def test_values_that_are_not_finite_stay_in_their_head():
     assert bool((mfa.qk_norm_rope(zero, zero)[0] == 0).all())
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("D,R", [(128, 0), (128, 64), (64, 32), (128, 40), (48, 24), (96, 96)])
+def test_dims_that_do_not_rotate_stay_alone(interleaved, D, R):
+    """A dim that is not finite after the norm leaves the others that do not rotate as they are,
+    wherever the rows lie in memory."""
+    g = torch.Generator(device=DEV).manual_seed(6)
+    x = torch.randn(1, 4, 3, D, device=DEV, generator=g).bfloat16()
+    w = torch.ones(D, device=DEV)
+    for d in {R, D - 9, D - 1} - {D}:  # (in the last shape: dims that do rotate)
+        w[d] = float("inf")
+    x[0, 1, 2, D - 2] = float("inf")
+    cos, sin = tables(9, R) if R else (None, None)
+    base = torch.zeros(1, 4, 3, D + 3, device=DEV).bfloat16()
+    base[..., 1:1 + D] = x
+    a = mfa.qk_norm_rope(x, x, w, None, cos, sin, interleaved=interleaved)
+    b = mfa.qk_norm_rope(base[..., 1:1 + D], base[..., 1:1 + D], w, None, cos, sin,
+                         interleaved=interleaved)
+    pos = torch.arange(4, device=DEV)[None]
+    for got, odd, weight in zip(a, b, (w, None)):
+        want, _ = formula(x, weight, cos, sin, pos, 1e-6, interleaved)
+        for t in (got, odd):
+            assert torch.equal(t.isnan(), want.isnan())
+            assert torch.equal(t.isinf(), want.isinf())
+        # two kernels whose sums add up in another order: 32 * 2^-24 of what is added, as in
+        # check(), may move a rounding by one step
+        torch.testing.assert_close(got, odd, rtol=2**-7, atol=2**-16, equal_nan=True)
+
+
 def test_empty_refusals_and_gradients():
     q, k = (torch.randn(2, 3, h, 64, device=DEV).half() for h in (4, 2))
     cos, sin = tables(8, 64)
