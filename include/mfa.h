@@ -297,7 +297,8 @@ int mfa_qk_norm_rope(const mfa_norm_rope_params* p, void* cuda_stream);
  * Token t of sequence b is slot t % page_size of page block_table[b][t / page_size]. A page index
  * outside [0, num_pages), or a token outside [0, max_pages * page_size), is never dereferenced:
  * MFA_ERR_INVALID goes to *err, and the token is not written, read back as 0, and left out of the
- * attention or, in calls with many query rows, attended as 0. */
+ * attention or, in calls with many query rows, attended as 0. The attention asks for the pages of
+ * visible tokens only: those that the window has left behind may be given to others. */
 typedef struct mfa_kv4_cache {
   void* k;            /* [num_pages, Hkv, page_size, D/2] bytes, contiguous, 16-byte aligned */
   void* v;

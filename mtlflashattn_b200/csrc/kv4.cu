@@ -104,7 +104,7 @@ struct Kv4Rows {
   int L;
   uint32_t L_mul, L_shift;  // row / L, as kv4_div
   // gather for the 16-bit forward: 1 = only the tokens that its blocks of 128 keys can touch, and
-  // zeros up to the end of a sequence's last block
+  // zeros for those of them that no row sees, which need not have a page
   int visible_only, Lq, wl, sink;
 };
 constexpr int kRowThreads = 128;
@@ -258,16 +258,17 @@ __global__ void __launch_bounds__(kRowThreads) kv4_gather_kernel(const Kv4Cache 
     if (row < all) {
       const int b = kv4_div(row, r.L_mul, r.L_shift), j = row - b * r.L, len = r.lens[b];
       const int64_t t = (int64_t)(r.start != nullptr ? r.start[b] : 0) + j;
-      bool touched = true;
+      bool touched = true, seen = true;
       if (r.visible_only) {
         if (j == 0 && (len < 0 || len > r.L) && h == 0 && !is_v) kv4_report(c);
         const int centre = len - r.Lq;  // of the first row
         const int lo = r.wl >= 0 && centre > r.wl ? centre - r.wl : 0;
         touched = t < ((int64_t)len + 127) / 128 * 128 &&
                   (t >= lo / 128 * 128 || t < ((int64_t)r.sink + 127) / 128 * 128);
+        seen = t >= lo || t < r.sink;
       }
       if (touched) {
-        src = kv4_find(c, b, t, h, t < len);
+        src = kv4_find(c, b, t, h, seen && t < len);
         if (src == -1) kv4_report(c);
         any = 1;
       }
@@ -443,6 +444,10 @@ struct Kv4Span {
   Kv4Range first, last;  // of the tile's first and last row
   int s1, w0, n;
   __device__ __forceinline__ int at(int j) const { return j < s1 ? j : w0 + j - s1; }
+  // whether a row sees one of the tokens [t, t + n)
+  __device__ __forceinline__ bool sees(int t, int n) const {
+    return (t + n > first.lo && t < last.hi) || t < last.sk;
+  }
 };
 template <int kRows>
 __device__ __forceinline__ Kv4Span kv4_span(const Kv4Args& a, int len, int rb) {
@@ -705,8 +710,8 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(D, NT))
     auto page_of = [&](const Kv4Walk<kRows>& w) {  // of the batch that begins at w.j
       const int j = w.j + (lane >> bshift);
       const int t = w.span.at(j) * kBlockTokens + ((lane & ((1 << bshift) - 1)) << pshift);
-      // -2: no token of the sequence is there, and there need not be a page
-      const bool on = w.take > 0 && lane < w.take << bshift && t < w.len;
+      // -2: no row sees a token there, and there need not be a page
+      const bool on = w.take > 0 && lane < w.take << bshift && w.span.sees(t, piece);
       return on ? c.table[(int64_t)w.b * c.table_stride + (t >> c.page_shift)] : -2;
     };
     auto skip = [&](Kv4Walk<kRows>& w) {  // to the next batch

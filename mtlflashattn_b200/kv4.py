@@ -224,7 +224,8 @@ def flash_attn_with_kv4cache(q, cache, block_table, cache_seqlens, softmax_scale
     ``cache_seqlens`` (int32 [B]) counts the keys of each sequence; q holds its newest Lq rows,
     whose keys are appended before the call. Masks, scale, softcap, ALiBi and ``sink_tokens`` are
     those of ``flash_attn_func`` with k and v of length cache_seqlens[b]; a row that sees no key
-    is 0. Returns [B, Lq, Hq, D] in q.dtype.
+    is 0. Pages whose tokens no row sees are not looked at: their entries in ``block_table`` may
+    be anything (-1, or a page that others use by now). Returns [B, Lq, Hq, D] in q.dtype.
     """
     if q.dim() != 4:
         raise ValueError(f"mtlflashattn_b200: expected 4-D [B,S,H,D] q, got q.dim()={q.dim()}")

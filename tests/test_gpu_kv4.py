@@ -427,6 +427,37 @@ def test_bad_tables_and_lengths_are_reported():
     assert bool((out == 0).all())
 
 
+@pytest.mark.parametrize("page", [16, 64, 256])
+@pytest.mark.parametrize("Lq,Hq,D", [(1, 4, 64), (3, 32, 128), (60, 4, 64), (40, 8, 128)])
+@pytest.mark.parametrize("kw", [dict(causal=True, window=(40, -1), sink=5),
+                                dict(causal=True, window=(300, -1), sink=150),
+                                dict(causal=True, window=(17, -1)),
+                                dict(window=(100, 3), sink=20)])
+def test_pages_that_no_row_sees_may_be_missing(page, Lq, Hq, D, kw):
+    """What a window has left behind may have been given back, whichever way the call goes."""
+    lens = (1500, 700, Lq)
+    cache, table, g = filled(lens, page, 2, D, seed=page)
+    q = torch.randn(3, Lq, Hq, D, device=DEV, generator=g).bfloat16()
+    want = compare(cache, table, lens, q, **kw)
+    bare = table.clone()
+    for b, n in enumerate(lens):
+        first, sink = max(0, n - Lq - kw["window"][0]), kw.get("sink", 0)
+        for p in range(table.shape[1]):
+            seen = range(max(p * page, first), min((p + 1) * page, n))
+            if not (len(seen) or p * page < min(sink, n)):
+                bare[b, p] = (-1, cache.num_pages, 2**31 - 1)[p % 3]
+    assert bool((bare != table).any())
+    got = mfa.flash_attn_with_kv4cache(q, cache, bare, i32(*lens), causal=kw.get("causal", False),
+                                       window_size=kw["window"], sink_tokens=kw.get("sink", 0))
+    _kernel.check_device_errors()
+    assert torch.equal(got, want)
+    # one that is seen is still reported
+    bare[0, (lens[0] - 1) // page] = -1
+    mfa.flash_attn_with_kv4cache(q, cache, bare, i32(*lens), causal=kw.get("causal", False),
+                                 window_size=kw["window"], sink_tokens=kw.get("sink", 0))
+    reported()
+
+
 def test_strided_queries_and_empty_batches():
     lens = (50, 33)
     cache, table, g = filled(lens, 16, 2, 64, seed=10)
