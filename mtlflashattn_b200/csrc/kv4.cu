@@ -256,11 +256,13 @@ __global__ void __launch_bounds__(kRowThreads) kv4_gather_kernel(const Kv4Cache 
     const int row = row0 + x;
     int64_t src = -3;  // a row that is not written
     if (row < all) {
-      const int b = kv4_div(row, r.L_mul, r.L_shift), j = row - b * r.L, len = r.lens[b];
+      const int b = kv4_div(row, r.L_mul, r.L_shift), j = row - b * r.L;
+      int len = r.lens[b];
       const int64_t t = (int64_t)(r.start != nullptr ? r.start[b] : 0) + j;
       bool touched = true, seen = true;
       if (r.visible_only) {
         if (j == 0 && (len < 0 || len > r.L) && h == 0 && !is_v) kv4_report(c);
+        len = max(0, min(len, r.L));  // as the forward cuts it: the window hangs on it
         const int centre = len - r.Lq;  // of the first row
         const int lo = r.wl >= 0 && centre > r.wl ? centre - r.wl : 0;
         touched = t < ((int64_t)len + 127) / 128 * 128 &&

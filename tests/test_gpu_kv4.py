@@ -458,6 +458,24 @@ def test_pages_that_no_row_sees_may_be_missing(page, Lq, Hq, D, kw):
     reported()
 
 
+@pytest.mark.parametrize("Lq", [1, 60])
+@pytest.mark.parametrize("window,sink", [((20, -1), 0), ((20, -1), 4), ((200, -1), 0)])
+def test_lengths_past_the_table_under_a_window(Lq, window, sink):
+    """A length beyond the table counts as what the table covers, and the window ends there: the
+    keys that it then shows are this cache's, not what an earlier call left in the workspace."""
+    n = 608
+    cache, table, g = filled((n,), 16, 2, 64, seed=13)
+    other, _, _ = filled((n,), 16, 2, 64, seed=14)
+    q = torch.randn(1, Lq, 4, 64, device=DEV, generator=g).bfloat16()
+    kw = dict(causal=True, window_size=window, sink_tokens=sink)
+    want = mfa.flash_attn_with_kv4cache(q, cache, table, i32(n), **kw)
+    for length in (n + 1, 900, 2**31 - 1):
+        mfa.flash_attn_with_kv4cache(q, other, table, i32(n), **kw)
+        out = mfa.flash_attn_with_kv4cache(q, cache, table, i32(length), **kw)
+        reported()
+        assert torch.equal(out, want)
+
+
 def test_strided_queries_and_empty_batches():
     lens = (50, 33)
     cache, table, g = filled(lens, 16, 2, 64, seed=10)
