@@ -1495,7 +1495,8 @@ Kv4Plan plan_fwd(const mfa_kv4_cache* c, const mfa_kv4_fwd_params* p, int sms) {
   }
   // One wave of resident CTAs, whatever the lengths are.
   k.nt = rows > 8 ? 2 : 1;
-  k.row_blocks = (int)((rows + 8 * k.nt - 1) / (8 * k.nt));
+  // (a table without pages may come with any number of rows: none of them has a place in the line)
+  k.row_blocks = c->max_pages == 0 ? 0 : (int)((rows + 8 * k.nt - 1) / (8 * k.nt));
   k.ctas = sms * kv4_ctas(c->D, k.nt);
   const int64_t parts = 2ll * k.ctas * 8 * k.nt;
   k.o = parts * c->D * 4;

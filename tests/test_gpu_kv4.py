@@ -476,6 +476,25 @@ def test_lengths_past_the_table_under_a_window(Lq, window, sink):
         assert torch.equal(out, want)
 
 
+def test_many_rows_over_a_table_without_pages():
+    """All rows are 0, in time that grows with the rows alone: 4096 x 32 rows write 34 MB, 6 us of
+    a copy; 20 ms is far more than that, and than a launch per row block would take."""
+    cache, table, g = filled((40,), 16, 8, 128, seed=15)
+    q = torch.randn(1, 4096, 32, 128, device=DEV, generator=g).bfloat16()
+    empty = table[:, :0]
+    mfa.flash_attn_with_kv4cache(q, cache, empty, i32(0))
+    start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    start.record()
+    out = mfa.flash_attn_with_kv4cache(q, cache, empty, i32(0), causal=True)
+    end.record()
+    end.synchronize()
+    _kernel.check_device_errors()
+    assert bool((out == 0).all())
+    assert start.elapsed_time(end) < 20
+    mfa.flash_attn_with_kv4cache(q, cache, empty, i32(7))  # a length that no page holds
+    reported()
+
+
 def test_strided_queries_and_empty_batches():
     lens = (50, 33)
     cache, table, g = filled(lens, 16, 2, 64, seed=10)
