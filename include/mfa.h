@@ -336,7 +336,8 @@ int mfa_kv4_gather(const mfa_kv4_cache* c, const mfa_kv4_rows* r, void* cuda_str
 
 typedef struct mfa_kv4_fwd_params {
   const void* q;      /* [B, Lq, Hq, D], 16-byte aligned, last dim stride 1, the other strides
-                         multiples of 8 elements */
+                         multiples of 8 elements (a stride of 0 over more than one element makes
+                         calls with many query rows about 100 times slower) */
   void* o;            /* [B, Lq, Hq, D], 8-byte aligned, strides multiples of 4 elements */
   int64_t q_stride[3];
   int64_t o_stride[3];

@@ -258,6 +258,8 @@ def flash_attn_with_kv4cache(q, cache, block_table, cache_seqlens, softmax_scale
             raise TypeError("mtlflashattn_b200: alibi_slopes must be a tensor of per-head slopes")
         alibi = _broadcast_alibi_slopes(alibi_slopes, B, Hq, dev)
     x = _in_pieces(q)
+    if 0 in x.stride():  # many broadcast rows would run on the CUDA cores: TMA takes no stride of 0
+        x = x.contiguous()
     out = torch.empty(q.shape, dtype=q.dtype, device=dev)
     scale = softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(D)
     far = 2**31 - 1

@@ -397,6 +397,20 @@ def test_what_masked_tokens_hold_does_not_matter():
     assert bool(out[0, 3].isnan().all()) and torch.equal(out[0, 2], good[0, 2])
 
 
+@pytest.mark.parametrize("shape", [(2, 60, 1), (2, 1, 4), (1, 60, 4), (1, 1, 4)])
+def test_broadcast_queries_give_the_same_bits(shape):
+    """Expanded over heads, rows or the batch: the same kernels as for a copy, so the same bits."""
+    lens = (500, 77)
+    cache, table, g = filled(lens, 16, 2, 64, seed=16)
+    for rows in (60, 1):
+        if shape[1] > rows:
+            continue
+        q = torch.randn(*shape, 64, device=DEV, generator=g).bfloat16().expand(2, rows, 4, 64)
+        want = mfa.flash_attn_with_kv4cache(q.contiguous(), cache, table, i32(*lens), causal=True)
+        got = mfa.flash_attn_with_kv4cache(q, cache, table, i32(*lens), causal=True)
+        assert torch.equal(got, want)
+
+
 def test_bad_tables_and_lengths_are_reported():
     lens = (90, 90)
     cache, table, g = filled(lens, 16, 2, 64, seed=9)
