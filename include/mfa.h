@@ -309,7 +309,9 @@ typedef struct mfa_kv4_cache {
   int32_t num_pages, page_size; /* page_size a power of two, 16 .. 1024;
                                    max_pages * page_size <= 2^31 - 4096 */
   int32_t Hkv, D;     /* D 64 or 128 */
-  int32_t B, max_pages;
+  int32_t B, max_pages; /* columns of the table that the call may use: mfa_kv4_fwd with many query
+                           rows takes time and workspace for max_pages * page_size tokens of every
+                           sequence, so pass what the lengths need (table_stride is the table's) */
   float k_unit, v_unit; /* powers of two, 2^-14 .. 2^4 */
   int32_t* err;       /* optional device int */
 } mfa_kv4_cache;

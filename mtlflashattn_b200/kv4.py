@@ -116,8 +116,9 @@ def _check_lens(name, t, B, index):
         raise ValueError("mtlflashattn_b200: all tensors must be on the cache's device")
 
 
-def _pack_cache(cache, block_table, B, dev):
-    """The cache and table as ``mfa_kv4_cache`` in this thread's buffer."""
+def _pack_cache(cache, block_table, B, dev, max_seqlen=None):
+    """The cache and table as ``mfa_kv4_cache`` in this thread's buffer; ``max_seqlen``: only as
+    many of the table's columns as hold that many tokens."""
     if not isinstance(cache, KV4Cache):
         raise TypeError("mtlflashattn_b200: cache must be a KV4Cache")
     k = cache.k
@@ -131,7 +132,7 @@ def _pack_cache(cache, block_table, B, dev):
     if dev.index != index or dev.type != "cuda" or block_table.get_device() != index:
         raise ValueError("mtlflashattn_b200: all tensors must be on the cache's device")
     pages, heads, size, half = k.shape
-    max_pages = table[1]
+    max_pages = table[1] if max_seqlen is None else min(table[1], -(-max_seqlen // size))
     if max_pages * size > 2**31 - 4096:
         raise ValueError("mtlflashattn_b200: block_table covers more than 2^31 - 4096 tokens")
     stride = block_table.stride()
@@ -143,6 +144,11 @@ def _pack_cache(cache, block_table, B, dev):
         cache.v_scale.data_ptr(), block_table.data_ptr(), stride[0], pages, size, heads, 2 * half,
         B, max_pages, cache.k_unit, cache.v_unit, _kernel._err_ptr(dev))
     return p
+
+
+def _check_max_seqlen(n):
+    if not isinstance(n, int) or isinstance(n, bool) or n < 0:
+        raise ValueError("mtlflashattn_b200: max_seqlen must be an int >= 0")
 
 
 def _in_pieces(t):
@@ -201,8 +207,7 @@ def kv4_gather(cache, block_table, cache_seqlens, max_seqlen, starts=None, dtype
     """
     if dtype not in _DTYPES:
         raise NotImplementedError(f"mtlflashattn_b200: dtype {dtype} (fp16/bf16/fp32)")
-    if not isinstance(max_seqlen, int) or isinstance(max_seqlen, bool) or max_seqlen < 0:
-        raise ValueError("mtlflashattn_b200: max_seqlen must be an int >= 0")
+    _check_max_seqlen(max_seqlen)
     B, dev = block_table.shape[0], block_table.device
     c = _pack_cache(cache, block_table, B, dev)
     _check_lens("cache_seqlens", cache_seqlens, B, dev.index)
@@ -218,7 +223,7 @@ def kv4_gather(cache, block_table, cache_seqlens, max_seqlen, starts=None, dtype
 
 def flash_attn_with_kv4cache(q, cache, block_table, cache_seqlens, softmax_scale=None,
                              causal=False, window_size=(-1, -1), softcap=0.0, alibi_slopes=None,
-                             sink_tokens=0):
+                             sink_tokens=0, max_seqlen=None):
     """Attention of q [B, Lq, Hq, D] (fp16/bf16) over the cached keys and values (forward only).
 
     ``cache_seqlens`` (int32 [B]) counts the keys of each sequence; q holds its newest Lq rows,
@@ -226,6 +231,13 @@ def flash_attn_with_kv4cache(q, cache, block_table, cache_seqlens, softmax_scale
     those of ``flash_attn_func`` with k and v of length cache_seqlens[b]; a row that sees no key
     is 0. Pages whose tokens no row sees are not looked at: their entries in ``block_table`` may
     be anything (-1, or a page that others use by now). Returns [B, Lq, Hq, D] in q.dtype.
+
+    ``max_seqlen``, an int that no length exceeds (None: the tokens that ``block_table`` has
+    columns for). More than 48 query rows per KV head (16 at D = 64) are attended by way of keys and
+    values in 16 bits: time and workspace of such calls follow this bound, not the lengths, so give
+    it where the table is much wider than they are (the workspace, up to 512 MiB or one sequence's
+    bound where that is more, is kept for the stream's next calls). A longer sequence is cut after the page of
+    the bound's last token and reported by ``check_device_errors``.
     """
     if q.dim() != 4:
         raise ValueError(f"mtlflashattn_b200: expected 4-D [B,S,H,D] q, got q.dim()={q.dim()}")
@@ -241,11 +253,13 @@ def flash_attn_with_kv4cache(q, cache, block_table, cache_seqlens, softmax_scale
     if not softcap >= 0:
         raise ValueError("mtlflashattn_b200: softcap must be >= 0 (0 disables capping)")
     sink = _check_sink(sink_tokens)
+    if max_seqlen is not None:
+        _check_max_seqlen(max_seqlen)
     if q.dtype not in (torch.float16, torch.bfloat16):
         raise NotImplementedError(f"mtlflashattn_b200: dtype {q.dtype} (fp16/bf16)")
     B, Lq, Hq, D = q.shape
     dev = q.device
-    c = _pack_cache(cache, block_table, B, dev)
+    c = _pack_cache(cache, block_table, B, dev, max_seqlen)
     Hkv = cache.num_heads_kv
     if D != cache.head_dim:
         raise ValueError("mtlflashattn_b200: q does not have the cache's head_dim")

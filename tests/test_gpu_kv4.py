@@ -509,6 +509,38 @@ def test_many_rows_over_a_table_without_pages():
     reported()
 
 
+@pytest.mark.parametrize("Lq,Hq,D", [(1, 4, 64), (100, 8, 64), (200, 4, 128)])
+def test_wide_tables_and_a_bound_of_the_lengths(Lq, Hq, D):
+    """With a bound, a table as wide as the longest context asks for no more workspace than a
+    narrow one, and gives the same bits; a longer sequence is cut at the bound's page and
+    reported."""
+    lens = (700, 256, 0)
+    cache, table, g = filled(lens, 16, 2, D, seed=17)
+    q = torch.randn(3, Lq, Hq, D, device=DEV, generator=g).bfloat16()
+    wide = torch.full((3, 2**17 // 16), -1, dtype=torch.int32, device=DEV)
+    wide[:, :table.shape[1]] = table
+    sizes = []  # of the workspaces of streams that make no other call
+    kw = dict(causal=True, window_size=(400, -1), sink_tokens=3)
+    for t, bound in ((table, None), (wide, 700), (wide, table.shape[1] * 16)):
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            out = mfa.flash_attn_with_kv4cache(q, cache, t, i32(*lens), max_seqlen=bound, **kw)
+            sizes.append(_kernel._workspaces.pop((q.device, side.cuda_stream)).numel())
+        side.synchronize()
+        if bound is None:
+            want = out
+        assert torch.equal(out, want)
+    assert sizes[0] == sizes[1] == sizes[2] < 16 << 20
+    compare(cache, wide, lens, q, causal=True, window=(400, -1), sink=3)
+    _kernel.check_device_errors()
+    cut = mfa.flash_attn_with_kv4cache(q, cache, wide, i32(700, 256, 0), max_seqlen=600, **kw)
+    reported()
+    assert torch.equal(cut, mfa.flash_attn_with_kv4cache(q, cache, table, i32(608, 256, 0), **kw))
+    assert bool((mfa.flash_attn_with_kv4cache(q, cache, wide, i32(0, 0, 0), max_seqlen=0) == 0).all())
+    _kernel.check_device_errors()
+
+
 def test_strided_queries_and_empty_batches():
     lens = (50, 33)
     cache, table, g = filled(lens, 16, 2, 64, seed=10)

@@ -116,6 +116,16 @@ def test_argument_refusals(call, exc):
         call(c, torch.zeros(2, 2, dtype=torch.int32), torch.zeros(2, dtype=torch.int32))
 
 
+@pytest.mark.parametrize("bad", [-1, 2.0, True, "9"])
+def test_bounds_of_the_lengths_are_refused(bad):
+    c = mfa.kv4_cache(3, 16, 2, 64, "cpu")
+    table, n = torch.zeros(2, 2, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="max_seqlen"):
+        mfa.flash_attn_with_kv4cache(rows(), c, table, n, max_seqlen=bad)
+    with pytest.raises(ValueError, match="max_seqlen"):
+        mfa.kv4_gather(c, table, n, bad)
+
+
 def cache_params(**kw):
     c = _lib.MfaKv4Cache(k=16, v=16, k_scale=16, v_scale=16, block_table=4, table_stride=1,
                          num_pages=1, page_size=16, Hkv=2, D=64, B=1, max_pages=1, k_unit=1.0,
