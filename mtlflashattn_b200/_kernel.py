@@ -140,7 +140,8 @@ def _err_word(device):
 
 def _err_ptr(device):
     """Address of the device's error word; 0 where the first call of all is being captured: a word
-    made then would be zeroed by every replay, and hold anything before the first."""
+    made then would be zeroed by every replay, and hold anything before the first. Such a graph
+    reports nothing."""
     if device not in _err_words and torch.cuda.is_current_stream_capturing():
         return 0
     return _err_word(device).data_ptr()

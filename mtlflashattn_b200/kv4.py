@@ -75,6 +75,8 @@ class KV4Cache:
                 "mtlflashattn_b200: k_unit and v_unit must be powers of two from 2^-14 to 2^4")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.k_unit, self.v_unit = float(k_unit), float(v_unit)
+        if k.is_cuda:
+            _kernel._err_ptr(dev)  # there before a first call that may be captured
 
     @property
     def num_pages(self):

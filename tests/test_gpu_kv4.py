@@ -697,6 +697,40 @@ def test_first_call_of_a_process_captured():
     assert r.returncode == 0 and "same" in r.stdout, r.stdout[-1000:] + r.stderr[-3000:]
 
 
+def test_a_first_call_that_is_captured_still_reports():
+    """Nothing but the cache was made before the capture."""
+    import os
+    import subprocess
+    import sys
+    import textwrap
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = textwrap.dedent("""
+        import torch, mtlflashattn_b200 as mfa
+        from mtlflashattn_b200 import _kernel, _lib
+        cache = mfa.kv4_cache(8, 16, 2, 64, "cuda")
+        table = torch.arange(4, device="cuda").int().view(1, 4)
+        n = torch.tensor([50], dtype=torch.int32, device="cuda")
+        q = torch.zeros(1, 1, 4, 64, device="cuda").half()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = mfa.flash_attn_with_kv4cache(q, cache, table, n, causal=True)
+        g.replay()
+        _kernel.check_device_errors("cuda")
+        table[0, 1] = 8
+        g.replay()
+        try:
+            _kernel.check_device_errors("cuda")
+        except _lib.MfaError:
+            print("told")
+        table[0, 1] = 1
+        g.replay()
+        _kernel.check_device_errors("cuda")
+    """)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=root,
+                       timeout=300)
+    assert r.returncode == 0 and "told" in r.stdout, r.stdout[-1000:] + r.stderr[-3000:]
+
+
 def test_two_threads_on_two_streams():
     import threading
     cache, table, g = filled((5000,), 64, 2, 64, seed=12)
