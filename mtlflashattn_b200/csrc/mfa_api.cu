@@ -127,13 +127,17 @@ int sm100_gen(const mfa_fwd_params* p) {
 }
 int sm100_tiles_rt(bool wide, int gen);
 bool sm100_sink(const mfa_fwd_params* p) { return p->sink > 0 && p->win_left >= 0; }
-// First visible keys and a short window: one-tile CTAs also at D = 128. A 128-row tile walks a
-// block less than a 256-row pair, its blocks at the window's ends are masked while the other CTA of
-// the SM computes, and the shorter CTAs fill the last wave better; a long window would rather
-// fetch each K/V block once for two tiles. B200, 16 heads, L = 8192, one tile / two: window 128
-// 56 / 66 us, 1024 107 / 111, 4096 231 / 216.
+// First visible keys and a short walk (the window and those keys): one-tile CTAs also at D = 128. A
+// 128-row tile walks a block less than a 256-row pair, its blocks at the window's ends are masked
+// while the other CTA of the SM computes, and the shorter CTAs fill the last wave better; a long
+// walk would rather fetch each K/V block once for two tiles. B200, 16 heads, us with one tile /
+// two, window + first keys, L = 8192 and 16384 (4 KV heads): 100 + 4 56 / 68 and 115 / 127, 1024 +
+// 4 102 / 109 and 223 / 226, 1024 + 500 116 / 125 and 263 / 263, 100 + 2000 139 / 136 and 296 / 297,
+// 2500 + 4 166 / 153 and 354 / 346, 4095 + 4 214 / 198 and 504 / 450, 100 + 8000 247 / 227 and 736 / 678.
 bool sm100_sink_one(const mfa_fwd_params* p) {
-  return sm100_sink(p) && p->win_left < 2048 && (p->causal || p->win_right >= 0);
+  const int lk = p->cu_q != nullptr ? p->max_lk : p->Lk;
+  return sm100_sink(p) && (int64_t)p->win_left + std::min(p->sink, lk) < 2048 &&
+         (p->causal || p->win_right >= 0);
 }
 
 // Query heads packed per KV head (log2; 0 = none). Decode-like launches (fewer than 128 query
@@ -200,7 +204,8 @@ SplitPlan plan_splits(const mfa_fwd_params* p, int sms) {
   const int64_t ctas = row_blocks * (p->Hq >> ps) * p->B;
   const int64_t key_blocks = (lk + 127) / 128;
   // kSink: an even share of a short window is worth a CTA from 4 blocks on (4 x 1 x 16384, 64/8
-  // heads, window 4095: 31 us with 4 splits of 8 blocks, 28 with 8 of 4)
+  // heads, a captured call: window 1023 20.0 us with 8 blocks at least, 16.5 with 4; 4095, 4 splits
+  // of up to 9 blocks 23.7 us, 7 of up to 5 21.8)
   const int64_t least = sm100_sink(p) ? 4 : MFA_SPLIT_MIN_BLOCKS;
   int64_t s = (slots - slots / 8) / ctas;
   s = s < key_blocks / least ? s : key_blocks / least;

@@ -93,6 +93,22 @@ def test_key_split_of_long_decode():
         check(out, formula(q, k, v, True, (1000, -1), sink), torch.bfloat16)
 
 
+@pytest.mark.parametrize("window,sink", [(2040, 7), (2040, 8), (100, 1947), (100, 1948), (60, 9000),
+                                         (2500, 3)])
+@pytest.mark.parametrize("Hq,Hkv,softcap", [(2, 2, 0.0), (4, 1, 20.0)])
+def test_walks_around_the_tile_rule(window, sink, Hq, Hkv, softcap):
+    """Window and first keys together decide between CTAs of one and of two tiles at D = 128."""
+    q, k, v = inputs(1, 2900, 2900, Hq, Hkv, 128, torch.bfloat16, seed=window + sink)
+    out = mfa.flash_attn_func(q, k, v, causal=True, window_size=(window, -1), softcap=softcap,
+                              sink_tokens=sink)
+    check(out, formula(q, k, v, True, (window, -1), sink, softcap), torch.bfloat16, softcap)
+    lens = torch.tensor([0, 2900], device="cuda").int()
+    flat = mfa.flash_attn_varlen_func(q[0], k[0], v[0], lens, lens, 2900, 2900, causal=True,
+                                      window_size=(window, -1), softcap=softcap, sink_tokens=sink)
+    check(flat[None], formula(q, k, v, True, (window, -1), sink, softcap), torch.bfloat16, softcap)
+    _kernel.check_device_errors()
+
+
 def test_varlen_sequences_have_their_own_first_tokens():
     lens_q, lens_k = [1, 300, 0, 77, 500], [400, 300, 9, 77, 513]
     cq = torch.tensor([0, *lens_q], device="cuda").cumsum(0).to(torch.int32)
