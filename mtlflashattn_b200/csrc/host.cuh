@@ -15,7 +15,9 @@ namespace mfa {
 
 // ------------------------------------------------------------------ host fault injection
 // MFA_FAULT=<site>[,<site>...] makes the named entry point fail before it launches anything,
-// so callers' error handling can be tested without touching a GPU. Sites: fwd, combine.
+// so callers' error handling can be tested without touching a GPU. Sites: fwd (every
+// form of the forward), combine (the merges), kv4 (append, gather and attention of the 4-bit
+// cache), norm_rope.
 inline bool fault_injected(const char* site) {
   const char* env = std::getenv("MFA_FAULT");
   if (env == nullptr || *env == 0) return false;

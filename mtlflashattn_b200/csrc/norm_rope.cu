@@ -301,14 +301,14 @@ void launch_vec(const NormRopeArgs& a, int64_t warps, cudaStream_t st) {
 }
 
 template <typename T>
-int launch_norm_rope(NormRopeArgs a, bool vec, cudaStream_t st) {
+int launch_norm_rope(NormRopeArgs a, bool vec, int sms, cudaStream_t st) {
   const int64_t tokens = (int64_t)a.B * a.L;
   const int H = a.Hq + a.Hkv;
   const int rows = a.D > 64 ? 4 : a.D > 32 ? 8 : 16;  // heads a warp holds at once
   // few tokens: spread each one's heads over warps until every SM has 16
   a.segments = 1;
   const int most = (a.Hq + rows - 1) / rows + (a.Hkv + rows - 1) / rows;
-  while (a.segments < most && tokens * a.segments < 148 * 16) ++a.segments;
+  while (a.segments < most && tokens * a.segments < 16 * sms) ++a.segments;
   const int64_t warps = vec ? tokens * a.segments : tokens * H;
   if (warps >= (1ll << 31)) return MFA_ERR_UNSUPPORTED;
   if (!vec) norm_rope_any<T><<<(unsigned)((warps + 3) / 4), 128, 0, st>>>(a);
@@ -364,9 +364,12 @@ extern "C" int mfa_qk_norm_rope(const mfa_norm_rope_params* p, void* stream) {
   a.w_vec = mfa::aligned16(p->q_weight) && mfa::aligned16(p->k_weight);
   a.rot_vec = mfa::aligned16(p->cos) && mfa::aligned16(p->sin) && p->cos_stride * rs % 16 == 0 &&
               p->sin_stride * rs % 16 == 0;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return MFA_ERR_NO_DEVICE;
+  const int sms = mfa::dev_info(dev).sms;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   (void)cudaGetLastError();
-  if (p->dtype == MFA_FP32) return mfa::launch_norm_rope<float>(a, vec, st);
-  if (p->dtype == MFA_BF16) return mfa::launch_norm_rope<__nv_bfloat16>(a, vec, st);
-  return mfa::launch_norm_rope<__half>(a, vec, st);
+  if (p->dtype == MFA_FP32) return mfa::launch_norm_rope<float>(a, vec, sms, st);
+  if (p->dtype == MFA_BF16) return mfa::launch_norm_rope<__nv_bfloat16>(a, vec, sms, st);
+  return mfa::launch_norm_rope<__half>(a, vec, sms, st);
 }
