@@ -164,7 +164,9 @@ __global__ void __launch_bounds__(128) norm_rope_any(const __grid_constant__ Nor
 // worked on. Per value there are few bytes and many instructions: the arithmetic is in
 // packed pairs and the registers are kept at 80 for 16-bit rows (16384 tokens, 32/8 heads, D = 128,
 // bf16: 65 us, 5.3 TB/s; with scalar arithmetic 77; 64 registers: 82).
-template <typename T, bool kInterleaved, int LP>
+// kAll: R = D, every dim rotates, so none has to be kept out of its pair's rotation (66.3 us for
+// that case with three sets of inputs in turn; 67.9 without the distinction).
+template <typename T, bool kInterleaved, bool kAll, int LP>
 __global__ void __launch_bounds__(128, sizeof(T) == 2 ? 6 : 5)
     norm_rope_vec(const __grid_constant__ NormRopeArgs a) {
   constexpr int kRows = 32 / LP;  // heads a warp holds at once
@@ -177,7 +179,7 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 ? 6 : 5)
   const int pairs = kInterleaved ? 0 : a.R / 16;  // leading lanes whose chunks rotate together
   const int c0 = 8 * (kInterleaved || sub >= pairs ? 2 * sub : sub);
   const int c1 = kInterleaved || sub >= pairs ? c0 + 8 : c0 + a.R / 2;
-  const bool rot0 = active && c0 < a.R, rot1 = active && c1 < a.R;
+  const bool rot0 = kAll || (active && c0 < a.R), rot1 = kAll || (active && c1 < a.R);
   const int gq = (a.Hq + kRows - 1) / kRows, all = gq + (a.Hkv + kRows - 1) / kRows;
   const int per = (all + a.segments - 1) / a.segments;
   const int g_end = min(all, (seg + 1) * per);
@@ -207,10 +209,10 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 ? 6 : 5)
     // the angles of the lane's 8 pairs stand side by side; interleaved, the last lane that
     // rotates may have 4 of them
     const int p = kInterleaved ? c0 / 2 : c0;
-    if (rot0 && (rot1 || !kInterleaved)) {
+    if (active && rot0 && (rot1 || !kInterleaved)) {
       load_eight<T>(a.cos, row * a.cos_row + p, a.rot_fp32, a.rot_vec, cs);
       load_eight<T>(a.sin, row * a.sin_row + p, a.rot_fp32, a.rot_vec, sn);
-    } else if (rot0) {
+    } else if (active && rot0) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         cs[i] = load_any<T>(a.cos, row * a.cos_row + p + i, a.rot_fp32);
@@ -292,12 +294,12 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 ? 6 : 5)
   }
 }
 
-template <typename T, bool kInterleaved>
+template <typename T, bool kInterleaved, bool kAll>
 void launch_vec(const NormRopeArgs& a, int64_t warps, cudaStream_t st) {
   const unsigned blocks = (unsigned)((warps + 3) / 4);
-  if (a.D > 64) norm_rope_vec<T, kInterleaved, 8><<<blocks, 128, 0, st>>>(a);
-  else if (a.D > 32) norm_rope_vec<T, kInterleaved, 4><<<blocks, 128, 0, st>>>(a);
-  else norm_rope_vec<T, kInterleaved, 2><<<blocks, 128, 0, st>>>(a);
+  if (a.D > 64) norm_rope_vec<T, kInterleaved, kAll, 8><<<blocks, 128, 0, st>>>(a);
+  else if (a.D > 32) norm_rope_vec<T, kInterleaved, kAll, 4><<<blocks, 128, 0, st>>>(a);
+  else norm_rope_vec<T, kInterleaved, kAll, 2><<<blocks, 128, 0, st>>>(a);
 }
 
 template <typename T>
@@ -312,8 +314,10 @@ int launch_norm_rope(NormRopeArgs a, bool vec, int sms, cudaStream_t st) {
   const int64_t warps = vec ? tokens * a.segments : tokens * H;
   if (warps >= (1ll << 31)) return MFA_ERR_UNSUPPORTED;
   if (!vec) norm_rope_any<T><<<(unsigned)((warps + 3) / 4), 128, 0, st>>>(a);
-  else if (a.interleaved) launch_vec<T, true>(a, warps, st);
-  else launch_vec<T, false>(a, warps, st);
+  else if (a.R == a.D)
+    (a.interleaved ? launch_vec<T, true, true> : launch_vec<T, false, true>)(a, warps, st);
+  else
+    (a.interleaved ? launch_vec<T, true, false> : launch_vec<T, false, false>)(a, warps, st);
   return cudaGetLastError() == cudaSuccess ? MFA_OK : MFA_ERR_CUDA;
 }
 
