@@ -83,7 +83,8 @@ __global__ void __launch_bounds__(simt::kThreads) fa_fwd_simt(const __grid_const
 #pragma unroll
   for (int c = 0; c < NC; ++c) acc[c] = 0.f;
 
-  // the window's key blocks, and before them those of the first keys that stay visible
+  // the window's key blocks, and before them those of the first keys that stay visible (fp32, 1 x 4096,
+  // 8 heads, D = 128, window 512 + 4: 932 us, 909 without the first keys)
   const int kw0 = khi > klo ? (klo / BN) * BN : (klo + BN - 1) / BN * BN;
   const int sk_last = min(key_range(a, sv, r_last).sk, kw0);
   const int kend = khi > klo ? khi : sk_last;

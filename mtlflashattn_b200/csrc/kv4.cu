@@ -91,9 +91,9 @@ __device__ __forceinline__ int kv4_div(int x, uint32_t mul, uint32_t shift) {
 }
 
 // ------------------------------------------------------------------ append and gather
-// 16-bit rows on one side, 0.28 of their bytes on the other; issue slots bound both (76 % of them
-// taken in the append, 61 % in the gather) before memory does. B200, 2 x 8192 tokens, 8 heads,
-// D = 128, bf16: append 20.6 us (4.2 TB/s), gather 15.6 us (5.5 TB/s). A CTA takes
+// 16-bit rows on one side, 0.28 of their bytes on the other; the append is bound by issue (74 % of
+// the slots taken), the gather (61 %) by nothing alone. B200, 2 x 8192 tokens, 8 heads,
+// D = 128, bf16: append 20.6 us (4.2 TB/s), gather 15.4 us (5.6 TB/s). A CTA takes
 // a tile of 4096 codes of one head (32 rows of D = 128, 64 of D = 64), keys or values, through
 // shared memory, where the layout's permutation happens, so that every access to memory is 16
 // bytes of a row; rows are (sequence, token) pairs in one line and look up their pages themselves.
@@ -373,10 +373,12 @@ __global__ void __launch_bounds__(kRowThreads) kv4_gather_kernel(const Kv4Cache 
 // shares. A share that covers a whole unit writes its rows; one that does not leaves a partial
 // result, and kv4_join adds those up. Lengths are read on the device.
 //
-// What bounds it is issue and the ALU pipe (55 % and 48 % busy), which converts the codes, before
-// memory. B200: 1 x 1 x 131072 tokens, 64/8 heads, D = 128: 38 us, 4.0 TB/s of codes and scales (62 %
-// of a copy's rate); 32 x 1 x up to 8192, 32/8 heads: 40 us; 1 x 1 x 4096: 7.4 us. The copies alone
-// took 21 us for the first, from L2. Eight warps of one tile instead of four of two: 51 us.
+// What bounds it is latency: no pipe is full (issue 57 %, ALU, which converts the codes, 46 %, tensor
+// 22 %, memory 57 % of a copy's rate), and 13 warps per SM wait for each other's loads and results.
+// B200, this kernel: 1 x 1 x 131072 tokens, 64/8 heads, D = 128: 39 us, 3.9 TB/s of codes and scales
+// (60 % of a copy's rate); 32 x 1 x up to 8192, 32/8 heads: 42 us; 1 x 1 x 4096: 7.5 us. An earlier
+// form's copies alone took 21 us for the first, from L2; with eight warps of one tile it took 51 us,
+// not 43.
 struct Kv4Args {
   Kv4Cache c;
   const void* q;
@@ -403,11 +405,12 @@ constexpr int kWarpTiles = 2;  // tiles of 16 tokens that a consumer takes of a 
 constexpr int kBlockTokens = 16 * kWarpTiles * kAttnWarps;
 constexpr int kBlockTiles = kBlockTokens / 16;
 constexpr int kAttnStages = 3;
-// Blocks per CTA at least: more leave SMs idle in short calls. 1 x 1 x 4096, 32/8 heads, attention
-// kernel with 2 / 4 / 8 blocks: 7.4 / 8.7 / 11.8 us; 1 x 1 x 16384: 10.3 / 11.6 / 14.4.
+// Blocks per CTA at least: more leave SMs idle in short calls. 1 x 1 x 4096, 32/8 heads, a captured
+// call with 2 / 4 / 8 blocks: 10.2 / 11.5 / 14.5 us; 1 x 1 x 16384: 14.5 / 15.1 / 17.7.
 constexpr int kMinShare = 2;
-// Beginning and ending a unit takes about as long as so many blocks. 32 x 1 x up to 8192, a call
-// with 2 / 3 / 4: 47.5 / 48.5 / 47.7 us; 8 x 1 x 26000: 44.0 / 45.6 / 45.6.
+// Beginning and ending a unit takes about as long as so many blocks. A captured call with 2 / 3 / 4:
+// 32 x 1 x up to 8192 48.7 / 46.7 / 48.0 us, 8 x 1 x up to 26000 54.0 / 53.6 / 53.8, 4 x 8 x 8192 47.1 /
+// 46.6 / 46.5, 1 x 8 x 32768 42.1 / 41.9 / 44.0 (32/8 heads): flat, within what the lengths make of it.
 constexpr int kUnitCost = 2;
 // CTAs per SM: what shared memory and 128 registers per thread allow; two tiles of rows at D = 128
 // take more of both.
@@ -1187,7 +1190,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas(D, NT))
 // Adds up the partial results of a row: one block per output row. Rows that one CTA finished are
 // left as they are; rows without visible keys become 0. The parts' weights are made first, all at
 // once, so that the long loop only loads and adds. Launched while kv4_attn still runs, it finds its
-// parts before the last CTAs end; 1 x 1 x 131072: a call takes 43.7 us, kv4_attn 38.0 of them.
+// parts before the last CTAs end; 1 x 1 x 131072: a captured call takes 42.8 us, kv4_attn 39.2.
 constexpr int kJoinThreads = 256;
 constexpr int kJoinParts = 512;  // weights held at a time
 template <int D, int NT>
@@ -1397,9 +1400,9 @@ int launch_rows(const Kv4Cache& c, const Kv4Rows& r, int D, cudaStream_t st) {
 
 // Query rows per KV head up to which the codes are read directly. Each 16 rows read and convert
 // the codes again, while the other way converts them once, to memory, for the tensor-core forward.
-// Measured on B200 (us a call, directly / not) at 32, 48, 64 and 96 rows: 4 x 8192 keys, 32/8
-// heads, D = 128: 42/63, 54/66, 68/63, 98/65; 1 x 32768: 47/72, 61/72, 75/73, 106/76; and at 16 and
-// 32 rows of D = 64, 16 x 2048 keys, 16/16 heads: 44/52, 75/53.
+// Measured on B200 (us a captured call, directly / not) at 32, 48, 64 and 96 rows: 4 x 8192 keys, 32/8
+// heads, D = 128: 47/69, 65/72, 80/69, 117/70; 1 x 32768: 42/68, 56/68, 70/68, 102/72; and at 16 and
+// 32 rows of D = 64, 16 x 2048 keys, 16/16 heads: 51/67, 87/67.
 int64_t direct_rows(int D) { return D == 128 ? 48 : 16; }
 
 int check_fwd(const mfa_kv4_cache* c, const mfa_kv4_fwd_params* p) {

@@ -105,7 +105,9 @@ __device__ __forceinline__ void load_eight(const void* p, int64_t i, int fp32, i
   }
 }
 
-// Any head dim, strides and rotation width: one warp per head row, one value per lane and step.
+// Any head dim, strides and rotation width: one warp per head row, one value per lane and step. Not
+// made for speed: 16384 tokens, 32/8 heads, bf16, D = 128 in unaligned rows 365 us (0.94 TB/s), D = 80
+// with R = 40 in split halves 296 us (the vector kernel, interleaved: 57).
 template <typename T>
 __global__ void __launch_bounds__(128) norm_rope_any(const __grid_constant__ NormRopeArgs a) {
   const int H = a.Hq + a.Hkv;
@@ -163,7 +165,7 @@ __global__ void __launch_bounds__(128) norm_rope_any(const __grid_constant__ Nor
 // token's cosines and sines in registers; the next group's rows are on their way while one is
 // worked on. Per value there are few bytes and many instructions: the arithmetic is in
 // packed pairs and the registers are kept at 80 for 16-bit rows (16384 tokens, 32/8 heads, D = 128,
-// bf16: 65 us, 5.3 TB/s; with scalar arithmetic 77; 64 registers: 82).
+// bf16: 65 us, 5.3 TB/s; with scalar arithmetic 77; 64 registers: 82; fp32 106 us, 6.4 TB/s).
 // kAll: R = D, every dim rotates, so none has to be kept out of its pair's rotation (66.3 us for
 // that case with three sets of inputs in turn; 67.9 without the distinction).
 template <typename T, bool kInterleaved, bool kAll, int LP>
