@@ -411,6 +411,35 @@ def test_broadcast_queries_give_the_same_bits(shape):
         assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("D,Hq,Hkv", [(64, 4, 2), (64, 4, 1), (128, 2, 1), (128, 8, 2), (128, 12, 1)])
+@pytest.mark.parametrize("page", [16, 128])
+def test_nan_values_reach_their_dims_of_the_rows_that_see_them(D, Hq, Hkv, page):
+    """A NaN among a token's values (its keys are finite) makes NaN of the 16 dims that share its
+    scale, in the rows that see it; all else is as if it were not there."""
+    n, Lq = 300, 4
+    g = torch.Generator(device=DEV).manual_seed(18)
+    table, pages = table_of(1, -(-n // page))
+    cache = dirty(mfa.kv4_cache(pages, page, Hkv, D, DEV))
+    k, v = (torch.randn(1, n, Hkv, D, device=DEV, generator=g).bfloat16() for _ in range(2))
+    mfa.kv4_append(cache, k, v, table, i32(0))
+    q = torch.randn(1, Lq, Hq, D, device=DEV, generator=g).bfloat16()
+    kw = dict(causal=True, window=(60, -1), sink=130)
+    good = compare(cache, table, (n,), q, **kw)
+    # the newest token but one: two rows see it; the oldest of the window: one; hidden; first keys
+    for token in (n - 2, n - Lq - 60, 200, 5):
+        bad = v.clone()
+        bad[0, token, 0, 33] = float("nan")
+        mfa.kv4_append(cache, k, bad, table, i32(0))
+        out = compare(cache, table, (n,), q, **kw)  # the oracle leaves out what is hidden
+        rows = [i for i in range(Lq) if token <= n - Lq + i
+                and (token >= n - Lq + i - 60 or token < 130)]
+        touched = torch.zeros(1, Lq, Hq, D, dtype=torch.bool, device=DEV)
+        touched[0, rows, :Hq // Hkv, 32:48] = True
+        assert bool(out[touched].isnan().all())
+        assert torch.equal(out[~touched], good[~touched])
+    _kernel.check_device_errors()
+
+
 def test_bad_tables_and_lengths_are_reported():
     lens = (90, 90)
     cache, table, g = filled(lens, 16, 2, 64, seed=9)
