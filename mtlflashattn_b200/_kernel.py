@@ -133,8 +133,8 @@ _err_words = {}
 def _err_word(device):
     t = _err_words.get(device)
     if t is None:
-        t = torch.zeros(1, dtype=torch.int32, device=device)
-        _err_words[device] = t
+        # of two threads that come here at once, both get the word that the first put there
+        t = _err_words.setdefault(device, torch.zeros(1, dtype=torch.int32, device=device))
     return t
 
 

@@ -50,6 +50,30 @@ def test_packed_fields_land_where_the_struct_has_them():
     assert _lib.MfaKv4FwdParams.workspace.offset == _lib.KV4_FWD_WORKSPACE_OFFSET
 
 
+def test_two_threads_share_the_error_word(monkeypatch):
+    """A word that one thread's launch points at must not be replaced by another's."""
+    import threading
+
+    from mtlflashattn_b200 import _kernel
+    meet = threading.Barrier(2, timeout=20)
+    zeros = torch.zeros
+
+    def both_at_once(*args, **kw):
+        meet.wait()
+        return zeros(*args, **kw)
+
+    monkeypatch.setattr(_kernel, "_err_words", {})
+    monkeypatch.setattr(_kernel.torch, "zeros", both_at_once)
+    got = []
+    threads = [threading.Thread(target=lambda: got.append(_kernel._err_word(torch.device("cpu"))))
+               for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(got) == 2 and got[0] is got[1] is _kernel._err_words[torch.device("cpu")]
+
+
 def rows(shape=(2, 3, 2, 64), dtype=torch.float16):
     return torch.zeros(*shape, dtype=dtype)
 
