@@ -133,8 +133,11 @@ _err_words = {}
 def _err_word(device):
     t = _err_words.get(device)
     if t is None:
+        # an ordinary tensor also under inference_mode: check_device_errors clears it anywhere
+        with torch.inference_mode(False):
+            t = torch.zeros(1, dtype=torch.int32, device=device)
         # of two threads that come here at once, both get the word that the first put there
-        t = _err_words.setdefault(device, torch.zeros(1, dtype=torch.int32, device=device))
+        t = _err_words.setdefault(device, t)
     return t
 
 

@@ -726,6 +726,18 @@ def test_first_call_of_a_process_captured():
     assert r.returncode == 0 and "same" in r.stdout, r.stdout[-1000:] + r.stderr[-3000:]
 
 
+def test_reports_of_a_process_under_inference_mode(monkeypatch):
+    monkeypatch.setattr(_kernel, "_err_words", {})
+    cache, table, g = filled((40,), 16, 2, 64)
+    torch.cuda.synchronize()
+    _kernel._err_words.clear()
+    with torch.inference_mode():
+        q = torch.zeros(1, 1, 4, 64, device=DEV).half()
+        mfa.flash_attn_with_kv4cache(q, cache, torch.full_like(table, -1), i32(40))
+    reported()
+    _kernel.check_device_errors()  # and is quiet again
+
+
 def test_a_first_call_that_is_captured_still_reports():
     """Nothing but the cache was made before the capture."""
     import os

@@ -74,6 +74,16 @@ def test_two_threads_share_the_error_word(monkeypatch):
     assert len(got) == 2 and got[0] is got[1] is _kernel._err_words[torch.device("cpu")]
 
 
+def test_error_word_made_under_inference_mode(monkeypatch):
+    from mtlflashattn_b200 import _kernel
+    monkeypatch.setattr(_kernel, "_err_words", {})
+    with torch.inference_mode():
+        t = _kernel._err_word(torch.device("cpu"))
+    t.fill_(_lib.ERR_INVALID)
+    t.zero_()  # as check_device_errors does, outside of that mode
+    assert t.item() == 0
+
+
 def rows(shape=(2, 3, 2, 64), dtype=torch.float16):
     return torch.zeros(*shape, dtype=dtype)
 
