@@ -106,8 +106,8 @@ __device__ __forceinline__ void load_eight(const void* p, int64_t i, int fp32, i
 }
 
 // Any head dim, strides and rotation width: one warp per head row, one value per lane and step. Not
-// made for speed: 16384 tokens, 32/8 heads, bf16, D = 128 in unaligned rows 365 us (0.94 TB/s), D = 80
-// with R = 40 in split halves 296 us (the vector kernel, interleaved: 57).
+// made for speed: 16384 tokens, 32/8 heads, bf16, D = 128 in unaligned rows 365 us (0.94 TB/s),
+// D = 80 with R = 40 in split halves 296 us (the vector kernel, interleaved: 57).
 template <typename T>
 __global__ void __launch_bounds__(128) norm_rope_any(const __grid_constant__ NormRopeArgs a) {
   const int H = a.Hq + a.Hkv;

@@ -238,8 +238,8 @@ def flash_attn_with_kv4cache(q, cache, block_table, cache_seqlens, softmax_scale
     columns for). More than 48 query rows per KV head (16 at D = 64) are attended by way of keys and
     values in 16 bits: time and workspace of such calls follow this bound, not the lengths, so give
     it where the table is much wider than they are (the workspace, up to 512 MiB or one sequence's
-    bound where that is more, is kept for the stream's next calls). A longer sequence is cut after the page of
-    the bound's last token and reported by ``check_device_errors``.
+    bound where that is more, is kept for the stream's next calls). A longer sequence is cut after
+    the page of the bound's last token and reported by ``check_device_errors``.
     """
     if q.dim() != 4:
         raise ValueError(f"mtlflashattn_b200: expected 4-D [B,S,H,D] q, got q.dim()={q.dim()}")
